@@ -9,6 +9,8 @@
 // generated and the vocabulary entry, never on the batch: a request draws the same
 // tokens alone or beside others.  u = (23 random bits + 0.5) / 2^23 is exact in fp32
 // and lies strictly inside (0, 1), so g = -log(-log(u)) is finite.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 __device__ __forceinline__ unsigned long long mix64(unsigned long long z) {
@@ -161,6 +163,417 @@ PYRE_API int pyre_sample(const float* logits, long long ld, const float* tempera
     }
     const int threads = V >= 8192 ? 1024 : (V >= 1024 ? 256 : 64);
     pyre_launch(sample_kernel, dim3(n_rows), dim3(threads), 0, stream, logits, ld, temperature, seeds, token_index, out, V);
+    PYRE_LAUNCH_CHECK();
+    return 0;
+}
+
+// ---------------------------------------------------------------------------
+// Sampling from the likeliest tokens of a row (temperature > 0):
+//   w_i = exp((l_i - max l) / T); the order of the tokens: larger l first, of equal ones the lower index.
+//   top_k  > 0 : the first k tokens            (0: all)
+//   top_p  < 1 : of those the shortest prefix whose mass is at least p of theirs, one token at least
+//   min_p  > 0 : of those the tokens with w_i >= min_p
+// All three keep a prefix of the order.  The token is argmax over it of (l_i - max l) / T + g(seed, index, i), the noise of the kernels
+// above.  A row without a filter is chosen from as above, bit for bit; a NaN counts as -inf.
+//
+// A cluster of CTAs shares a row; each keeps its slice in shared memory, so the row is read from memory once.  Masses are whole numbers
+// (w 2^31, summed in 64 bits), so neither the order of the additions nor the cluster's size can move a border: results do not depend on them.
+//   1. max l.
+//   2. a histogram by distance from it in steps of 1/64 (count and mass per step; l decides the step alone and in order): the step in which
+//      the k-th token or the p-th part of the mass lies.
+//   3. that step's tokens, a few hundred as a rule, go to one CTA's list and are ranked by (l, index): the border token.  If they are more than
+//      the list holds, their span of (l, index) is cut into as many steps again, until they fit.
+//   4. noise for the tokens up to the border.
+// ---------------------------------------------------------------------------
+namespace {
+namespace cg = cooperative_groups;
+typedef unsigned long long u64;
+constexpr int F_THREADS = 512, F_WARPS = F_THREADS / 32, BINS = 2048, LISTED = 512, MAX_CLUSTER = 8;
+constexpr float BINS_PER_NAT = 64.f;
+
+struct FilterParams {
+    const float* logits;
+    long long ld;
+    const float* temperature;
+    const u64* seeds;
+    const int* token_index;
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    int* out;
+    int V, slice;      // entries per CTA, a multiple of 4
+    int resident;      // the slice lies in shared memory
+};
+
+struct FilterShared {
+    unsigned count[BINS], low[BINS], high[BINS];      // mass: high 2^32 + low
+    u64 list[LISTED];
+    unsigned list_mass[LISTED];
+    u64 slots[2][MAX_CLUSTER][2];                     // what the cluster's CTAs tell each other
+    u64 warp_u64[2][F_WARPS];
+    Best warp_best[F_WARPS];
+    Best cluster_best[MAX_CLUSTER];
+    // the step that a search ended in (`above`: before it), or the border
+    int step;
+    u64 above_count, above_mass, inside, border, border_mass;
+    unsigned listed;
+};
+
+// A number whose order as an unsigned integer is that of the floats (-0 and +0 are one).
+__device__ __forceinline__ unsigned order_key(float l) {
+    const unsigned u = __float_as_uint(l + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float entry(float l) { return l == l ? l : -INFINITY; }
+
+__global__ void __launch_bounds__(F_THREADS)
+sample_filtered_kernel(const FilterParams p) {
+    extern __shared__ float4 dyn[];
+    __shared__ FilterShared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int r = blockIdx.x / C;
+    pdl_trigger();
+    cluster.sync();      // the others have started: their shared memory can be written to
+    pdl_wait();
+    const float* row = p.logits + (size_t)r * p.ld;
+    const int begin = min(rank * p.slice, p.V), n = min(p.slice, p.V - begin);
+    const float T = p.temperature ? p.temperature[r] : 0.f;
+    const bool greedy = !(T > 0.f);
+    const float inv_t = greedy ? 1.f : 1.0f / T;
+    const u64 seed = p.seeds ? p.seeds[r] : 0ull;
+    const unsigned tix = p.token_index ? (unsigned)p.token_index[r] : 0u;
+    const int k = p.top_k ? p.top_k[r] : 0;
+    const float top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p ? fminf(p.min_p[r], 1.f) : 0.f;
+    const bool by_count = k > 0 && k < p.V, by_mass = top_p < 1.f;
+    const bool filtered = !greedy && (k > 0 || by_mass || min_p > 0.f);
+
+    int turn = 0;
+    // every CTA's pair of numbers, known to all threads of the cluster afterwards in sh.slots[returned]
+    auto exchange = [&](u64 a, u64 b) {      // a, b: in the first C threads
+        const int at = turn;
+        turn ^= 1;
+        if (tid < C) {
+            FilterShared* other = cluster.map_shared_rank(&sh, tid);
+            other->slots[at][rank][0] = a;
+            other->slots[at][rank][1] = b;
+        }
+        cluster.sync();
+        return at;
+    };
+    auto finish = [&](Best best) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.score, o), __shfl_xor_sync(0xffffffffu, best.index, o)});
+        if (lane == 0) sh.warp_best[warp] = best;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < F_WARPS; ++w) best = better(best, sh.warp_best[w]);
+            cluster.map_shared_rank(&sh, 0)->cluster_best[rank] = best;
+        }
+        cluster.sync();
+        if (rank == 0 && tid == 0) {
+            for (int c = 1; c < C; ++c) best = better(best, sh.cluster_best[c]);
+            p.out[r] = best.index == 0x7fffffff ? 0 : best.index;
+        }
+    };
+    Best best{-INFINITY, 0x7fffffff};
+    if (!filtered) {
+        for (int i = tid; i < n; i += F_THREADS) {
+            float s = entry(row[begin + i]);
+            if (!greedy) s = __fadd_rn(__fmul_rn(s, inv_t), gumbel(seed, tix, (unsigned)(begin + i)));
+            if (s > best.score || best.index == 0x7fffffff) best = Best{s, begin + i};
+        }
+        finish(best);
+        return;
+    }
+
+    // 1. the slice, and the largest entry
+    const float* held = row + begin;
+    float most = -INFINITY;
+    {
+        const float* src = row + begin;
+        const int shift = (int)(((uintptr_t)src >> 2) & 3), head = min(n, (4 - shift) & 3), body = (n - head) / 4;
+        float* mine = reinterpret_cast<float*>(dyn) + shift;      // the same place within 16 bytes
+        auto take = [&](int i) {
+            const float l = entry(src[i]);
+            most = fmaxf(most, l);
+            if (p.resident) mine[i] = l;
+        };
+        if (tid < head) take(tid);
+        for (int i = tid; i < body; i += F_THREADS) {
+            float4 v = *reinterpret_cast<const float4*>(src + head + 4 * i);
+            v = make_float4(entry(v.x), entry(v.y), entry(v.z), entry(v.w));
+            most = fmaxf(most, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+            if (p.resident) *reinterpret_cast<float4*>(mine + head + 4 * i) = v;
+        }
+        if (head + 4 * body + tid < n) take(head + 4 * body + tid);
+        if (p.resident) held = mine;
+    }
+    most = warp_max(most);
+    if (lane == 0) sh.warp_best[warp].score = most;
+    for (int b = tid; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    if (tid < C)
+        for (int w = 0; w < F_WARPS; ++w) most = fmaxf(most, sh.warp_best[w].score);
+    {
+        const int at = exchange(__float_as_uint(most), 0);
+        for (int c = 0; c < C; ++c) most = fmaxf(most, __uint_as_float((unsigned)sh.slots[at][c][0]));
+    }
+    // (the distance of the largest entry is zero even where it is infinite or the temperature's inverse is)
+    auto distance = [&](float l) { return l == most ? 0.f : (most - l) * inv_t; };
+    auto mass_of = [&](float d) { return __float2uint_rn(expf(-d) * 2147483648.f); };
+    auto first_step = [&](float d) { return (int)fminf(d * BINS_PER_NAT, (float)(BINS - 1)); };
+    auto composite = [&](float l, int i) { return (u64)order_key(l) << 32 | (unsigned)~(unsigned)(begin + i); };
+    auto tally = [&](int b, unsigned f) {
+        atomicAdd(&sh.count[b], 1u);
+        const unsigned old = atomicAdd(&sh.low[b], f);
+        if (old + f < old) atomicAdd(&sh.high[b], 1u);
+    };
+
+    // Adds up the cluster's histograms and finds the step in which the sum (of counts or masses) reaches `target`: sh.step, .above_*, .inside in every
+    // CTA.  Each CTA adds up a run of steps.  target 0: only the whole mass is wanted (returned).
+    auto locate = [&](bool mass, u64 target, u64 before_count, u64 before_mass, bool add) {
+        const int run = BINS / C, per = (run + F_THREADS - 1) / F_THREADS, first = rank * run;
+        cluster.sync();
+        if (add && C > 1) {
+            for (int b = first + tid; b < first + run; b += F_THREADS) {
+                u64 sum = ((u64)sh.high[b] << 32) + sh.low[b];
+                unsigned count = sh.count[b];
+                for (int c = 1; c < C; ++c) {
+                    const FilterShared* other = cluster.map_shared_rank(&sh, (rank + c) % C);
+                    sum += ((u64)other->high[b] << 32) + other->low[b];
+                    count += other->count[b];
+                }
+                sh.high[b] = (unsigned)(sum >> 32);
+                sh.low[b] = (unsigned)sum;
+                sh.count[b] = count;
+            }
+            __syncthreads();
+        }
+        // a thread's own steps, then the threads before it
+        u64 counts = 0, masses = 0;
+        for (int q = 0; q < per; ++q) {
+            const int b = tid * per + q;
+            if (b < run) {
+                counts += sh.count[first + b];
+                masses += ((u64)sh.high[first + b] << 32) + sh.low[first + b];
+            }
+        }
+        u64 c_up = counts, m_up = masses;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 a = __shfl_up_sync(0xffffffffu, c_up, o), b = __shfl_up_sync(0xffffffffu, m_up, o);
+            if (lane >= o) { c_up += a; m_up += b; }
+        }
+        if (lane == 31) { sh.warp_u64[0][warp] = c_up; sh.warp_u64[1][warp] = m_up; }
+        __syncthreads();
+        u64 c_all = 0, m_all = 0;
+        for (int w = 0; w < F_WARPS; ++w) {
+            if (w == warp) { c_up += c_all; m_up += m_all; }
+            c_all += sh.warp_u64[0][w];
+            m_all += sh.warp_u64[1][w];
+        }
+        const int at = exchange(c_all, m_all);
+        u64 c_before = before_count, m_before = before_mass, m_whole = before_mass;
+        for (int c = 0; c < C; ++c) {
+            if (c < rank) { c_before += sh.slots[at][c][0]; m_before += sh.slots[at][c][1]; }
+            m_whole += sh.slots[at][c][1];
+        }
+        if (target == 0) return m_whole;
+        u64 c_at = c_before + c_up - counts, m_at = m_before + m_up - masses;      // before the thread's own
+        if ((mass ? m_at : c_at) < target && (mass ? m_at + masses : c_at + counts) >= target) {
+            int b = tid * per;
+            for (;; ++b) {
+                const u64 c = sh.count[first + b], m = ((u64)sh.high[first + b] << 32) + sh.low[first + b];
+                if ((mass ? m_at + m : c_at + c) >= target) {
+                    for (int q = 0; q < C; ++q) {
+                        FilterShared* other = cluster.map_shared_rank(&sh, q);
+                        other->step = first + b;
+                        other->above_count = c_at;
+                        other->above_mass = m_at;
+                        other->inside = c;
+                    }
+                    break;
+                }
+                c_at += c;
+                m_at += m;
+            }
+        }
+        cluster.sync();
+        return m_whole;
+    };
+    // From the first histogram (already added up where !add) to the border token: sh.border and, with everything before it, its mass, in every CTA.
+    auto search = [&](bool mass, u64 target, bool add) {
+        locate(mass, target, 0, 0, add);
+        const int step0 = sh.step;
+        u64 from = 0, to = ~0ull;      // the span of (l, index) left
+        auto inside = [&](float l, int i) {
+            const u64 key = composite(l, i);
+            return first_step(distance(l)) == step0 && key >= from && key <= to;
+        };
+        bool spanned = false;
+        for (int level = 0; sh.inside > LISTED && level < 7; ++level) {      // 64 bits, eleven a time
+            if (!spanned) {
+                u64 low = ~0ull, high = 0;
+                for (int i = tid; i < n; i += F_THREADS)
+                    if (inside(held[i], i)) {
+                        low = min(low, composite(held[i], i));
+                        high = max(high, composite(held[i], i));
+                    }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+                    high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
+                }
+                __syncthreads();
+                if (lane == 0) { sh.warp_u64[0][warp] = low; sh.warp_u64[1][warp] = high; }
+                __syncthreads();
+                for (int w = 0; w < F_WARPS; ++w) {
+                    low = min(low, sh.warp_u64[0][w]);
+                    high = max(high, sh.warp_u64[1][w]);
+                }
+                const int at = exchange(low, high);
+                for (int c = 0; c < C; ++c) {
+                    low = min(low, sh.slots[at][c][0]);
+                    high = max(high, sh.slots[at][c][1]);
+                }
+                from = low;
+                to = high;
+                spanned = true;
+            }
+            int shift = 0;
+            while ((to - from) >> shift >= BINS) ++shift;
+            const u64 before_count = sh.above_count, before_mass = sh.above_mass;
+            cluster.sync();      // all have read the last histogram and what it gave
+            for (int b = tid; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += F_THREADS) {
+                const float l = held[i];
+                if (inside(l, i)) tally((int)((to - composite(l, i)) >> shift), mass_of(distance(l)));
+            }
+            locate(mass, target, before_count, before_mass, true);
+            to -= (u64)sh.step << shift;
+            from = max(from, to - ((1ull << shift) - 1));
+        }
+        // the tokens of the span, ranked by the first CTA
+        FilterShared* const lead = cluster.map_shared_rank(&sh, 0);
+        for (int i = tid; i < n; i += F_THREADS) {
+            const float l = held[i];
+            if (inside(l, i)) {
+                const unsigned at = atomicAdd(&lead->listed, 1u);
+                if (at < LISTED) {
+                    lead->list[at] = composite(l, i);
+                    lead->list_mass[at] = mass_of(distance(l));
+                }
+            }
+        }
+        cluster.sync();
+        if (rank == 0) {
+            const int count = min((int)sh.listed, LISTED);
+            for (int q = tid; q < count; q += F_THREADS) {
+                const u64 key = sh.list[q], own = sh.list_mass[q];
+                u64 c_at = sh.above_count, m_at = sh.above_mass;
+                for (int j = 0; j < count; ++j)
+                    if (sh.list[j] > key) { ++c_at; m_at += sh.list_mass[j]; }
+                if (mass ? m_at < target && m_at + own >= target : c_at + 1 == target)
+                    for (int c = 0; c < C; ++c) {
+                        FilterShared* other = cluster.map_shared_rank(&sh, c);
+                        other->border = key;
+                        other->border_mass = m_at + own;
+                    }
+            }
+            __syncthreads();
+            if (tid == 0) sh.listed = 0;
+        }
+        cluster.sync();
+    };
+
+    u64 border = 0;
+    if (most == -INFINITY) {
+        if (rank == 0 && tid == 0) p.out[r] = 0;      // nothing left to choose from
+        cluster.sync();
+        return;
+    }
+    if (by_count || by_mass) {
+        auto histogram = [&]() {
+            for (int i = tid; i < n; i += F_THREADS) {
+                const float d = distance(held[i]);
+                tally(first_step(d), mass_of(d));
+            }
+        };
+        histogram();
+        u64 whole = 0;
+        bool added = false;
+        if (by_count) {
+            search(false, (u64)k, true);
+            border = sh.border;
+            whole = sh.border_mass;
+            if (by_mass) {      // the first histogram again (the search may have cut it into finer steps)
+                __syncthreads();
+                for (int b = tid; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
+                __syncthreads();
+                histogram();
+            }
+        } else {
+            whole = locate(true, 0, 0, 0, true);
+            added = true;
+        }
+        if (by_mass) {
+            search(true, max(1ull, (u64)ceil((double)top_p * (double)whole)), !added);
+            border = sh.border;
+        }
+    }
+    for (int i = tid; i < n; i += F_THREADS) {
+        const float l = held[i];
+        if (composite(l, i) < border) continue;
+        const float d = distance(l);
+        if (min_p > 0.f && !(expf(-d) >= min_p)) continue;
+        const float s = entry(__fadd_rn(-d, gumbel(seed, tix, (unsigned)(begin + i))));
+        if (s > best.score || best.index == 0x7fffffff) best = Best{s, begin + i};
+    }
+    finish(best);
+}
+}  // namespace
+
+// logits [R, V] fp32 with row stride ld; temperature [R], seeds [R], token_index [R] (null where all rows are greedy); top_k [R] int32 (0: all), top_p [R]
+// (1: all), min_p [R] (0: all), each may be null; out [R] int32.
+PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float* temperature, const unsigned long long* seeds,
+                                  const int* token_index, const int* top_k, const float* top_p, const float* min_p, int* out, int n_rows,
+                                  int V, cudaStream_t stream) {
+    if (n_rows <= 0) return 0;
+    if (V <= 0 || (temperature && (!seeds || !token_index))) return PYRE_ERR_BAD_ARG;
+    // CTAs per row: as many as keep two to an SM busy, and as two slices in an SM's shared memory ask for
+    int C = 1;
+    while (C < MAX_CLUSTER && ((n_rows * (long long)C < 2 * pyre_sm_count() && V > 2048 * C) || ceil_div(V, C) > 76 * 256)) C *= 2;
+    FilterParams p = {logits, ld, temperature, seeds, token_index, top_k, top_p, min_p, out, V, (ceil_div(V, C) + 3) / 4 * 4, 0};
+    size_t bytes = (size_t)p.slice * 4 + 16;
+    p.resident = bytes <= 190 * 1024;
+    if (!p.resident) bytes = 0;
+    static bool configured[PYRE_MAX_DEVICES] = {};      // the attribute is per device
+    bool& done = configured[pyre_current_device()];
+    if (!done) {
+        const cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 190 * 1024);
+        if (e != cudaSuccess) return (int)e;
+        done = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n_rows * C);
+    cfg.blockDim = dim3(F_THREADS);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pyre_pdl_enabled() ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_filtered_kernel, p);
+    if (e != cudaSuccess) return (int)e;
     PYRE_LAUNCH_CHECK();
     return 0;
 }

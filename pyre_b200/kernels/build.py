@@ -44,6 +44,8 @@ LIBRARIES = {
     "wkv": "wkv.cu",
     "seqmix": "seqmix.cu",
     "matrix_state": "matrix_state.cu",
+    "rows8": "rows8.cu",
+    "gemm_w4": "gemm_w4.cu",
 }
 
 HEADERS = ["common.cuh", "tensor_core.cuh", "attention_mma_noalloc.h"]

@@ -38,6 +38,7 @@ SIGNATURES: dict[str, tuple[str, list]] = {
     "pyre_scale_rows": ("elementwise", [P, P, I, P, I, I, F, P]),
     "pyre_sample": ("sampling", [P, LL, P, P, P, P, I, I, P, P]),
     "pyre_sample_slices": ("sampling", [I]),
+    "pyre_sample_filtered": ("sampling", [P, LL, P, P, P, P, P, P, P, I, I, P]),
     "pyre_paged_attention_generic": ("attention_generic", [P, P, P, P, I, P, P, I, I, I, I, I, I, I, F, F, P, I, LL, P, I, I, P]),
     "pyre_sgemm_nt": ("gemm_f32", [P, LL, P, LL, P, LL, P, I, I, I, P]),
     "pyre_fixed_exponents": ("gemm_fixed", [P, LL, I, I, P, P, P]),
@@ -87,6 +88,12 @@ SIGNATURES: dict[str, tuple[str, list]] = {
     "pyre_rotate_heads": ("seqmix", [P, LL, I, P, P, I, I, I, I, F, I, P]),
     "pyre_side_gate": ("seqmix", [P, P, LL, I, P, I, P, I, I, I, P, P]),
     "pyre_token_gate_add": ("seqmix", [P, P, P, P, I, I, I, I, P]),
+    "pyre_norm_rows8": ("rows8", [P, P, P, I, LL, P, P, P, P, I, I, F, I, I, P]),
+    "pyre_rows8": ("rows8", [P, LL, P, P, I, I, I, I, F, I, P]),
+    "pyre_rows8_values": ("rows8", [P, P, LL, P, I, I, I, P]),
+    "pyre_w4_quantize": ("gemm_w4", [P, LL, P, P, I, I, I, P]),
+    "pyre_w4_values": ("gemm_w4", [P, P, P, I, I, I, P]),
+    "pyre_w4_linear": ("gemm_w4", [P, P, LL, P, P, P, I, I, I, I, P]),
 }
 
 #: functions that return a number of another type than int (sizes; see ``call_value``)
@@ -106,7 +113,9 @@ class KernelError(RuntimeError):
 DEFAULT_CLASS = {
     "pyre_embedding": "embed", "pyre_add_rmsnorm": "norm", "pyre_add_residual": "norm", "pyre_rope_table": "rotary+write",
     "pyre_qkv_rope_write": "rotary+write", "pyre_silu_mul": "activation", "pyre_sum_partials": "sum_partials",
-    "pyre_feed_tokens": "feed", "pyre_delay": "delay", "pyre_gemm_tc": "product", "pyre_sgemm_nt": "product", "pyre_fixed_linear": "product", "pyre_scale_rows": "norm", "pyre_sample": "sampler",
+    "pyre_feed_tokens": "feed", "pyre_delay": "delay", "pyre_gemm_tc": "product", "pyre_sgemm_nt": "product", "pyre_fixed_linear": "product", "pyre_scale_rows": "norm", "pyre_sample": "sampler", "pyre_sample_filtered": "sampler",
+    "pyre_norm_rows8": "norm", "pyre_rows8": "activation", "pyre_rows8_values": "activation", "pyre_w4_quantize": "load", "pyre_w4_values": "load",
+    "pyre_w4_linear": "product",
     "pyre_paged_attention_generic": "attention", "pyre_paged_attention_mma": "attention",
     "pyre_attention_prefill_tc": "attention", "pyre_attention_prefill": "attention",
     "pyre_cast_rows": "norm", "pyre_norm_add": "norm", "pyre_activation": "activation", "pyre_qk_norm_rope_write": "rotary+write",

@@ -125,14 +125,80 @@ class NormedBranch:
         return out if self.dtype == torch.float32 else PartialSums(out.unsqueeze(0), self.dtype)
 
 
+GROUP8 = 128      # neighbouring elements that share a scale, of rows in 8 bits and of weights in 4
+
+
+class Rows8:
+    """Activations in 8 bits (csrc/rows8.cu): ``rows`` int8 [T, 128 G], zeros beyond ``width`` elements, and ``scales`` float32 [G, T], one per
+    128 neighbouring elements of a row (G = ceil(width / 128)): element i of token t stands for ``rows[t, i] * scales[i // 128, t]``.  A
+    product with a ``Weight4`` reads them as they are; anything else calls ``materialize``, which rounds to ``dtype``."""
+
+    def __init__(self, rows: torch.Tensor, scales: torch.Tensor, width: int, dtype: torch.dtype = torch.bfloat16):
+        groups = -(-width // GROUP8)
+        if rows.dtype != torch.int8 or rows.dim() != 2 or rows.shape[1] != groups * GROUP8 or width <= 0:
+            raise ValueError(f"rows of {width} elements in 8 bits are int8 [T, {groups * GROUP8}], got {rows.dtype} {tuple(rows.shape)}")
+        if scales.dtype != torch.float32 or tuple(scales.shape) != (groups, rows.shape[0]):
+            raise ValueError(f"scales must be float32 {(groups, rows.shape[0])}, got {scales.dtype} {tuple(scales.shape)}")
+        self.rows, self.scales, self.width, self.dtype = rows, scales, width, dtype
+
+    @property
+    def shape(self):
+        return torch.Size((self.rows.shape[0], self.width))
+
+    @property
+    def device(self):
+        return self.rows.device
+
+
+class Weight4:
+    """A weight [N, K] in 4 bits with a bfloat16 scale per 128 neighbouring elements of a feature (csrc/gemm_w4.cu; ``quantize_weight4``):
+    ``packed`` uint8 [N, 64 G], zeros beyond K, and ``scales`` [G, N] (G = ceil(K / 128)).  Of every four bytes, which hold eight elements,
+    byte i holds element i in its lower half and element i + 4 in its upper one, two's complement -8 .. 7; an element stands for itself
+    times its group's scale."""
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, width: int):
+        groups = -(-width // GROUP8)
+        if packed.dtype != torch.uint8 or packed.dim() != 2 or packed.shape[1] != groups * (GROUP8 // 2) or width <= 0:
+            raise ValueError(f"a weight of {width} columns in 4 bits is uint8 [N, {groups * GROUP8 // 2}], got {packed.dtype} {tuple(packed.shape)}")
+        if scales.dtype != torch.bfloat16 or tuple(scales.shape) != (groups, packed.shape[0]):
+            raise ValueError(f"scales must be bfloat16 {(groups, packed.shape[0])}, got {scales.dtype} {tuple(scales.shape)}")
+        for t, name in ((packed, "packed"), (scales, "scales")):
+            if not t.is_cuda or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous CUDA tensor")
+        if packed.data_ptr() % 16:
+            raise ValueError("packed must start on a 16-byte boundary")
+        self.packed, self.scales, self.width = packed, scales, width
+
+    @property
+    def shape(self):
+        return torch.Size((self.packed.shape[0], self.width))
+
+    @property
+    def device(self):
+        return self.packed.device
+
+    def values(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The weight as a plain tensor [N, K]."""
+        require_current_device(self.device, "the weight")
+        out = torch.empty(tuple(self.shape), dtype=dtype, device=self.device)
+        lib.call("pyre_w4_values", self.packed.data_ptr(), self.scales.data_ptr(), out.data_ptr(), out.shape[0], out.shape[1], _dt(dtype), _stream())
+        return out
+
+
 def formed(t):
     """A pending branch output without the forms that only some consumers know."""
     return t.formed() if isinstance(t, NormedBranch) else materialize(t) if isinstance(t, BiasedRows) else t
 
 
-def materialize(t: "torch.Tensor | PartialSums | DeferredProduct | ScaledRows | ScaledSum | BiasedRows | NormedBranch") -> torch.Tensor:
+def materialize(t: "torch.Tensor | PartialSums | DeferredProduct | ScaledRows | ScaledSum | BiasedRows | NormedBranch | Rows8") -> torch.Tensor:
     """A plain tensor in the activation dtype from a tensor or any of the lazy forms a branch output or a
     norm's output may take."""
+    if isinstance(t, Rows8):
+        _check_rows8(t)
+        T, K = t.shape
+        out = torch.empty((T, K), dtype=t.dtype, device=t.rows.device)
+        lib.call("pyre_rows8_values", t.rows.data_ptr(), t.scales.data_ptr(), t.scales.stride(0), out.data_ptr(), T, K, _dt(t.dtype), _stream())
+        return out
     if isinstance(t, NormedBranch):
         t = t.formed()
     if isinstance(t, BiasedRows):
@@ -305,6 +371,109 @@ def add_rmsnorm(x: torch.Tensor, delta: "torch.Tensor | None", weight: torch.Ten
     return out
 
 
+def _check_rows8(x: Rows8) -> None:
+    if not x.rows.is_cuda or not x.scales.is_cuda or x.scales.device != x.rows.device:
+        raise ValueError("rows in 8 bits and their scales must lie on one CUDA device (pyre_b200 has no CPU path)")
+    require_current_device(x.rows.device, "x")
+    if not x.rows.is_contiguous() or x.rows.data_ptr() % 16 or (x.scales.shape[1] > 1 and x.scales.stride(1) != 1):
+        raise ValueError("rows in 8 bits must be contiguous and start on a 16-byte boundary, their scales contiguous along the tokens")
+
+
+def _rows8_out(T: int, width: int, device, dtype: torch.dtype) -> Rows8:
+    groups = -(-width // GROUP8)
+    return Rows8(torch.empty((T, groups * GROUP8), dtype=torch.int8, device=device), torch.empty((groups, T), dtype=torch.float32, device=device),
+                 width, dtype)
+
+
+def add_rmsnorm_rows8(x: torch.Tensor, delta: "torch.Tensor | PartialSums | DeferredProduct | None", weight: torch.Tensor, eps: float,
+                      dtype: torch.dtype = torch.bfloat16, rows: "torch.Tensor | None" = None, update_x: bool = True) -> Rows8:
+    """``add_rmsnorm`` with its result in 8 bits: ``Rows8`` of rmsnorm(x[src] + delta[src]) * weight, src = rows[r] (or r).  ``x`` is the
+    fp32 residual stream and takes the sum as there; ``delta`` has the activation dtype ``dtype`` or is a lazy form of a branch output.
+    Each 128 neighbouring elements of a row share the scale max |.| / 127, so the values are off by at most half of it: the norm is
+    not rounded to ``dtype`` in between."""
+    delta = formed(delta)
+    _check(x, "x", torch.float32, 2)
+    _check(weight, "weight", torch.float32, 1)
+    T, H = x.shape
+    if weight.shape[0] != H:
+        raise ValueError(f"norm weight has {weight.shape[0]} entries, rows have {H}")
+    if delta is not None and tuple(delta.shape) != (T, H):
+        raise ValueError(f"delta shape {tuple(delta.shape)} != x shape {(T, H)}")
+    if isinstance(delta, DeferredProduct):
+        delta = delta.partials()
+    parts, n_parts = None, 0
+    if isinstance(delta, PartialSums):
+        parts, n_parts, delta = delta.parts, delta.n, None
+    elif delta is not None:
+        _check(delta, "delta", dtype, 2)
+    n_rows = T
+    if rows is not None:
+        _check(rows, "rows", torch.int32, 1)
+        n_rows = rows.shape[0]
+        update_x = False
+    out = _rows8_out(n_rows, H, x.device, dtype)
+    lib.call("pyre_norm_rows8", x.data_ptr(), _ptr(delta), _ptr(parts), n_parts, T * H, weight.data_ptr(), out.rows.data_ptr(), out.scales.data_ptr(),
+             _ptr(rows), n_rows, H, float(eps), int(bool(update_x and (delta is not None or parts is not None))), _dt(dtype), _stream())
+    return out
+
+
+def quantize_rows8(x: torch.Tensor) -> Rows8:
+    """``Rows8`` of plain activations [T, K] (contiguous rows; bfloat16 or float32)."""
+    if not x.is_cuda or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or not x.shape[1]:
+        raise ValueError("x must be a CUDA matrix with contiguous rows")
+    require_current_device(x.device, "x")
+    T, K = x.shape
+    out = _rows8_out(T, K, x.device, x.dtype)
+    lib.call("pyre_rows8", x.data_ptr(), x.stride(0), out.rows.data_ptr(), out.scales.data_ptr(), T, K, 0, 0, 0.0, _dt(x.dtype), _stream())
+    return out
+
+
+def gate_rows8(gate_up: torch.Tensor, kind: str = "silu", limit: float = 0.0) -> Rows8:
+    """``Rows8`` of act(gate) * up for rows [T, 2 I] of [gates | ups]: ``silu_mul`` with its result in 8 bits (``kind``, ``limit``: see there)."""
+    _check(gate_up, "gate_up", dim=2)
+    T, two_i = gate_up.shape
+    if two_i % 2 or not two_i:
+        raise ValueError("gate_up must have an even number of columns")
+    if kind not in GATE_KINDS:
+        raise UnsupportedSize(f"gate activation {kind!r}: this kernel knows {sorted(GATE_KINDS)}")
+    out = _rows8_out(T, two_i // 2, gate_up.device, gate_up.dtype)
+    lib.call("pyre_rows8", gate_up.data_ptr(), two_i, out.rows.data_ptr(), out.scales.data_ptr(), T, two_i // 2, 1, {"silu": 0, "relu": 1, "clamped": 2}[kind],
+             float(limit), _dt(gate_up.dtype), _stream())
+    return out
+
+
+def quantize_weight4(w: torch.Tensor) -> Weight4:
+    """A weight [N, K] (bfloat16 or float32, contiguous rows) in 4 bits: per 128 neighbouring elements of a feature the scale is
+    bfloat16(max |w| / 7) and an element the nearest multiple of it within -8 .. 7."""
+    if not w.is_cuda or w.dim() != 2 or (w.shape[1] > 1 and w.stride(1) != 1) or not w.shape[1]:
+        raise ValueError("w must be a CUDA matrix with contiguous rows")
+    N, K = w.shape
+    groups = -(-K // GROUP8)
+    with torch.cuda.device(w.device):      # a model may be loaded while another device is current
+        packed = torch.empty((N, groups * GROUP8 // 2), dtype=torch.uint8, device=w.device)
+        scales = torch.empty((groups, N), dtype=torch.bfloat16, device=w.device)
+        lib.call("pyre_w4_quantize", w.data_ptr(), w.stride(0), packed.data_ptr(), scales.data_ptr(), N, K, _dt(w.dtype), _stream())
+    return Weight4(packed, scales, K)
+
+
+def linear4(x: "torch.Tensor | Rows8", w: Weight4, out_dtype: "torch.dtype | None" = None) -> torch.Tensor:
+    """y = x W^T for a weight in 4 bits: whole numbers summed exactly within a group, the groups in float32.  Activations that are
+    not in 8 bits yet go through ``quantize_rows8`` first."""
+    if not isinstance(x, Rows8):
+        x = quantize_rows8(materialize(x))
+    _check_rows8(x)
+    T, K = x.shape
+    N, K2 = w.shape
+    if K != K2:
+        raise ValueError(f"inner sizes differ: x is [{T}, {K}], w is [{N}, {K2}]")
+    require_current_device(w.packed.device, "w")
+    dtype = out_dtype or x.dtype
+    out = torch.empty((T, N), dtype=dtype, device=x.rows.device)
+    lib.call("pyre_w4_linear", x.rows.data_ptr(), x.scales.data_ptr(), x.scales.stride(0), w.packed.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
+             T, N, w.scales.shape[0], _dt(dtype), _stream())
+    return out
+
+
 def add_residual(x: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:
     """x += float32(delta) in place on the fp32 residual stream: for a block arrangement in which no
     norm follows a branch (the built-in pre-norm block adds its branches inside the next norm's kernel)."""
@@ -423,8 +592,14 @@ def delay(milliseconds: float) -> None:
 
 
 def sample(logits: torch.Tensor, temperature: "torch.Tensor | None" = None, seeds: "torch.Tensor | None" = None,
-           token_index: "torch.Tensor | None" = None, out: "torch.Tensor | None" = None) -> torch.Tensor:
-    """One token id per row of fp32 logits [R, V]: argmax where temperature is 0, else Gumbel-max."""
+           token_index: "torch.Tensor | None" = None, out: "torch.Tensor | None" = None, top_k: "torch.Tensor | None" = None,
+           top_p: "torch.Tensor | None" = None, min_p: "torch.Tensor | None" = None) -> torch.Tensor:
+    """One token id per row of fp32 logits [R, V]: argmax where temperature is 0, else Gumbel-max.
+
+    Where temperature is not 0, ``top_k`` (int32 [R], 0 = off), ``top_p`` (float32 [R], 1 = off) and ``min_p`` (float32 [R], 0 = off) leave
+    a row's likeliest tokens to choose from, in the order of the logits (the lower index first where they are equal): the first k; of
+    those the shortest run from the best on with at least p of their mass; of those the ones with at least min_p of the best
+    one's probability.  The best one always stays.  A row without any of them gets the same token with and without the arguments; a NaN counts as -inf."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda or logits.stride(1) != 1:
         raise ValueError("logits must be a CUDA float32 matrix with contiguous rows")
     R, V = logits.shape
@@ -438,6 +613,20 @@ def sample(logits: torch.Tensor, temperature: "torch.Tensor | None" = None, seed
             raise ValueError("temperature, seeds and token_index need one entry per row")
     if out is None:
         out = torch.empty((R,), dtype=torch.int32, device=logits.device)
+    if top_k is not None or top_p is not None or min_p is not None:
+        require_current_device(logits.device, "logits")
+        if temperature is None:
+            raise ValueError("top_k, top_p and min_p go with a temperature (0 for rows that take the best token)")
+        for t, name, dtype in ((top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32), (out, "out", torch.int32)):
+            if t is not None:
+                _check(t, name, dtype, 1)
+                if t.shape[0] != R:
+                    raise ValueError(f"{name} needs one entry per row")
+        if not V:
+            raise ValueError("rows of logits need an entry")
+        lib.call("pyre_sample_filtered", logits.data_ptr(), logits.stride(0), temperature.data_ptr(), seeds.data_ptr(), token_index.data_ptr(), _ptr(top_k),
+                 _ptr(top_p), _ptr(min_p), out.data_ptr(), R, V, _stream())
+        return out
     slices = lib.call_value("pyre_sample_slices", V)
     scratch = torch.empty(R * slices * 2, dtype=torch.int32, device=logits.device) if slices else None
     lib.call("pyre_sample", logits.data_ptr(), logits.stride(0), _ptr(temperature), _ptr(seeds), _ptr(token_index),
@@ -1269,7 +1458,13 @@ def linear(x: "torch.Tensor | ScaledRows", w: torch.Tensor, out_dtype: "torch.dt
     ``deferred_ok="residual"`` says that the consumer is the norm (the product is a branch output): then a product
     of many tokens in one split is deferred too, since its epilogue can fold the residual add (``folds_residual``).
     ``deferred_ok=("rope", head_dim)``: the consumer is a position encoding that may fold bias, rotation and the cache
-    write into the stacked q/k/v product (``folds_rope``)."""
+    write into the stacked q/k/v product (``folds_rope``).  A ``Weight4`` takes ``Rows8`` (other activations are put in 8 bits first); with
+    ``partials_ok`` its result stays unrounded, as one part."""
+    if isinstance(w, Weight4):
+        if partials_ok and out_dtype is None and x.dtype == torch.bfloat16:
+            return PartialSums(linear4(x, w, torch.float32).unsqueeze(0), torch.bfloat16)
+        return linear4(x, w, out_dtype)
+    x = materialize(x) if isinstance(x, Rows8) else x
     if x.dtype == torch.float32:
         return fixed_linear(x, w) if isinstance(w, FixedWeight) else sgemm_nt(x, w)
     if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
