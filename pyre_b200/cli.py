@@ -49,11 +49,11 @@ def cmd_generate(args) -> int:
     ec = EngineConfig(dtype=args.dtype, device=args.device, page_size=args.page_size, num_pages=args.num_pages,
                       cache_memory_fraction=args.cache_memory_fraction, lookahead=not args.no_lookahead,
                       max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_batched_tokens,
-                      prefill_chunk=args.prefill_chunk, record_steps=bool(args.step_log))
+                      prefill_chunk=args.prefill_chunk, record_steps=bool(args.step_log), weight_bits=args.weight_bits)
     print(f"loading {args.model} on {args.device} ...", file=sys.stderr)
     engine = Engine(args.model, ec)
     params = [SamplingParams(temperature=args.temperature, seed=args.seed + i, max_new_tokens=args.max_new_tokens,
-                             eos_id=args.eos_id) for i in range(len(prompts))]
+                             eos_id=args.eos_id, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p) for i in range(len(prompts))]
     torch.cuda.synchronize()
     t0 = time.perf_counter()
     outs = engine.generate(prompts, params)
@@ -104,6 +104,10 @@ def main(argv=None) -> int:
     g.add_argument("--max-new-tokens", type=int, default=128)
     g.add_argument("--temperature", type=float, default=0.0, help="0 = greedy")
     g.add_argument("--seed", type=int, default=0, help="sampling seed of the first prompt; prompt i uses seed + i")
+    g.add_argument("--top-k", type=int, default=0, help="draw from the k likeliest tokens (0 = all)")
+    g.add_argument("--top-p", type=float, default=1.0, help="draw from the likeliest tokens that hold this share of the probability (1 = all)")
+    g.add_argument("--min-p", type=float, default=0.0, help="draw from the tokens with at least this share of the likeliest one's probability (0 = all)")
+    g.add_argument("--weight-bits", type=int, choices=[4], default=None, help="hold the layers' projections in 4 bits (bfloat16 only)")
     g.add_argument("--eos-id", type=int, default=None)
     g.add_argument("--page-size", type=int, default=16, help="tokens per cache page")
     g.add_argument("--num-pages", type=int, default=None, help="pages of the cache pool")

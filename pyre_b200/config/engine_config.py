@@ -35,6 +35,9 @@ class EngineConfig:
     ``dtype``: ``bfloat16`` (weights and cache in bf16, fp32 accumulation, fp32
     softmax/norm/rotary/residual) or ``float32`` (every tensor and every product in
     IEEE fp32, no reduced-precision matrix mode).
+    ``weight_bits``: 4 = the layers' projections are held in 4 bits with a scale per 128 elements of a feature, put there
+    from the checkpoint's values at load, and read activations in 8 bits with a scale per 128 elements of a token (bfloat16
+    only; embedding, norms, biases, head and cache stay as they are); None = in ``dtype``.
     ``page_size``: tokens per cache page (the reference's BLOCK_SIZE).
     ``max_cache_tokens``: capacity of the paged pools in tokens; ``num_pages`` wins if set.
     ``cache_memory_fraction``: with neither of the two, size the pools to this fraction of the
@@ -59,6 +62,7 @@ class EngineConfig:
 
     dtype: "str | torch.dtype" = "bfloat16"
     device: str = "cuda:0"
+    weight_bits: int | None = None
     page_size: int = 16
     num_pages: int | None = None
     max_cache_tokens: int | None = None
@@ -76,6 +80,10 @@ class EngineConfig:
 
     def __post_init__(self):
         self.dtype = parse_dtype(self.dtype)
+        if self.weight_bits not in (None, 4):
+            raise ValueError(f"weight_bits must be 4 or None (weights in dtype), got {self.weight_bits!r}")
+        if self.weight_bits is not None and self.dtype != torch.bfloat16:
+            raise ValueError("weights in 4 bits go with dtype bfloat16")
         if self.page_size <= 0:
             raise ValueError("page_size must be positive")
         if self.cache_memory_fraction is not None and not 0.0 < self.cache_memory_fraction <= 1.0:

@@ -24,6 +24,7 @@ from ..cache import CacheManager, pages_per_group
 from ..config import EngineConfig, ModelConfig, architecture_of, load_config
 from ..kernels import build, lib
 from ..models.model import Model
+from ..models.spec import with_weight_bits
 from ..sampling import Sampler, SamplingParams
 from .scheduler import PENDING, Request, Scheduler, step_record
 from .step import StepEntry, Stepper
@@ -56,7 +57,7 @@ class Engine:
         if (model is None) == (config is None):
             raise ValueError("give either a model folder or config= with seed=")
         self.model_config = load_config(model) if model is not None else config
-        spec = architecture_of(self.model_config).build(self.model_config)
+        spec = with_weight_bits(architecture_of(self.model_config).build(self.model_config), ec.weight_bits)
         self.model = Model(spec, ec.dtype, ec.device)
         build.ensure_built(self.model.kernel_libraries())
         with torch.cuda.device(self.model.device):

@@ -1026,9 +1026,18 @@ def fixed_supported(w: torch.Tensor) -> bool:
             and w.stride(0) >= w.shape[1] and FIXED_MIN_K <= w.shape[1] <= FIXED_MAX_K and w.numel() >= FIXED_MIN_SIZE)
 
 
-def linear_weight(w: torch.Tensor) -> "torch.Tensor | FixedWeight":
-    """A weight as ``linear`` wants it: float32 matrices that the fixed-point product takes with their rows' exponents, others as
+def known_weight_bits(bits: "int | None") -> "int | None":
+    """``bits`` if there are products for weights of that many (None: in the compute dtype)."""
+    if bits not in (None, 4):
+        raise UnsupportedSize(f"weights of {bits} bits: 4, or None for the compute dtype")
+    return bits
+
+
+def linear_weight(w: torch.Tensor, bits: "int | None" = None) -> "torch.Tensor | FixedWeight | Weight4":
+    """A weight as ``linear`` wants it: with ``bits`` 4 a ``Weight4``; else float32 matrices that the fixed-point product takes with their rows' exponents, others as
     they are; so are those of which more than one feature in 64 has no scale (an element far above the rest of its row)."""
+    if bits == 4:
+        return quantize_weight4(w)
     if not fixed_supported(w):
         return w
     with torch.cuda.device(w.device):
@@ -1036,8 +1045,10 @@ def linear_weight(w: torch.Tensor) -> "torch.Tensor | FixedWeight":
         return fixed if int((fixed.exponents >= FIXED_NO_SCALE).sum()) <= w.shape[0] // 64 else w      # reading the number waits
 
 
-def product_libraries(dtype: torch.dtype) -> "list[str]":
+def product_libraries(dtype: torch.dtype, bits: "int | None" = None) -> "list[str]":
     """The kernel libraries that ``linear`` launches from for weights of ``linear_weight``."""
+    if bits == 4:
+        return ["gemm_w4", "rows8"]
     return ["gemm_f32", "gemm_fixed"] if dtype == torch.float32 else ["gemm_tc"]
 
 

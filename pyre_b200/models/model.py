@@ -13,7 +13,7 @@ from ..parts.base import (BoundCall, PagedKVSpec, StateSpec, all_graph_safe, col
                           load_part, make_part)
 from ..weights import loader, random_init
 from ..weights.specs import TensorSpec
-from .spec import ModelSpec
+from .spec import ModelSpec, with_weight_bits
 
 
 @dataclass(frozen=True)
@@ -180,16 +180,17 @@ class Model:
         return self.tail.forward(ctx, x, pending)
 
 
-def load_model(model_dir: "str | Path", device: str = "cuda:0", dtype="bfloat16"):
+def load_model(model_dir: "str | Path", device: str = "cuda:0", dtype="bfloat16", weight_bits: "int | None" = None):
     """A model folder (config.json + safetensors) -> (model with its weights on ``device``, its configuration):
     the reference's ``load_model(path, device, dtype)`` (pyre/loader.py:33-79).  The model class comes from
     the registry by the configuration's architecture name, and the kernel libraries this model and dtype
-    need are built if they are not there yet."""
-    from ..config import architecture_of, load_config, parse_dtype
+    need are built if they are not there yet.  ``weight_bits``: as in ``EngineConfig``."""
+    from ..config import EngineConfig, architecture_of, load_config
     from ..kernels import build
 
     config = load_config(model_dir)
-    model = Model(architecture_of(config).build(config), parse_dtype(dtype), device)
+    ec = EngineConfig(dtype=dtype, device=device, weight_bits=weight_bits)
+    model = Model(with_weight_bits(architecture_of(config).build(config), ec.weight_bits), ec.dtype, device)
     build.ensure_built(model.kernel_libraries())
     model.load_weights(model_dir)
     return model, config

@@ -2,9 +2,10 @@
 
 from __future__ import annotations
 
+import dataclasses
 from dataclasses import dataclass, field
 
-from ..parts.base import PartSpec
+from ..parts.base import PartSpec, takes_weight_bits
 
 
 @dataclass(frozen=True)
@@ -76,3 +77,23 @@ class ModelSpec:
                 raise ValueError("a model needs a tail: give final_norm and head, or tail")
             self.tail = PartSpec("norm_head", {"norm": self.final_norm, "head": self.head,
                                                "names": {"norm": self.final_norm_prefix, "head": self.head_prefix}})
+
+
+def with_weight_bits(spec: ModelSpec, bits: "int | None") -> ModelSpec:
+    """The same model with the products of its blocks' mixers and feed-forwards held in ``bits`` bits.  A model with a mixer or
+    feed-forward that has no such form is refused as a whole: some of its layers in 4 bits is not what was asked for."""
+    if bits is None:
+        return spec
+
+    def of(block: PartSpec) -> PartSpec:
+        params = dict(block.params)
+        for role in ("mixer", "ffn"):
+            part = params.get(role)
+            if part is None:
+                continue
+            if not takes_weight_bits(role, part.kind):
+                raise ValueError(f"weights in {bits} bits: the {role} part {part.kind!r} of this architecture has none")
+            params[role] = PartSpec(part.kind, {**part.params, "weight_bits": bits})
+        return PartSpec(block.kind, params)
+
+    return dataclasses.replace(spec, blocks=[of(b) for b in spec.blocks])

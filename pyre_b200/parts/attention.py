@@ -64,6 +64,8 @@ class Attention(StackedMixer):
     and rotation;
     ``weight_suffix`` / ``bias_suffix``: what follows a projection's name in the checkpoint (".weight", ".bias").
     With any of these the mixer is a ``StackedMixer``: it may also stand beside other mixers.
+
+    ``weight_bits``: 4 = the projections are held as ``ops.Weight4`` (without the parameters of the second list).
     """
 
     DEFAULT_NAMES = {"q": "q_proj", "k": "k_proj", "v": "v_proj", "o": "o_proj", "g": "g_proj", "q_norm": "q_norm.weight",
@@ -71,6 +73,7 @@ class Attention(StackedMixer):
 
     graph_safe = True
     takes_scaled_rows = True      # ``h`` may be ``ops.ScaledRows``: the q/k/v product applies the norm's 1/rms itself
+    takes_weight_bits = True
 
     def __init__(self, dtype, device, width: int, n_heads: int, n_kv_heads: int, head_dim: int,
                  position: "PartSpec | None" = None, qkv_bias: bool = True, o_bias: bool = False,
@@ -78,7 +81,7 @@ class Attention(StackedMixer):
                  v_head_dim: "int | None" = None, qk_norm: "dict | None" = None, sink: "float | None" = None,
                  out_gate: "bool | str" = False, own_kv: bool = True, weight_suffix: str = ".weight",
                  value_position: "PartSpec | None" = None, keep_first: int = 0, qk_unit: "dict | None" = None,
-                 value_is_key: bool = False, bias_suffix: str = ".bias"):
+                 value_is_key: bool = False, bias_suffix: str = ".bias", weight_bits: "int | None" = None):
         super().__init__(dtype, device)
         self.value_is_key, self.bias_suffix, self.has_o_bias = bool(value_is_key), str(bias_suffix), bool(o_bias)
         if self.value_is_key and (not own_kv or (v_head_dim is not None and int(v_head_dim) != int(head_dim))):
@@ -105,6 +108,11 @@ class Attention(StackedMixer):
                         or self.value_position is not None or self.learned_sink or qk_unit is not None
                         or self.value_is_key or self.has_o_bias
                         or (position is not None and position.params.get("pairing") == "interleaved"))
+        self.weight_bits = ops.known_weight_bits(weight_bits)
+        if self.weight_bits is not None:
+            if self.general:
+                raise ops.UnsupportedSize("projections in 4 bits: plain attention only (one head size, no gate, norm, sink or bias of its own)")
+            self.takes_scaled_rows, self.takes_rows8 = False, True
         self.names = dict(self.DEFAULT_NAMES, **(names or {}))
         self.width, self.n_heads, self.n_kv_heads, self.head_dim = int(width), int(n_heads), int(n_kv_heads), int(head_dim)
         if self.n_heads % self.n_kv_heads:
@@ -184,17 +192,17 @@ class Attention(StackedMixer):
             if self.learned_sink:
                 self.sink = tensors[n["sink"]]
             return
-        self.w_qkv = ops.linear_weight(torch.cat([tensors[f"{n[k]}.weight"] for k in "qkv"], dim=0).contiguous())
+        self.w_qkv = ops.linear_weight(torch.cat([tensors[f"{n[k]}.weight"] for k in "qkv"], dim=0).contiguous(), self.weight_bits)
         if self.qkv_bias:
             self.b_qkv = torch.cat([tensors[f"{n[k]}.bias"] for k in "qkv"]).contiguous()
-        self.w_o = ops.linear_weight(tensors[f"{n['o']}.weight"])
+        self.w_o = ops.linear_weight(tensors[f"{n['o']}.weight"], self.weight_bits)
 
     def kernel_libraries(self):
         libs = ["elementwise"]      # the position encoding, a sub-part, names its own
         if self.general:
             libs.append("blockops")
         libs += attention_libraries(self.dtype, self.row_dim)
-        libs += ops.product_libraries(self.dtype)
+        libs += ops.product_libraries(self.dtype, self.weight_bits)
         return libs
 
     def cache_spec(self):

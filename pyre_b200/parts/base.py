@@ -165,6 +165,8 @@ class Part:
     # (no host reads of the step's arrays, no host synchronisation): such a part may be
     # captured in a CUDA graph and replayed for later steps of the same shape.
     graph_safe: bool = False
+    # True for a part with products that takes the parameter ``weight_bits`` (4: its weights are held as ``ops.Weight4``).
+    takes_weight_bits: bool = False
 
     def __init__(self, dtype: torch.dtype, device: torch.device):
         self.dtype = dtype
@@ -263,6 +265,11 @@ def register_part(category: str, kind: str, cls: Callable[..., Part], *, replace
     if kind in _REGISTRY[category] and not replace:
         raise ValueError(f"{category} part {kind!r} is already registered")
     _REGISTRY[category][kind] = cls
+
+
+def takes_weight_bits(category: str, kind: str) -> bool:
+    """Can parts of this kind hold their weights in 4 bits?"""
+    return bool(getattr(_REGISTRY[category].get(kind), "takes_weight_bits", False))
 
 
 def registered_parts(category: str) -> list[str]:

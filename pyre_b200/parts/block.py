@@ -34,6 +34,8 @@ class PreNormBlock(Part):
         # opt-in attributes of the parts; parts without them see plain tensors.
 
         def lazy(norm, consumer):
+            if getattr(norm, "gives_rows8", False) and getattr(consumer, "takes_rows8", False):
+                return {"rows8_ok": True}      # the consumer's weights are in 4 bits and read rows in 8
             ok = getattr(norm, "fuses_into_product", False) and getattr(consumer, "takes_scaled_rows", False)
             return {"scaled_ok": True} if ok else {}
         self._kw1, self._kw2 = lazy(self.norm1, self.mixer), lazy(self.norm2, self.ffn)

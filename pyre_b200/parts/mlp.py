@@ -32,17 +32,22 @@ class GatedMLP(Part):
     ``weight_suffix``: what follows a projection's name (".weight").  ``activation``: ``silu`` or ``relu``
     (both in the product's epilogue), or ``gelu_tanh`` (product, then the activation kernel on the stacked [gates | ups]);
     ``clamped`` with ``limit`` (in the epilogue): g sigmoid(1.702 g) (u + 1) for g = min(gate(h), limit) and
-    u = clamp(up(h), -limit, limit)."""
+    u = clamp(up(h), -limit, limit).
+    ``weight_bits``: 4 = the weights are held as ``ops.Weight4``; a kernel of its own then applies the activation and leaves the inner rows in
+    8 bits."""
 
     DEFAULT_NAMES = {"gate": "gate_proj", "up": "up_proj", "down": "down_proj"}
 
     graph_safe = True
     takes_scaled_rows = True      # ``h`` may be ``ops.ScaledRows``: the gate/up product applies the norm's 1/rms itself
+    takes_weight_bits = True
 
     def __init__(self, dtype, device, width: int, intermediate: int, activation: str = "silu",
-                 names: "dict[str, str] | None" = None, weight_suffix: str = ".weight", limit: "float | None" = None):
+                 names: "dict[str, str] | None" = None, weight_suffix: str = ".weight", limit: "float | None" = None,
+                 weight_bits: "int | None" = None):
         super().__init__(dtype, device)
         self.limit = _limit(activation, limit)
+        self.weight_bits = ops.known_weight_bits(weight_bits)
         self.names = dict(self.DEFAULT_NAMES, **(names or {}))
         self.suffix = str(weight_suffix)
         self.width, self.intermediate = int(width), int(intermediate)
@@ -52,9 +57,10 @@ class GatedMLP(Part):
         self.w_gate_up = self.w_down = None
         # the product's epilogue knows silu and relu; another activation runs after the product on [gates | ups]
         self.in_product = activation in ops.GATE_KINDS
-        self.interleaved = self.in_product and dtype == torch.bfloat16 and self.intermediate % (2 * ops.GATED_BLOCK) == 0
-        if not self.in_product:
+        self.interleaved = self.in_product and dtype == torch.bfloat16 and self.weight_bits is None and self.intermediate % (2 * ops.GATED_BLOCK) == 0
+        if not self.in_product or self.weight_bits is not None:
             self.takes_scaled_rows = False
+        self.takes_rows8 = self.weight_bits is not None
 
     def tensors(self):
         n, sfx = self.names, self.suffix
@@ -70,16 +76,18 @@ class GatedMLP(Part):
         if self.interleaved:
             self.w_gate_up = ops.interleave_gate_up(gate, up)
         else:
-            self.w_gate_up = ops.linear_weight(torch.cat([gate, up], dim=0).contiguous())
-        self.w_down = ops.linear_weight(tensors[n["down"] + sfx])
+            self.w_gate_up = ops.linear_weight(torch.cat([gate, up], dim=0).contiguous(), self.weight_bits)
+        self.w_down = ops.linear_weight(tensors[n["down"] + sfx], self.weight_bits)
 
     def kernel_libraries(self):
         return ["elementwise"] + (["parallel_block"] if not self.in_product else []) + \
-            ops.product_libraries(self.dtype)
+            ops.product_libraries(self.dtype, self.weight_bits)
 
     def forward(self, ctx, h):
         with lib.section("gate_up"):
-            if self.in_product:
+            if self.in_product and self.weight_bits is not None:
+                act = ops.gate_rows8(ops.linear(h, self.w_gate_up), self.activation, self.limit)
+            elif self.in_product:
                 act = ops.gated_linear(h, self.w_gate_up, self.interleaved, **_kind(self.activation, self.limit))
             else:
                 act = ops.act_mul(ops.materialize(ops.linear(h, self.w_gate_up)), self.activation, **({"limit": self.limit} if self.limit else {}))

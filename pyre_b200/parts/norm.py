@@ -21,6 +21,7 @@ class RMSNorm(Part):
     graph_safe = True
     fuses_into_product = True     # forward takes ``scaled_ok``: with it, the norm may run as the fix-up of the product
                                   # that ``delta`` stands for and hand its consumer ``ops.ScaledRows``
+    gives_rows8 = True            # forward takes ``rows8_ok``: with it, the result is ``ops.Rows8``
 
     def __init__(self, dtype, device, width: int, eps: float, offset: float = 0.0, tensor_name: str = "weight"):
         super().__init__(dtype, device)
@@ -37,7 +38,9 @@ class RMSNorm(Part):
     def kernel_libraries(self):
         return ["elementwise"]
 
-    def forward(self, ctx, x, delta=None, rows=None, update_x=True, scaled_ok=False):
+    def forward(self, ctx, x, delta=None, rows=None, update_x=True, scaled_ok=False, rows8_ok=False):
+        if rows8_ok:
+            return ops.add_rmsnorm_rows8(x, delta, self.weight, self.eps, self.dtype, rows=rows, update_x=update_x)
         return ops.add_rmsnorm(x, delta, self.weight, self.eps, self.dtype, rows=rows, update_x=update_x, scaled_ok=scaled_ok)
 
     def add_normed(self, ctx, x, y, want_next: bool = False):

@@ -20,7 +20,7 @@ class SampleTicket:
 
 
 class Sampler:
-    """Greedy and temperature sampling in one kernel launch; one device-to-host copy of
+    """Greedy and temperature sampling, over all tokens or the likeliest ones, in one kernel launch; one device-to-host copy of
     the chosen ids per step (the reference copies once per request, pyre/scheduler.py:94)."""
 
     def __init__(self, device):
@@ -45,15 +45,24 @@ class Sampler:
             ids = ops.sample(logits)
         else:
             seeds = np.asarray([p.seed & 0x7FFFFFFFFFFFFFFF for p in params], dtype=np.int64)
-            small = np.empty((2, R), dtype=np.int32)
+            filters = any(p.filters for p in params)
+            small = np.empty((5 if filters else 2, R), dtype=np.int32)
             small[0] = np.asarray([p.temperature for p in params], dtype=np.float32).view(np.int32)
             small[1] = np.asarray(token_index, dtype=np.int32)
+            if filters:
+                small[2] = np.asarray([p.top_k for p in params], dtype=np.int32)
+                small[3] = np.asarray([p.top_p for p in params], dtype=np.float32).view(np.int32)
+                small[4] = np.asarray([p.min_p for p in params], dtype=np.float32).view(np.int32)
             seeds_dev = torch.from_numpy(seeds).to(self.device)
             small_dev = torch.from_numpy(small).to(self.device)
             temperature = small_dev[0].view(torch.float32)
             self.bytes_uploaded += seeds.nbytes + small.nbytes
             tix = small_dev[1]
-            ids = ops.sample(logits, temperature, seeds_dev, tix)
+            if filters:
+                ids = ops.sample(logits, temperature, seeds_dev, tix, top_k=small_dev[2], top_p=small_dev[3].view(torch.float32),
+                                 min_p=small_dev[4].view(torch.float32))
+            else:
+                ids = ops.sample(logits, temperature, seeds_dev, tix)
         self.bytes_downloaded += R * 4
         i = self._turn
         self._turn ^= 1
