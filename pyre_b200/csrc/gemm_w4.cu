@@ -6,7 +6,7 @@
 // The inner sums are exact (32-bit integers: |sum| <= 16 * 8 * 127 * 128 < 2^21, a weight's half byte stays in the upper half of its byte, which
 // makes it sixteen times as large and spares the sign's extension), the outer ones in float, by ascending group in each of a CTA's warps,
 // then over the warps in order.
-#include "common.cuh"
+#include "tensor_core.cuh"
 
 namespace {
 constexpr int GROUP = 128;
@@ -95,6 +95,362 @@ int launch_few(const W4Params& p, cudaStream_t stream) {
     return 0;
 }
 
+// ---------------------------------------------------------------------------
+// Many rows, on the 5th-generation tensor cores.  A CTA owns 128 features (the MMA's rows) and TN tokens and takes a group of 128 k at a time:
+//   warp 0, one thread : TMA.  The group's weights as they are packed (128 x 64 bytes) into one ring, the tokens' bytes (TN x 128) into another.
+//   warps 4..7         : a thread owns a feature: 64 bytes of a group to 128 (two masks and a shift per eight), stored to tensor memory, which
+//                        is where the MMAs take their A operand from.
+//   warp 1, one thread : four MMAs (kind::i8, 32 k each) a group, into one of two accumulators of 32-bit integers.
+//   warps 8..15        : a thread owns a feature and half of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
+//                        feature and added to float sums in registers, by ascending group.
+// An output tile whose K is shared among CTAs (few tiles) leaves float shares, added up in order by whoever reads them.
+// ---------------------------------------------------------------------------
+constexpr int ERR_TIMEOUT = 2;
+constexpr int FEATURES = 128, MANY_THREADS = 512, W_STAGES = 6, A_STAGES = 6, B_STAGES = 6, A_COLS = 32;
+constexpr int W_BYTES = FEATURES * GROUP / 2;
+
+struct ManyParams {
+    const float* row_scales;
+    long long ld_scales;
+    const __nv_bfloat16* scales;
+    void* out;                    // [M][N], or float [splits][M][N]
+    int M, N, G;
+    int tiles_m, tiles;           // tiles of tokens (fastest); of everything
+    int splits, per_split;        // of K, in groups
+    int* err_flag;
+};
+
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err_flag) {
+    return mbar_wait_or<ERR_TIMEOUT>(bar, parity, abort_flag, err_flag);
+}
+// ... that does not look at the abort flag: for copies and MMAs in flight, before the CTA gives its memory back.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity) && clock64() - t0 < PYRE_WAIT_CYCLES) {}
+}
+// D (tensor memory, 32-bit integers) += A (tensor memory, signed bytes) * B (shared memory, signed bytes)
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+
+template <int TN> struct Many {
+    static constexpr int B_BYTES = TN * GROUP;
+    static constexpr int W_OFF = 0, B_OFF = W_STAGES * W_BYTES, S_OFF = B_OFF + B_STAGES * B_BYTES;      // scales: [8 warps][2][TN / 2] floats
+    static constexpr int BARS = S_OFF + 8 * 2 * (TN / 2) * 4;
+    static constexpr int N_BARS = 2 * (W_STAGES + A_STAGES + B_STAGES + 2) + 1;
+    static constexpr int TOTAL = BARS + N_BARS * 8 + 24 + 1024;
+    static constexpr int A_COL0 = 2 * TN;
+    static_assert(A_COL0 + A_STAGES * A_COLS <= 512 && TOTAL <= 232448 && TN % 32 == 0, "fits");
+};
+
+template <int TN, typename T>
+__global__ void __launch_bounds__(MANY_THREADS, 1)
+w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ ManyParams p) {
+    using L = Many<TN>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t w_full = base + L::BARS, w_empty = w_full + 8 * W_STAGES;
+    const uint32_t b_full = w_empty + 8 * W_STAGES, b_empty = b_full + 8 * B_STAGES;
+    const uint32_t a_full = b_empty + 8 * B_STAGES, a_empty = a_full + 8 * A_STAGES;
+    const uint32_t acc_full = a_empty + 8 * A_STAGES, acc_empty = acc_full + 16, drained = acc_empty + 16;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::BARS + L::N_BARS * 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::BARS + L::N_BARS * 8 + 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int items = p.tiles * p.splits;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < W_STAGES; ++s) { mbar_init(w_full + 8 * s, 1); mbar_init(w_empty + 8 * s, 4); }
+        for (int s = 0; s < B_STAGES; ++s) { mbar_init(b_full + 8 * s, 1); mbar_init(b_empty + 8 * s, 1); }
+        for (int s = 0; s < A_STAGES; ++s) { mbar_init(a_full + 8 * s, 4); mbar_init(a_empty + 8 * s, 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 8); }
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    pdl_trigger();
+
+    auto range = [&](int item, int& tile, int& split, int& first, int& n) {
+        tile = item % p.tiles;
+        split = item / p.tiles;
+        first = split * p.per_split;
+        n = max(0, min(p.per_split, p.G - first));
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
+            bool waited = false, ok = true;
+            int it = 0, w_asked = 0, b_asked = 0;
+            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+                int tile, split, first, n;
+                range(item, tile, split, first, n);
+                const int f0 = tile / p.tiles_m * FEATURES, t0 = tile % p.tiles_m * TN;
+                auto weights = [&](int i) {
+                    const int at = it + i, s = at % W_STAGES;
+                    if (!mbar_wait(w_empty + 8 * s, ((at / W_STAGES) & 1) ^ 1, abort_flag, p.err_flag)) return false;
+                    mbar_expect_tx(w_full + 8 * s, W_BYTES);
+                    tma_load_2d(base + L::W_OFF + s * W_BYTES, &map_w, w_full + 8 * s, (first + i) * (GROUP / 2), f0);
+                    w_asked = at + 1;
+                    return true;
+                };
+                int done = 0;
+                if (!waited) {
+                    // the weights depend on no earlier kernel
+                    done = min(n, W_STAGES);
+                    for (int i = 0; i < done; ++i) weights(i);
+                    pdl_wait();
+                    waited = true;
+                }
+                for (int i = 0; i < n && ok; ++i) {
+                    const int at = it + i, s = at % B_STAGES;
+                    if (i >= done && !(ok = weights(i))) break;
+                    if (!(ok = mbar_wait(b_empty + 8 * s, ((at / B_STAGES) & 1) ^ 1, abort_flag, p.err_flag))) break;
+                    mbar_expect_tx(b_full + 8 * s, L::B_BYTES);
+                    tma_load_2d(base + L::B_OFF + s * L::B_BYTES, &map_x, b_full + 8 * s, (first + i) * GROUP, t0);
+                    b_asked = at + 1;
+                }
+                it += n;
+            }
+            if (!waited) pdl_wait();
+            if (!ok) {      // a wait ran out: the copies in flight end first
+                for (int at = max(0, w_asked - W_STAGES); at < w_asked; ++at) mbar_drain(w_full + 8 * (at % W_STAGES), (at / W_STAGES) & 1);
+                for (int at = max(0, b_asked - B_STAGES); at < b_asked; ++at) mbar_drain(b_full + 8 * (at % B_STAGES), (at / B_STAGES) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // D 32-bit integers (2 at bit 4), A and B signed bytes (1 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24
+            constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(FEATURES >> 4) << 24);
+            int it = 0;
+            bool ok = true;
+            pdl_wait();      // no bounded wait should have to last as long as the kernels before
+            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+                int tile, split, first, n;
+                range(item, tile, split, first, n);
+                for (int i = 0; i < n && ok; ++i, ++it) {
+                    const int sb = it % B_STAGES, sa = it % A_STAGES, d = it & 1;
+                    ok = mbar_wait(acc_empty + 8 * d, ((it >> 1) & 1) ^ 1, abort_flag, p.err_flag) &&
+                         mbar_wait(b_full + 8 * sb, (it / B_STAGES) & 1, abort_flag, p.err_flag) &&
+                         mbar_wait(a_full + 8 * sa, (it / A_STAGES) & 1, abort_flag, p.err_flag);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t db = umma_desc(base + L::B_OFF + sb * L::B_BYTES);
+                    const uint32_t a = tmem + L::A_COL0 + sa * A_COLS;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) umma_i8(tmem + d * TN, a + 8 * q, db + 2 * q, idesc, q > 0);      // 32 bytes of k further
+                    umma_commit(acc_full + 8 * d);
+                    umma_commit(a_empty + 8 * sa);
+                    umma_commit(b_empty + 8 * sb);
+                }
+            }
+            umma_commit(drained);      // the MMAs end before tensor memory is given back, also where a wait ran out
+            mbar_drain(drained, 0);
+        }
+    } else if (warp >= 4 && warp < 8) {
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        bool waited = false, ok = true;
+        int it = 0;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            int tile, split, first, n;
+            range(item, tile, split, first, n);
+            for (int i = 0; i < n && ok; ++i, ++it) {
+                const int s = it % W_STAGES, sa = it % A_STAGES;
+                ok = mbar_wait(w_full + 8 * s, (it / W_STAGES) & 1, abort_flag, p.err_flag);
+                const uint32_t src = base + L::W_OFF + s * W_BYTES + row * 64;      // 64-byte swizzle: a chunk of 16 bytes by bits 7 and 8
+                uint32_t v[16], a[32];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[4 * q]), "=r"(v[4 * q + 1]), "=r"(v[4 * q + 2]), "=r"(v[4 * q + 3])
+                                 : "r"(src + ((q ^ ((row >> 1) & 3)) << 4)) : "memory");
+#pragma unroll
+                for (int q = 0; q < 16; ++q) { a[2 * q] = lower(v[q]); a[2 * q + 1] = upper(v[q]); }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(w_empty + 8 * s);
+                if (!waited && it >= A_STAGES) { pdl_wait(); waited = true; }      // from here on the MMAs have to run
+                ok = mbar_wait(a_empty + 8 * sa, ((it / A_STAGES) & 1) ^ 1, abort_flag, p.err_flag) && ok;
+                ok = __all_sync(0xffffffffu, ok);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                tmem_st16(tmem + lanes + L::A_COL0 + sa * A_COLS, a);
+                tmem_st16(tmem + lanes + L::A_COL0 + sa * A_COLS + 16, a + 16);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(a_full + 8 * sa);
+            }
+        }
+        if (!waited) pdl_wait();
+    } else if (warp >= 8) {
+        constexpr int COLS = TN / 2, PER_LANE = COLS / 32;
+        const int e = warp - 8, quarter = warp & 3, row = quarter * 32 + lane, col0 = (e >> 2) * COLS;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        float* const mine = reinterpret_cast<float*>(gen + L::S_OFF) + e * 2 * COLS;
+        pdl_wait();
+        bool ok = true;
+        int it = 0;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            int tile, split, first, n;
+            range(item, tile, split, first, n);
+            const int f = tile / p.tiles_m * FEATURES + row, t0 = tile % p.tiles_m * TN + col0;
+            const __nv_bfloat16* sw = p.scales + (size_t)first * p.N + min(f, p.N - 1);
+            const float* sx = p.row_scales + (size_t)first * p.ld_scales;
+            int at[PER_LANE];
+#pragma unroll
+            for (int q = 0; q < PER_LANE; ++q) at[q] = min(t0 + q * 32 + lane, p.M - 1);
+            // scales are asked for AHEAD groups before they are used
+            constexpr int AHEAD = 4;
+            float x_ahead[AHEAD][PER_LANE], w_ahead[AHEAD];
+            auto ask = [&](int i, float (&x)[PER_LANE], float& w) {
+                const int g = min(i, n - 1);
+                w = __bfloat162float(sw[(size_t)g * p.N]) * 0.0625f;
+#pragma unroll
+                for (int q = 0; q < PER_LANE; ++q) x[q] = sx[(size_t)g * p.ld_scales + at[q]];
+            };
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) ask(q, x_ahead[q], w_ahead[q]);
+            uint64_t sum[COLS / 2];
+#pragma unroll
+            for (int q = 0; q < COLS / 2; ++q) sum[q] = 0;
+            for (int i = 0; i < n && ok; ++i, ++it) {
+                const int d = it & 1;
+                float* const buffer = mine + d * COLS;
+#pragma unroll
+                for (int q = 0; q < PER_LANE; ++q) buffer[q * 32 + lane] = x_ahead[0][q];
+                const uint64_t scale = pack2(w_ahead[0], w_ahead[0]);
+#pragma unroll
+                for (int a = 0; a + 1 < AHEAD; ++a) {
+                    w_ahead[a] = w_ahead[a + 1];
+#pragma unroll
+                    for (int q = 0; q < PER_LANE; ++q) x_ahead[a][q] = x_ahead[a + 1][q];
+                }
+                ask(i + AHEAD, x_ahead[AHEAD - 1], w_ahead[AHEAD - 1]);
+                ok = mbar_wait(acc_full + 8 * d, (it >> 1) & 1, abort_flag, p.err_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                __syncwarp();      // the scales written above are there
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int c = 0; c < COLS; c += 16) {
+                    int v[16];
+                    tmem_ld16(tmem + lanes + d * TN + col0 + c, v);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int q = 0; q < 16; q += 4) {
+                        const ulonglong2 x4 = *reinterpret_cast<const ulonglong2*>(buffer + c + q);
+                        uint64_t& s0 = sum[(c + q) / 2];
+                        uint64_t& s1 = sum[(c + q) / 2 + 1];
+                        s0 = fma2(mul2(pack2((float)v[q], (float)v[q + 1]), x4.x), scale, s0);
+                        s1 = fma2(mul2(pack2((float)v[q + 2], (float)v[q + 3]), x4.y), scale, s1);
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + 8 * d);
+            }
+            if (ok && f < p.N) {
+                T* out = (T*)p.out + (size_t)split * p.M * p.N + (size_t)t0 * p.N + f;
+#pragma unroll
+                for (int q = 0; q < COLS; ++q) {
+                    const uint32_t bits = q & 1 ? (uint32_t)(sum[q / 2] >> 32) : (uint32_t)sum[q / 2];
+                    if (t0 + q < p.M) ElemOps<T>::store(out + (size_t)q * p.N, __uint_as_float(bits));
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled() {
+    static EncodeTiledFn fn = nullptr;
+    if (!fn) {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(ptr);
+    }
+    return fn;
+}
+// A map of bytes [rows][pitch] in boxes of `high` rows of `wide` bytes.
+bool byte_map(CUtensorMap* map, const void* p, int rows, long long pitch, int wide, int high) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)pitch};
+    cuuint32_t box[2] = {(cuuint32_t)wide, (cuuint32_t)high}, elem[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              wide == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int TN, typename T>
+int launch_many(const W4Params& w, int splits, int* err_flag, cudaStream_t stream) {
+    using L = Many<TN>;
+    static bool configured_on[PYRE_MAX_DEVICES] = {};      // the attribute is per device
+    bool& configured = configured_on[pyre_current_device()];
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(w4_many_kernel<TN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    CUtensorMap mw, mx;
+    if (!byte_map(&mw, w.packed, w.N, 64ll * w.G, 64, FEATURES) || !byte_map(&mx, w.rows, w.M, 128ll * w.G, 128, TN)) return PYRE_ERR_BAD_ARG;
+    ManyParams p = {w.row_scales, w.ld_scales, w.scales, w.out, w.M, w.N, w.G, ceil_div(w.M, TN), 0, splits, ceil_div(w.G, splits), err_flag};
+    const long long tiles = (long long)p.tiles_m * ceil_div(w.N, FEATURES);
+    if (tiles * splits > 0x7fffffffll) return PYRE_ERR_UNSUPPORTED;
+    p.tiles = (int)tiles;
+    const int items = p.tiles * splits, sms = pyre_sm_count();
+    const cudaError_t e = pyre_launch(w4_many_kernel<TN, T>, dim3(items < sms ? items : sms), dim3(MANY_THREADS), (size_t)L::TOTAL, stream, mw, mx, p);
+    if (e != cudaSuccess) return (int)e;
+    PYRE_LAUNCH_CHECK();
+    return 0;
+}
+constexpr int FEW = 32;      // rows up to here take the other kernel
+
 // A warp per group of a feature: s = bf16(max |w| / 7), q = rint(w / s) within -8 .. 7.  A group of zeros (or below 2^-100) has s = 0, one with an
 // infinity or a NaN s = NaN.
 template <typename T>
@@ -165,13 +521,25 @@ PYRE_API int pyre_w4_values(const void* packed, const void* scales, void* out, i
     return 0;
 }
 
-// rows [M][128 G] and packed [N][64 G] on 16-byte boundaries; out [M, N] of `dtype`
+// Shares of K that a product of these sizes leaves (1: none), by what fills the SMs.
+PYRE_API int pyre_w4_splits(int M, int N, int G) {
+    if (M <= FEW) return 1;
+    const int tiles = ceil_div(M, M <= 64 ? 64 : 128) * ceil_div(N, FEATURES), sms = pyre_sm_count();
+    int splits = min(min(8, sms / max(1, tiles)), G / 4);
+    if (splits <= 1) return 1;
+    return ceil_div(G, ceil_div(G, splits));      // no empty share
+}
+
+// rows [M][128 G] and packed [N][64 G] on 16-byte boundaries; out [M, N] of `dtype`, or where `splits` is not 1 float [splits][M][N] (to be added up in
+// order)
 PYRE_API int pyre_w4_linear(const void* rows, const float* row_scales, long long ld_scales, const void* packed, const void* scales, void* out,
-                            int M, int N, int G, int dtype, cudaStream_t stream) {
+                            int M, int N, int G, int splits, int dtype, int* err_flag, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (G <= 0 || ((uintptr_t)rows & 15) || ((uintptr_t)packed & 15)) return PYRE_ERR_BAD_ARG;
+    if (dtype != PYRE_F32 && dtype != PYRE_BF16) return PYRE_ERR_BAD_ARG;
+    if (splits < 1 || (splits > 1 && (M <= FEW || dtype != PYRE_F32 || (splits - 1) * ceil_div(G, splits) >= G))) return PYRE_ERR_BAD_ARG;
     const W4Params p = {(const uint8_t*)rows, row_scales, ld_scales, (const uint8_t*)packed, (const __nv_bfloat16*)scales, out, M, N, G};
-    if (dtype == PYRE_F32) return launch_few<float>(p, stream);
-    if (dtype == PYRE_BF16) return launch_few<__nv_bfloat16>(p, stream);
-    return PYRE_ERR_BAD_ARG;
+    if (M <= FEW) return dtype == PYRE_F32 ? launch_few<float>(p, stream) : launch_few<__nv_bfloat16>(p, stream);
+    if (M <= 64) return dtype == PYRE_F32 ? launch_many<64, float>(p, splits, err_flag, stream) : launch_many<64, __nv_bfloat16>(p, splits, err_flag, stream);
+    return dtype == PYRE_F32 ? launch_many<128, float>(p, splits, err_flag, stream) : launch_many<128, __nv_bfloat16>(p, splits, err_flag, stream);
 }

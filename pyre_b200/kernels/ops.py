@@ -456,9 +456,10 @@ def quantize_weight4(w: torch.Tensor) -> Weight4:
     return Weight4(packed, scales, K)
 
 
-def linear4(x: "torch.Tensor | Rows8", w: Weight4, out_dtype: "torch.dtype | None" = None) -> torch.Tensor:
+def linear4(x: "torch.Tensor | Rows8", w: Weight4, out_dtype: "torch.dtype | None" = None, partials_ok: bool = False) -> "torch.Tensor | PartialSums":
     """y = x W^T for a weight in 4 bits: whole numbers summed exactly within a group, the groups in float32.  Activations that are
-    not in 8 bits yet go through ``quantize_rows8`` first."""
+    not in 8 bits yet go through ``quantize_rows8`` first.  ``partials_ok``: ``PartialSums`` in float32 come back, one part or, where K is
+    shared among CTAs, several."""
     if not isinstance(x, Rows8):
         x = quantize_rows8(materialize(x))
     _check_rows8(x)
@@ -468,10 +469,16 @@ def linear4(x: "torch.Tensor | Rows8", w: Weight4, out_dtype: "torch.dtype | Non
         raise ValueError(f"inner sizes differ: x is [{T}, {K}], w is [{N}, {K2}]")
     require_current_device(w.packed.device, "w")
     dtype = out_dtype or x.dtype
-    out = torch.empty((T, N), dtype=dtype, device=x.rows.device)
+    groups = w.scales.shape[0]
+    splits = lib.call_value("pyre_w4_splits", T, N, groups)
+    shares = partials_ok or splits > 1
+    out = torch.empty((splits, T, N) if shares else (T, N), dtype=torch.float32 if shares else dtype, device=x.rows.device)
     lib.call("pyre_w4_linear", x.rows.data_ptr(), x.scales.data_ptr(), x.scales.stride(0), w.packed.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
-             T, N, w.scales.shape[0], _dt(dtype), _stream())
-    return out
+             T, N, groups, splits, _dt(out.dtype), device_error_flag(x.rows.device).data_ptr(), _stream())
+    if not shares:
+        return out
+    out = PartialSums(out, dtype)
+    return out if partials_ok else materialize(out)
 
 
 def add_residual(x: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:
@@ -1470,11 +1477,9 @@ def linear(x: "torch.Tensor | ScaledRows", w: torch.Tensor, out_dtype: "torch.dt
     of many tokens in one split is deferred too, since its epilogue can fold the residual add (``folds_residual``).
     ``deferred_ok=("rope", head_dim)``: the consumer is a position encoding that may fold bias, rotation and the cache
     write into the stacked q/k/v product (``folds_rope``).  A ``Weight4`` takes ``Rows8`` (other activations are put in 8 bits first); with
-    ``partials_ok`` its result stays unrounded, as one part."""
+    ``partials_ok`` its result stays unrounded."""
     if isinstance(w, Weight4):
-        if partials_ok and out_dtype is None and x.dtype == torch.bfloat16:
-            return PartialSums(linear4(x, w, torch.float32).unsqueeze(0), torch.bfloat16)
-        return linear4(x, w, out_dtype)
+        return linear4(x, w, out_dtype, partials_ok and out_dtype is None and x.dtype == torch.bfloat16)
     x = materialize(x) if isinstance(x, Rows8) else x
     if x.dtype == torch.float32:
         return fixed_linear(x, w) if isinstance(w, FixedWeight) else sgemm_nt(x, w)
