@@ -101,12 +101,15 @@ int launch_few(const W4Params& p, cudaStream_t stream) {
 //   warps 4..7         : a thread owns a feature: 64 bytes of a group to 128 (two masks and a shift per eight), stored to tensor memory, which
 //                        is where the MMAs take their A operand from.
 //   warp 1, one thread : four MMAs (kind::i8, 32 k each) a group, into one of two accumulators of 32-bit integers.
-//   warps 8..15        : a thread owns a feature and half of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
-//                        feature and added to float sums in registers, by ascending group.
+//   warps 2, 3         : the scales of four groups at a time, of features and of tokens, to shared memory.
+//   warps 8..23        : a thread owns a feature and a quarter of the tokens.  The group's integers come out of tensor memory at once, which frees the
+//                        accumulator, are scaled by token and by feature and added to float sums in registers, by ascending group.
 // An output tile whose K is shared among CTAs (few tiles) leaves float shares, added up in order by whoever reads them.
 // ---------------------------------------------------------------------------
 constexpr int ERR_TIMEOUT = 2;
-constexpr int FEATURES = 128, MANY_THREADS = 512, W_STAGES = 6, A_STAGES = 6, B_STAGES = 6, A_COLS = 32;
+constexpr int FEATURES = 128, MANY_THREADS = 768, EPI_WARP0 = 8, EPI_WARPS = 16, A_COLS = 32;
+constexpr int W_STAGES = 6, STAGES = 6;               // packed weights; both operands of the MMAs
+constexpr int BATCH = 4, S_STAGES = 2;                // groups whose scales come at a time
 constexpr int W_BYTES = FEATURES * GROUP / 2;
 
 struct ManyParams {
@@ -134,7 +137,7 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint32_t tmem_a, uint64
                  "tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
@@ -161,13 +164,14 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 template <int TN> struct Many {
-    static constexpr int B_BYTES = TN * GROUP;
-    static constexpr int W_OFF = 0, B_OFF = W_STAGES * W_BYTES, S_OFF = B_OFF + B_STAGES * B_BYTES;      // scales: [8 warps][2][TN / 2] floats
-    static constexpr int BARS = S_OFF + 8 * 2 * (TN / 2) * 4;
-    static constexpr int N_BARS = 2 * (W_STAGES + A_STAGES + B_STAGES + 2) + 1;
+    static constexpr int X_BYTES = TN * GROUP;
+    static constexpr int W_OFF = 0, X_OFF = W_STAGES * W_BYTES;
+    static constexpr int SX_OFF = X_OFF + STAGES * X_BYTES, SW_OFF = SX_OFF + S_STAGES * BATCH * TN * 4;      // [stage][group][token], [..][feature]
+    static constexpr int BARS = SW_OFF + S_STAGES * BATCH * FEATURES * 4;
+    static constexpr int N_BARS = 2 * (W_STAGES + STAGES + S_STAGES + 2) + 1;
     static constexpr int TOTAL = BARS + N_BARS * 8 + 24 + 1024;
     static constexpr int A_COL0 = 2 * TN;
-    static_assert(A_COL0 + A_STAGES * A_COLS <= 512 && TOTAL <= 232448 && TN % 32 == 0, "fits");
+    static_assert(A_COL0 + STAGES * A_COLS <= 512 && TOTAL <= 232448 && TN % 64 == 0, "fits");
 };
 
 template <int TN, typename T>
@@ -178,9 +182,9 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t w_full = base + L::BARS, w_empty = w_full + 8 * W_STAGES;
-    const uint32_t b_full = w_empty + 8 * W_STAGES, b_empty = b_full + 8 * B_STAGES;
-    const uint32_t a_full = b_empty + 8 * B_STAGES, a_empty = a_full + 8 * A_STAGES;
-    const uint32_t acc_full = a_empty + 8 * A_STAGES, acc_empty = acc_full + 16, drained = acc_empty + 16;
+    const uint32_t ab_full = w_empty + 8 * W_STAGES, ab_empty = ab_full + 8 * STAGES;      // both operands: converted weights and the tokens' bytes
+    const uint32_t s_full = ab_empty + 8 * STAGES, s_empty = s_full + 8 * S_STAGES;
+    const uint32_t acc_full = s_empty + 8 * S_STAGES, acc_empty = acc_full + 16, drained = acc_empty + 16;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::BARS + L::N_BARS * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::BARS + L::N_BARS * 8 + 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -189,9 +193,9 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < W_STAGES; ++s) { mbar_init(w_full + 8 * s, 1); mbar_init(w_empty + 8 * s, 4); }
-        for (int s = 0; s < B_STAGES; ++s) { mbar_init(b_full + 8 * s, 1); mbar_init(b_empty + 8 * s, 1); }
-        for (int s = 0; s < A_STAGES; ++s) { mbar_init(a_full + 8 * s, 4); mbar_init(a_empty + 8 * s, 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 8); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(ab_full + 8 * s, 5); mbar_init(ab_empty + 8 * s, 1); }
+        for (int s = 0; s < S_STAGES; ++s) { mbar_init(s_full + 8 * s, 2); mbar_init(s_empty + 8 * s, EPI_WARPS); }
+        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, EPI_WARPS); }
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -206,23 +210,24 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const uint32_t tmem = *tmem_slot;
     pdl_trigger();
 
-    auto range = [&](int item, int& tile, int& split, int& first, int& n) {
-        tile = item % p.tiles;
+    auto range = [&](int item, int& f0, int& t0, int& split, int& first, int& n) {
+        const int tile = item % p.tiles;
         split = item / p.tiles;
+        f0 = tile / p.tiles_m * FEATURES;
+        t0 = tile % p.tiles_m * TN;
         first = split * p.per_split;
-        n = max(0, min(p.per_split, p.G - first));
+        n = min(p.per_split, p.G - first);      // at least one: no share is empty
     };
 
+    int f0, t0, split, first, n;
     if (warp == 0) {
         if (lane == 0) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
             bool waited = false, ok = true;
-            int it = 0, w_asked = 0, b_asked = 0;
+            int it = 0, w_asked = 0, x_asked = 0;
             for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-                int tile, split, first, n;
-                range(item, tile, split, first, n);
-                const int f0 = tile / p.tiles_m * FEATURES, t0 = tile % p.tiles_m * TN;
+                range(item, f0, t0, split, first, n);
                 auto weights = [&](int i) {
                     const int at = it + i, s = at % W_STAGES;
                     if (!mbar_wait(w_empty + 8 * s, ((at / W_STAGES) & 1) ^ 1, abort_flag, p.err_flag)) return false;
@@ -240,60 +245,90 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     waited = true;
                 }
                 for (int i = 0; i < n && ok; ++i) {
-                    const int at = it + i, s = at % B_STAGES;
+                    const int at = it + i, s = at % STAGES;
                     if (i >= done && !(ok = weights(i))) break;
-                    if (!(ok = mbar_wait(b_empty + 8 * s, ((at / B_STAGES) & 1) ^ 1, abort_flag, p.err_flag))) break;
-                    mbar_expect_tx(b_full + 8 * s, L::B_BYTES);
-                    tma_load_2d(base + L::B_OFF + s * L::B_BYTES, &map_x, b_full + 8 * s, (first + i) * GROUP, t0);
-                    b_asked = at + 1;
+                    if (!(ok = mbar_wait(ab_empty + 8 * s, ((at / STAGES) & 1) ^ 1, abort_flag, p.err_flag))) break;
+                    mbar_expect_tx(ab_full + 8 * s, L::X_BYTES);
+                    tma_load_2d(base + L::X_OFF + s * L::X_BYTES, &map_x, ab_full + 8 * s, (first + i) * GROUP, t0);
+                    x_asked = at + 1;
                 }
                 it += n;
             }
             if (!waited) pdl_wait();
             if (!ok) {      // a wait ran out: the copies in flight end first
                 for (int at = max(0, w_asked - W_STAGES); at < w_asked; ++at) mbar_drain(w_full + 8 * (at % W_STAGES), (at / W_STAGES) & 1);
-                for (int at = max(0, b_asked - B_STAGES); at < b_asked; ++at) mbar_drain(b_full + 8 * (at % B_STAGES), (at / B_STAGES) & 1);
+                for (int at = max(0, x_asked - STAGES); at < x_asked; ++at) mbar_drain(ab_full + 8 * (at % STAGES), (at / STAGES) & 1);
             }
         }
     } else if (warp == 1) {
         if (lane == 0) {
             // D 32-bit integers (2 at bit 4), A and B signed bytes (1 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24
             constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(FEATURES >> 4) << 24);
-            int it = 0;
+            const uint64_t db0 = umma_desc(base + L::X_OFF);
+            int it = 0, s = 0;
             bool ok = true;
             pdl_wait();      // no bounded wait should have to last as long as the kernels before
             for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-                int tile, split, first, n;
-                range(item, tile, split, first, n);
-                for (int i = 0; i < n && ok; ++i, ++it) {
-                    const int sb = it % B_STAGES, sa = it % A_STAGES, d = it & 1;
+                range(item, f0, t0, split, first, n);
+                for (int i = 0; i < n; ++i, ++it) {
+                    const int d = it & 1;
                     ok = mbar_wait(acc_empty + 8 * d, ((it >> 1) & 1) ^ 1, abort_flag, p.err_flag) &&
-                         mbar_wait(b_full + 8 * sb, (it / B_STAGES) & 1, abort_flag, p.err_flag) &&
-                         mbar_wait(a_full + 8 * sa, (it / A_STAGES) & 1, abort_flag, p.err_flag);
+                         mbar_wait(ab_full + 8 * s, (it / STAGES) & 1, abort_flag, p.err_flag);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t db = umma_desc(base + L::B_OFF + sb * L::B_BYTES);
-                    const uint32_t a = tmem + L::A_COL0 + sa * A_COLS;
+                    const uint64_t db = db0 + s * (L::X_BYTES >> 4);
+                    const uint32_t a = tmem + L::A_COL0 + s * A_COLS;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) umma_i8(tmem + d * TN, a + 8 * q, db + 2 * q, idesc, q > 0);      // 32 bytes of k further
                     umma_commit(acc_full + 8 * d);
-                    umma_commit(a_empty + 8 * sa);
-                    umma_commit(b_empty + 8 * sb);
+                    umma_commit(ab_empty + 8 * s);
+                    s = s + 1 == STAGES ? 0 : s + 1;
                 }
             }
             umma_commit(drained);      // the MMAs end before tensor memory is given back, also where a wait ran out
             mbar_drain(drained, 0);
         }
-    } else if (warp >= 4 && warp < 8) {
+    } else if (warp < 4) {
+        // warp 2: the tokens' scales, warp 3: the features' (a sixteenth of them: the integers are sixteen times as large)
+        bool ok = true;
+        int bt = 0;
+        pdl_wait();
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            range(item, f0, t0, split, first, n);
+            for (int i0 = 0; i0 < n && ok; i0 += BATCH, ++bt) {
+                const int s = bt % S_STAGES;
+                constexpr int PER_LANE = FEATURES / 32;
+                float v[BATCH][PER_LANE];
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    const size_t g = first + min(i0 + j, n - 1);
+#pragma unroll
+                    for (int q = 0; q < PER_LANE; ++q) {
+                        if (warp == 2) v[j][q] = q * 32 < TN ? p.row_scales[g * p.ld_scales + min(t0 + q * 32 + lane, p.M - 1)] : 0.f;
+                        else v[j][q] = __bfloat162float(p.scales[g * p.N + min(f0 + q * 32 + lane, p.N - 1)]) * 0.0625f;
+                    }
+                }
+                ok = mbar_wait(s_empty + 8 * s, ((bt / S_STAGES) & 1) ^ 1, abort_flag, p.err_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                float* const to = reinterpret_cast<float*>(gen + (warp == 2 ? L::SX_OFF + s * BATCH * TN * 4 : L::SW_OFF + s * BATCH * FEATURES * 4));
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j)
+#pragma unroll
+                    for (int q = 0; q < PER_LANE; ++q)
+                        if (warp == 3 || q * 32 < TN) to[j * (warp == 2 ? TN : FEATURES) + q * 32 + lane] = v[j][q];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_full + 8 * s);
+            }
+        }
+    } else if (warp < EPI_WARP0) {
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         bool waited = false, ok = true;
         int it = 0;
         for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-            int tile, split, first, n;
-            range(item, tile, split, first, n);
+            range(item, f0, t0, split, first, n);
             for (int i = 0; i < n && ok; ++i, ++it) {
-                const int s = it % W_STAGES, sa = it % A_STAGES;
+                const int s = it % W_STAGES, sa = it % STAGES;
                 ok = mbar_wait(w_full + 8 * s, (it / W_STAGES) & 1, abort_flag, p.err_flag);
                 const uint32_t src = base + L::W_OFF + s * W_BYTES + row * 64;      // 64-byte swizzle: a chunk of 16 bytes by bits 7 and 8
                 uint32_t v[16], a[32];
@@ -305,8 +340,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 for (int q = 0; q < 16; ++q) { a[2 * q] = lower(v[q]); a[2 * q + 1] = upper(v[q]); }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(w_empty + 8 * s);
-                if (!waited && it >= A_STAGES) { pdl_wait(); waited = true; }      // from here on the MMAs have to run
-                ok = mbar_wait(a_empty + 8 * sa, ((it / A_STAGES) & 1) ^ 1, abort_flag, p.err_flag) && ok;
+                if (!waited && it >= STAGES) { pdl_wait(); waited = true; }      // from here on the MMAs have to run
+                ok = mbar_wait(ab_empty + 8 * sa, ((it / STAGES) & 1) ^ 1, abort_flag, p.err_flag) && ok;
                 ok = __all_sync(0xffffffffu, ok);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 tmem_st16(tmem + lanes + L::A_COL0 + sa * A_COLS, a);
@@ -314,83 +349,59 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(a_full + 8 * sa);
+                if (lane == 0) mbar_arrive(ab_full + 8 * sa);
             }
         }
         if (!waited) pdl_wait();
-    } else if (warp >= 8) {
-        constexpr int COLS = TN / 2, PER_LANE = COLS / 32;
-        const int e = warp - 8, quarter = warp & 3, row = quarter * 32 + lane, col0 = (e >> 2) * COLS;
+    } else {
+        constexpr int COLS = TN / 4;
+        static_assert(EPI_WARPS == 16 && COLS % 16 == 0, "four warps side by side, whole loads from tensor memory");
+        const int quarter = warp & 3, row = quarter * 32 + lane, col0 = ((warp - EPI_WARP0) >> 2) * COLS;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        float* const mine = reinterpret_cast<float*>(gen + L::S_OFF) + e * 2 * COLS;
         pdl_wait();
         bool ok = true;
-        int it = 0;
+        int it = 0, bt = 0;
         for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-            int tile, split, first, n;
-            range(item, tile, split, first, n);
-            const int f = tile / p.tiles_m * FEATURES + row, t0 = tile % p.tiles_m * TN + col0;
-            const __nv_bfloat16* sw = p.scales + (size_t)first * p.N + min(f, p.N - 1);
-            const float* sx = p.row_scales + (size_t)first * p.ld_scales;
-            int at[PER_LANE];
-#pragma unroll
-            for (int q = 0; q < PER_LANE; ++q) at[q] = min(t0 + q * 32 + lane, p.M - 1);
-            // scales are asked for AHEAD groups before they are used
-            constexpr int AHEAD = 4;
-            float x_ahead[AHEAD][PER_LANE], w_ahead[AHEAD];
-            auto ask = [&](int i, float (&x)[PER_LANE], float& w) {
-                const int g = min(i, n - 1);
-                w = __bfloat162float(sw[(size_t)g * p.N]) * 0.0625f;
-#pragma unroll
-                for (int q = 0; q < PER_LANE; ++q) x[q] = sx[(size_t)g * p.ld_scales + at[q]];
-            };
-#pragma unroll
-            for (int q = 0; q < AHEAD; ++q) ask(q, x_ahead[q], w_ahead[q]);
+            range(item, f0, t0, split, first, n);
             uint64_t sum[COLS / 2];
 #pragma unroll
             for (int q = 0; q < COLS / 2; ++q) sum[q] = 0;
-            for (int i = 0; i < n && ok; ++i, ++it) {
-                const int d = it & 1;
-                float* const buffer = mine + d * COLS;
+            for (int i0 = 0; i0 < n && ok; i0 += BATCH, ++bt) {
+                const int s = bt % S_STAGES;
+                ok = mbar_wait(s_full + 8 * s, (bt / S_STAGES) & 1, abort_flag, p.err_flag);
+                const float* sx = reinterpret_cast<const float*>(gen + L::SX_OFF) + s * BATCH * TN + col0;
+                const float* sw = reinterpret_cast<const float*>(gen + L::SW_OFF) + s * BATCH * FEATURES + row;
+                const int most = min(BATCH, n - i0);
+                for (int j = 0; j < most; ++j, ++it, sx += TN, sw += FEATURES) {
+                    const int d = it & 1;
+                    ok = mbar_wait(acc_full + 8 * d, (it >> 1) & 1, abort_flag, p.err_flag) && ok;
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    int v[COLS];
 #pragma unroll
-                for (int q = 0; q < PER_LANE; ++q) buffer[q * 32 + lane] = x_ahead[0][q];
-                const uint64_t scale = pack2(w_ahead[0], w_ahead[0]);
-#pragma unroll
-                for (int a = 0; a + 1 < AHEAD; ++a) {
-                    w_ahead[a] = w_ahead[a + 1];
-#pragma unroll
-                    for (int q = 0; q < PER_LANE; ++q) x_ahead[a][q] = x_ahead[a + 1][q];
-                }
-                ask(i + AHEAD, x_ahead[AHEAD - 1], w_ahead[AHEAD - 1]);
-                ok = mbar_wait(acc_full + 8 * d, (it >> 1) & 1, abort_flag, p.err_flag);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                __syncwarp();      // the scales written above are there
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                for (int c = 0; c < COLS; c += 16) {
-                    int v[16];
-                    tmem_ld16(tmem + lanes + d * TN + col0 + c, v);
+                    for (int c = 0; c < COLS; c += 16) tmem_ld16(tmem + lanes + d * TN + col0 + c, v + c);
+                    const uint64_t scale = pack2(*sw, *sw);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty + 8 * d);
 #pragma unroll
-                    for (int q = 0; q < 16; q += 4) {
-                        const ulonglong2 x4 = *reinterpret_cast<const ulonglong2*>(buffer + c + q);
-                        uint64_t& s0 = sum[(c + q) / 2];
-                        uint64_t& s1 = sum[(c + q) / 2 + 1];
-                        s0 = fma2(mul2(pack2((float)v[q], (float)v[q + 1]), x4.x), scale, s0);
-                        s1 = fma2(mul2(pack2((float)v[q + 2], (float)v[q + 3]), x4.y), scale, s1);
+                    for (int q = 0; q < COLS; q += 4) {
+                        const ulonglong2 x4 = *reinterpret_cast<const ulonglong2*>(sx + q);
+                        sum[q / 2] = fma2(mul2(pack2((float)v[q], (float)v[q + 1]), x4.x), scale, sum[q / 2]);
+                        sum[q / 2 + 1] = fma2(mul2(pack2((float)v[q + 2], (float)v[q + 3]), x4.y), scale, sum[q / 2 + 1]);
                     }
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty + 8 * d);
+                if (lane == 0) mbar_arrive(s_empty + 8 * s);
             }
-            if (ok && f < p.N) {
-                T* out = (T*)p.out + (size_t)split * p.M * p.N + (size_t)t0 * p.N + f;
+            if (ok && f0 + row < p.N) {
+                T* out = (T*)p.out + (size_t)split * p.M * p.N + (size_t)(t0 + col0) * p.N + f0 + row;
 #pragma unroll
                 for (int q = 0; q < COLS; ++q) {
                     const uint32_t bits = q & 1 ? (uint32_t)(sum[q / 2] >> 32) : (uint32_t)sum[q / 2];
-                    if (t0 + q < p.M) ElemOps<T>::store(out + (size_t)q * p.N, __uint_as_float(bits));
+                    if (t0 + col0 + q < p.M) ElemOps<T>::store(out + (size_t)q * p.N, __uint_as_float(bits));
                 }
             }
         }
