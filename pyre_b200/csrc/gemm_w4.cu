@@ -102,8 +102,8 @@ int launch_few(const W4Params& p, cudaStream_t stream) {
 //                        is where the MMAs take their A operand from.
 //   warp 1, one thread : four MMAs (kind::i8, 32 k each) a group, into one of two accumulators of 32-bit integers.
 //   warps 2, 3         : the scales of four groups at a time, of features and of tokens, to shared memory.
-//   warps 8..23        : a thread owns a feature and a quarter of the tokens.  The group's integers come out of tensor memory at once, which frees the
-//                        accumulator, are scaled by token and by feature and added to float sums in registers, by ascending group.
+//   warps 8..23        : a thread owns a feature and a quarter of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
+//                        feature and added to float sums in registers, by ascending group.
 // An output tile whose K is shared among CTAs (few tiles) leaves float shares, added up in order by whoever reads them.
 // ---------------------------------------------------------------------------
 constexpr int ERR_TIMEOUT = 2;
@@ -120,6 +120,7 @@ struct ManyParams {
     int M, N, G;
     int tiles_m, tiles;           // tiles of tokens (fastest); of everything
     int splits, per_split;        // of K, in groups
+    int vec;                      // output rows lie on 16-byte boundaries
     int* err_flag;
 };
 
@@ -130,6 +131,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
     const long long t0 = clock64();
     while (!mbar_try_wait(bar, parity) && clock64() - t0 < PYRE_WAIT_CYCLES) {}
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 // D (tensor memory, 32-bit integers) += A (tensor memory, signed bytes) * B (shared memory, signed bytes)
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
@@ -167,7 +173,8 @@ template <int TN> struct Many {
     static constexpr int X_BYTES = TN * GROUP;
     static constexpr int W_OFF = 0, X_OFF = W_STAGES * W_BYTES;
     static constexpr int SX_OFF = X_OFF + STAGES * X_BYTES, SW_OFF = SX_OFF + S_STAGES * BATCH * TN * 4;      // [stage][group][token], [..][feature]
-    static constexpr int BARS = SW_OFF + S_STAGES * BATCH * FEATURES * 4;
+    static constexpr int OUT_OFF = SW_OFF + S_STAGES * BATCH * FEATURES * 4;      // [warp][16 tokens][32 features] floats
+    static constexpr int BARS = OUT_OFF + EPI_WARPS * 512 * 4;
     static constexpr int N_BARS = 2 * (W_STAGES + STAGES + S_STAGES + 2) + 1;
     static constexpr int TOTAL = BARS + N_BARS * 8 + 24 + 1024;
     static constexpr int A_COL0 = 2 * TN;
@@ -261,33 +268,39 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // D 32-bit integers (2 at bit 4), A and B signed bytes (1 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24
-            constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(FEATURES >> 4) << 24);
-            const uint64_t db0 = umma_desc(base + L::X_OFF);
-            int it = 0, s = 0;
-            bool ok = true;
-            pdl_wait();      // no bounded wait should have to last as long as the kernels before
-            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-                range(item, f0, t0, split, first, n);
-                for (int i = 0; i < n; ++i, ++it) {
-                    const int d = it & 1;
-                    ok = mbar_wait(acc_empty + 8 * d, ((it >> 1) & 1) ^ 1, abort_flag, p.err_flag) &&
-                         mbar_wait(ab_full + 8 * s, (it / STAGES) & 1, abort_flag, p.err_flag);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t db = db0 + s * (L::X_BYTES >> 4);
-                    const uint32_t a = tmem + L::A_COL0 + s * A_COLS;
+        // D 32-bit integers (2 at bit 4), A and B signed bytes (1 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24
+        constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(FEATURES >> 4) << 24);
+        const uint64_t db0 = umma_desc(base + L::X_OFF);
+        const bool elected = elect_one();      // the whole warp goes through the loop, so that the operands stay in uniform registers
+        int it = 0, s = 0;
+        bool ok = true;
+        pdl_wait();      // no bounded wait should have to last as long as the kernels before
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+            range(item, f0, t0, split, first, n);
+            for (int i = 0; i < n; ++i, ++it) {
+                const int d = it & 1;
+                ok = mbar_wait(acc_empty + 8 * d, ((it >> 1) & 1) ^ 1, abort_flag, p.err_flag) &&
+                     mbar_wait(ab_full + 8 * s, (it / STAGES) & 1, abort_flag, p.err_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t db = db0 + s * (L::X_BYTES >> 4);
+                const uint32_t a = tmem + L::A_COL0 + s * A_COLS;
+                if (elected) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) umma_i8(tmem + d * TN, a + 8 * q, db + 2 * q, idesc, q > 0);      // 32 bytes of k further
                     umma_commit(acc_full + 8 * d);
                     umma_commit(ab_empty + 8 * s);
-                    s = s + 1 == STAGES ? 0 : s + 1;
                 }
+                __syncwarp();
+                s = s + 1 == STAGES ? 0 : s + 1;
             }
+        }
+        if (elected) {
             umma_commit(drained);      // the MMAs end before tensor memory is given back, also where a wait ran out
             mbar_drain(drained, 0);
         }
+        __syncwarp();
     } else if (warp < 4) {
         // warp 2: the tokens' scales, warp 3: the features' (a sixteenth of them: the integers are sixteen times as large)
         bool ok = true;
@@ -396,12 +409,43 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_empty + 8 * s);
             }
-            if (ok && f0 + row < p.N) {
-                T* out = (T*)p.out + (size_t)split * p.M * p.N + (size_t)(t0 + col0) * p.N + f0 + row;
+            if (!ok) break;
+            // The tile leaves by whole 16-byte pieces, 16 tokens at a time through shared memory: single elements (32 stores a thread) took a fifth of the
+            // kernel's time, while the accumulators waited.  Rows off 16-byte boundaries leave by elements.
+            T* const out = (T*)p.out + (size_t)split * p.M * p.N;
+            constexpr int PIECE = 16 / sizeof(T), PIECES = 32 / PIECE, ROWS = 32 / PIECES;      // elements; a warp's features in pieces; rows at a time
+            const int left = p.M - t0 - col0;
 #pragma unroll
-                for (int q = 0; q < COLS; ++q) {
-                    const uint32_t bits = q & 1 ? (uint32_t)(sum[q / 2] >> 32) : (uint32_t)sum[q / 2];
-                    if (t0 + col0 + q < p.M) ElemOps<T>::store(out + (size_t)q * p.N, __uint_as_float(bits));
+            for (int c = 0; c < COLS; c += 16) {
+                if (p.vec) {
+                    float* const stage = reinterpret_cast<float*>(gen + L::OUT_OFF) + (warp - EPI_WARP0) * 512;
+                    __syncwarp();
+#pragma unroll
+                    for (int q = 0; q < 16; q += 2) {
+                        stage[q * 32 + lane] = __uint_as_float((uint32_t)sum[(c + q) / 2]);
+                        stage[(q + 1) * 32 + lane] = __uint_as_float((uint32_t)(sum[(c + q) / 2] >> 32));
+                    }
+                    __syncwarp();
+                    const int f = f0 + quarter * 32 + lane % PIECES * PIECE;
+#pragma unroll
+                    for (int t = lane / PIECES; t < 16; t += ROWS) {
+                        Vec<T, PIECE> v;
+#pragma unroll
+                        for (int k = 0; k < PIECE; k += 4) {
+                            const float4 a = *reinterpret_cast<const float4*>(stage + t * 32 + lane % PIECES * PIECE + k);
+                            v.v[k] = from_f32<T>(a.x);
+                            v.v[k + 1] = from_f32<T>(a.y);
+                            v.v[k + 2] = from_f32<T>(a.z);
+                            v.v[k + 3] = from_f32<T>(a.w);
+                        }
+                        if (c + t < left && f < p.N) store_vec<T, PIECE>(out + (size_t)(t0 + col0 + c + t) * p.N + f, v);
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        const uint32_t bits = q & 1 ? (uint32_t)(sum[(c + q) / 2] >> 32) : (uint32_t)sum[(c + q) / 2];
+                        if (c + q < left && f0 + row < p.N) ElemOps<T>::store(out + (size_t)(t0 + col0 + c + q) * p.N + f0 + row, __uint_as_float(bits));
+                    }
                 }
             }
         }
@@ -450,7 +494,7 @@ int launch_many(const W4Params& w, int splits, int* err_flag, cudaStream_t strea
     }
     CUtensorMap mw, mx;
     if (!byte_map(&mw, w.packed, w.N, 64ll * w.G, 64, FEATURES) || !byte_map(&mx, w.rows, w.M, 128ll * w.G, 128, TN)) return PYRE_ERR_BAD_ARG;
-    ManyParams p = {w.row_scales, w.ld_scales, w.scales, w.out, w.M, w.N, w.G, ceil_div(w.M, TN), 0, splits, ceil_div(w.G, splits), err_flag};
+    ManyParams p = {w.row_scales, w.ld_scales, w.scales, w.out, w.M, w.N, w.G, ceil_div(w.M, TN), 0, splits, ceil_div(w.G, splits), w.N % (16 / (int)sizeof(T)) == 0 && !((uintptr_t)w.out & 15), err_flag};
     const long long tiles = (long long)p.tiles_m * ceil_div(w.N, FEATURES);
     if (tiles * splits > 0x7fffffffll) return PYRE_ERR_UNSUPPORTED;
     p.tiles = (int)tiles;
