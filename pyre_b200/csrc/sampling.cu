@@ -176,19 +176,23 @@ PYRE_API int pyre_sample(const float* logits, long long ld, const float* tempera
 // All three keep a prefix of the order.  The token is argmax over it of (l_i - max l) / T + g(seed, index, i), the noise of the kernels
 // above.  A row without a filter is chosen from as above, bit for bit; a NaN counts as -inf.
 //
-// A cluster of CTAs shares a row; each keeps its slice in shared memory, so the row is read from memory once.  Masses are whole numbers
+// A cluster of CTAs shares a row; each keeps its slice in shared memory where it fits.  Masses are whole numbers
 // (w 2^31, summed in 64 bits), so neither the order of the additions nor the cluster's size can move a border: results do not depend on them.
 //   1. max l.
-//   2. a histogram by distance from it in steps of 1/64 (count and mass per step; l decides the step alone and in order): the step in which
-//      the k-th token or the p-th part of the mass lies.
-//   3. that step's tokens, a few hundred as a rule, go to one CTA's list and are ranked by (l, index): the border token.  If they are more than
-//      the list holds, their span of (l, index) is cut into as many steps again, until they fit.
-//   4. noise for the tokens up to the border.
+//   2. a histogram by distance from it in steps of 1/64 (count and mass per step; l decides the step alone and in order), of the tokens less than
+//      NEAR steps away; the others' mass stays in registers.  The step in which the k-th token or the p-th part of the mass lies follows.
+//   3. the tokens up to that step, some hundreds as a rule, go to the first CTA's list, and the others are done.  It ranks the ones of that step by
+//      (l, index): the border token; and once more for p after k.  Then noise for the tokens up to the border.
+// Where the border lies further away, or more tokens lie before it than the list holds (flat rows, rows of equal entries):
+//   2. the histogram of all tokens,
+//   3. the border step's tokens alone go to the list; if they are more than it holds, their span of (l, index) is cut into as many steps again, until
+//      they fit.
+//   4. all CTAs look for the tokens up to the border.
 // ---------------------------------------------------------------------------
 namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
-constexpr int F_THREADS = 512, F_WARPS = F_THREADS / 32, BINS = 2048, LISTED = 512, MAX_CLUSTER = 8;
+constexpr int F_THREADS = 512, F_WARPS = F_THREADS / 32, BINS = 2048, NEAR = F_THREADS, LISTED = 512, NEAR_LISTED = 2048, MAX_CLUSTER = 8;
 constexpr float BINS_PER_NAT = 64.f;
 
 struct FilterParams {
@@ -206,13 +210,25 @@ struct FilterParams {
 };
 
 struct FilterShared {
-    unsigned count[BINS], low[BINS], high[BINS];      // mass: high 2^32 + low
+    unsigned near_count[NEAR], near_low[NEAR], near_high[NEAR];      // mass: high 2^32 + low
+    union {
+        struct {
+            unsigned count[BINS], low[BINS], high[BINS];
+        };
+        struct {
+            u64 near_list[NEAR_LISTED];
+            unsigned near_mass[NEAR_LISTED];
+        };
+    };
     u64 list[LISTED];
     unsigned list_mass[LISTED];
     u64 slots[2][MAX_CLUSTER][2];                     // what the cluster's CTAs tell each other
     u64 warp_u64[2][F_WARPS];
     Best warp_best[F_WARPS];
     Best cluster_best[MAX_CLUSTER];
+    unsigned near_listed;
+    int near_step;                                    // the tokens up to this step are listed; < 0: too far or too many
+    u64 rest;                                         // the mass beyond the near steps
     // the step that a search ended in (`above`: before it), or the border
     int step;
     u64 above_count, above_mass, inside, border, border_mass;
@@ -262,16 +278,18 @@ sample_filtered_kernel(const FilterParams p) {
         cluster.sync();
         return at;
     };
-    auto finish = [&](Best best) {
+    auto best_of_block = [&](Best& best) {      // in thread 0
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
             best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.score, o), __shfl_xor_sync(0xffffffffu, best.index, o)});
         if (lane == 0) sh.warp_best[warp] = best;
         __syncthreads();
-        if (tid == 0) {
+        if (tid == 0)
             for (int w = 1; w < F_WARPS; ++w) best = better(best, sh.warp_best[w]);
-            cluster.map_shared_rank(&sh, 0)->cluster_best[rank] = best;
-        }
+    };
+    auto finish = [&](Best best) {
+        best_of_block(best);
+        if (tid == 0) cluster.map_shared_rank(&sh, 0)->cluster_best[rank] = best;
         cluster.sync();
         if (rank == 0 && tid == 0) {
             for (int c = 1; c < C; ++c) best = better(best, sh.cluster_best[c]);
@@ -292,29 +310,48 @@ sample_filtered_kernel(const FilterParams p) {
     // 1. the slice, and the largest entry
     const float* held = row + begin;
     float most = -INFINITY;
-    {
-        const float* src = row + begin;
-        const int shift = (int)(((uintptr_t)src >> 2) & 3), head = min(n, (4 - shift) & 3), body = (n - head) / 4;
-        float* mine = reinterpret_cast<float*>(dyn) + shift;      // the same place within 16 bytes
-        auto take = [&](int i) {
-            const float l = entry(src[i]);
-            most = fmaxf(most, l);
-            if (p.resident) mine[i] = l;
-        };
-        if (tid < head) take(tid);
-        for (int i = tid; i < body; i += F_THREADS) {
-            float4 v = *reinterpret_cast<const float4*>(src + head + 4 * i);
-            v = make_float4(entry(v.x), entry(v.y), entry(v.z), entry(v.w));
-            most = fmaxf(most, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-            if (p.resident) *reinterpret_cast<float4*>(mine + head + 4 * i) = v;
+    const int shift16 = (int)(((uintptr_t)held >> 2) & 3), head = min(n, (4 - shift16) & 3), body = (n - head) / 4;
+    // f(four entries, the index of the first) for all of the slice, by whole vectors but for its ends (of which the first entry alone counts)
+    auto vectors = [&](const float* src, auto f) {
+        if (tid < head) f(make_float4(entry(src[tid]), -INFINITY, -INFINITY, -INFINITY), tid, 1);
+        constexpr int AHEAD = 4;
+        for (int i = tid; i < body; i += AHEAD * F_THREADS) {
+            float4 v[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+                if (i + q * F_THREADS < body) v[q] = *reinterpret_cast<const float4*>(src + head + 4 * (i + q * F_THREADS));
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+                if (i + q * F_THREADS < body)
+                    f(make_float4(entry(v[q].x), entry(v[q].y), entry(v[q].z), entry(v[q].w)), head + 4 * (i + q * F_THREADS), 4);
         }
-        if (head + 4 * body + tid < n) take(head + 4 * body + tid);
+        const int last = head + 4 * body + tid;
+        if (last < n) f(make_float4(entry(src[last]), -INFINITY, -INFINITY, -INFINITY), last, 1);
+    };
+    {
+        float* const mine = reinterpret_cast<float*>(dyn) + shift16;      // the same place within 16 bytes
+        vectors(held, [&](const float4& v, int i, int count) {
+            most = fmaxf(most, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+            if (!p.resident) return;
+            if (count == 4) *reinterpret_cast<float4*>(mine + i) = v;
+            else mine[i] = v.x;
+        });
         if (p.resident) held = mine;
     }
+    // f(entry, its index) for all of the slice
+    auto entries = [&](auto f) {
+        vectors(held, [&](const float4& v, int i, int count) {
+            f(v.x, i);
+            if (count == 4) { f(v.y, i + 1); f(v.z, i + 2); f(v.w, i + 3); }
+        });
+    };
     most = warp_max(most);
     if (lane == 0) sh.warp_best[warp].score = most;
-    for (int b = tid; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
-    if (tid == 0) sh.listed = 0;
+    sh.near_count[tid] = sh.near_low[tid] = sh.near_high[tid] = 0;
+    if (tid == 0) {
+        sh.listed = sh.near_listed = 0;
+        sh.rest = 0;
+    }
     __syncthreads();
     if (tid < C)
         for (int w = 0; w < F_WARPS; ++w) most = fmaxf(most, sh.warp_best[w].score);
@@ -418,11 +455,12 @@ sample_filtered_kernel(const FilterParams p) {
         for (int level = 0; sh.inside > LISTED && level < 7; ++level) {      // 64 bits, eleven a time
             if (!spanned) {
                 u64 low = ~0ull, high = 0;
-                for (int i = tid; i < n; i += F_THREADS)
-                    if (inside(held[i], i)) {
-                        low = min(low, composite(held[i], i));
-                        high = max(high, composite(held[i], i));
+                entries([&](float l, int i) {
+                    if (inside(l, i)) {
+                        low = min(low, composite(l, i));
+                        high = max(high, composite(l, i));
                     }
+                });
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) {
                     low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
@@ -450,18 +488,16 @@ sample_filtered_kernel(const FilterParams p) {
             cluster.sync();      // all have read the last histogram and what it gave
             for (int b = tid; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
             __syncthreads();
-            for (int i = tid; i < n; i += F_THREADS) {
-                const float l = held[i];
+            entries([&](float l, int i) {
                 if (inside(l, i)) tally((int)((to - composite(l, i)) >> shift), mass_of(distance(l)));
-            }
+            });
             locate(mass, target, before_count, before_mass, true);
             to -= (u64)sh.step << shift;
             from = max(from, to - ((1ull << shift) - 1));
         }
         // the tokens of the span, ranked by the first CTA
         FilterShared* const lead = cluster.map_shared_rank(&sh, 0);
-        for (int i = tid; i < n; i += F_THREADS) {
-            const float l = held[i];
+        entries([&](float l, int i) {
             if (inside(l, i)) {
                 const unsigned at = atomicAdd(&lead->listed, 1u);
                 if (at < LISTED) {
@@ -469,7 +505,7 @@ sample_filtered_kernel(const FilterParams p) {
                     lead->list_mass[at] = mass_of(distance(l));
                 }
             }
-        }
+        });
         cluster.sync();
         if (rank == 0) {
             const int count = min((int)sh.listed, LISTED);
@@ -497,12 +533,158 @@ sample_filtered_kernel(const FilterParams p) {
         cluster.sync();
         return;
     }
+    auto clear = [&]() {
+        for (int b = tid; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
+        __syncthreads();
+    };
+    auto share = [&](u64 whole) { return max(1ull, (u64)ceil((double)top_p * (double)whole)); };
+    auto score = [&](float l, unsigned index) {
+        const float d = distance(l);
+        if (min_p > 0.f && !(expf(-d) >= min_p)) return;
+        const float s = entry(__fadd_rn(-d, gumbel(seed, tix, index)));
+        best = better(best, Best{s, (int)index});
+    };
     if (by_count || by_mass) {
-        auto histogram = [&]() {
-            for (int i = tid; i < n; i += F_THREADS) {
-                const float d = distance(held[i]);
-                tally(first_step(d), mass_of(d));
+        FilterShared* const lead = cluster.map_shared_rank(&sh, 0);
+        // 2. the near steps; what lies beyond them counts where the whole mass is wanted
+        u64 rest = 0;
+        entries([&](float l, int) {
+            const float d = distance(l);
+            if (d * BINS_PER_NAT < (float)NEAR) {
+                const int b = first_step(d);
+                const unsigned f = mass_of(d);
+                atomicAdd(&sh.near_count[b], 1u);
+                const unsigned old = atomicAdd(&sh.near_low[b], f);
+                if (old + f < old) atomicAdd(&sh.near_high[b], 1u);
             }
+            else if (!by_count && d < 23.f) rest += mass_of(d);      // (below 2^-32 beyond)
+        });
+        if (!by_count) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+            if (lane == 0 && rest) atomicAdd(&lead->rest, rest);
+        }
+        __syncthreads();
+        if (rank != 0) {
+            const unsigned count = sh.near_count[tid], low = sh.near_low[tid];
+            if (count) {
+                atomicAdd(&lead->near_count[tid], count);
+                const unsigned old = atomicAdd(&lead->near_low[tid], low);
+                const unsigned high = sh.near_high[tid] + (old + low < old);
+                if (high) atomicAdd(&lead->near_high[tid], high);
+            }
+        }
+        cluster.sync();
+        // the steps' sums up to and with each one of the first CTA's threads', and the search among them
+        u64 counts = 0, masses = 0, c_up = 0, m_up = 0, target = k;
+        auto near_step = [&](bool mass, u64 target) {      // all threads of the first CTA; the step in sh.step, what is before it in sh.above_*
+            if (tid == 0) sh.step = -1;
+            __syncthreads();
+            if ((mass ? m_up : c_up) >= target && (mass ? m_up - masses : c_up - counts) < target) {
+                sh.step = tid;
+                sh.above_count = c_up - counts;
+                sh.above_mass = m_up - masses;
+                sh.inside = counts;
+            }
+            __syncthreads();
+        };
+        if (rank == 0) {
+            counts = c_up = sh.near_count[tid];
+            masses = m_up = ((u64)sh.near_high[tid] << 32) + sh.near_low[tid];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 x = __shfl_up_sync(0xffffffffu, c_up, o), y = __shfl_up_sync(0xffffffffu, m_up, o);
+                if (lane >= o) { c_up += x; m_up += y; }
+            }
+            if (lane == 31) { sh.warp_u64[0][warp] = c_up; sh.warp_u64[1][warp] = m_up; }
+            __syncthreads();
+            u64 m_all = 0;
+            for (int w = 0; w < F_WARPS; ++w) {
+                if (w < warp) { c_up += sh.warp_u64[0][w]; m_up += sh.warp_u64[1][w]; }
+                m_all += sh.warp_u64[1][w];
+            }
+            if (!by_count) target = share(m_all + sh.rest);
+            near_step(!by_count, target);
+            if (tid < C) {
+                const bool fits = sh.step >= 0 && sh.above_count + sh.inside <= NEAR_LISTED;
+                cluster.map_shared_rank(&sh, tid)->near_step = fits ? sh.step : -1;
+            }
+        }
+        cluster.sync();
+        const int near = sh.near_step;
+        if (near >= 0) {
+            // 3. the tokens up to that step
+            entries([&](float l, int i) {
+                if (distance(l) * BINS_PER_NAT < (float)(near + 1)) {
+                    const unsigned at = atomicAdd(&lead->near_listed, 1u);
+                    if (at < NEAR_LISTED) {
+                        lead->near_list[at] = composite(l, i);
+                        lead->near_mass[at] = mass_of(distance(l));
+                    }
+                }
+            });
+            cluster.sync();
+            if (rank != 0) return;      // nothing of theirs is read any more
+            const int listed = min((int)sh.near_listed, NEAR_LISTED);
+            auto value = [&](u64 key) {
+                const unsigned u = (unsigned)(key >> 32);
+                return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+            };
+            // the border token, from the ones of sh.step alone where they fit into the short list, else from all listed ones
+            auto rank_step = [&](bool mass, u64 target) {
+                const bool brief = sh.inside <= LISTED;
+                if (brief) {
+                    for (int q = tid; q < listed; q += F_THREADS) {
+                        const u64 key = sh.near_list[q];
+                        if (first_step(distance(value(key))) == sh.step) {
+                            const unsigned at = atomicAdd(&sh.listed, 1u);
+                            if (at < LISTED) {
+                                sh.list[at] = key;
+                                sh.list_mass[at] = sh.near_mass[q];
+                            }
+                        }
+                    }
+                    __syncthreads();
+                }
+                const int count = brief ? min((int)sh.listed, LISTED) : listed;
+                const u64* const keys = brief ? sh.list : sh.near_list;
+                const unsigned* const of = brief ? sh.list_mass : sh.near_mass;
+                for (int q = tid; q < count; q += F_THREADS) {
+                    const u64 key = keys[q], own = of[q];
+                    u64 c_at = brief ? sh.above_count : 0, m_at = brief ? sh.above_mass : 0;
+                    for (int j = 0; j < count; ++j)
+                        if (keys[j] > key) { ++c_at; m_at += of[j]; }
+                    if (mass ? m_at < target && m_at + own >= target : c_at + 1 == target) {
+                        sh.border = key;
+                        sh.border_mass = m_at + own;
+                    }
+                }
+                __syncthreads();
+                if (tid == 0) sh.listed = 0;
+                __syncthreads();
+            };
+            rank_step(!by_count, target);
+            if (by_count && by_mass) {
+                target = share(sh.border_mass);
+                near_step(true, target);
+                rank_step(true, target);
+            }
+            const u64 border = sh.border;
+            for (int q = tid; q < listed; q += F_THREADS) {
+                const u64 key = sh.near_list[q];
+                if (key >= border) score(value(key), ~(unsigned)key);
+            }
+            best_of_block(best);
+            if (tid == 0) p.out[r] = best.index == 0x7fffffff ? 0 : best.index;
+            return;
+        }
+        // (flat rows) all steps
+        auto histogram = [&]() {
+            clear();
+            entries([&](float l, int) {
+                const float d = distance(l);
+                tally(first_step(d), mass_of(d));
+            });
         };
         histogram();
         u64 whole = 0;
@@ -511,9 +693,7 @@ sample_filtered_kernel(const FilterParams p) {
             search(false, (u64)k, true);
             border = sh.border;
             whole = sh.border_mass;
-            if (by_mass) {      // the first histogram again (the search may have cut it into finer steps)
-                __syncthreads();
-                for (int b = tid; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
+            if (by_mass) {      // the first histogram again (the search has added it up, or cut it into finer steps)
                 __syncthreads();
                 histogram();
             }
@@ -522,32 +702,29 @@ sample_filtered_kernel(const FilterParams p) {
             added = true;
         }
         if (by_mass) {
-            search(true, max(1ull, (u64)ceil((double)top_p * (double)whole)), !added);
+            search(true, share(whole), !added);
             border = sh.border;
         }
     }
-    for (int i = tid; i < n; i += F_THREADS) {
-        const float l = held[i];
-        if (composite(l, i) < border) continue;
-        const float d = distance(l);
-        if (min_p > 0.f && !(expf(-d) >= min_p)) continue;
-        const float s = entry(__fadd_rn(-d, gumbel(seed, tix, (unsigned)(begin + i))));
-        if (s > best.score || best.index == 0x7fffffff) best = Best{s, begin + i};
-    }
+    entries([&](float l, int i) {
+        if (composite(l, i) >= border) score(l, (unsigned)(begin + i));
+    });
     finish(best);
 }
 }  // namespace
 
 // logits [R, V] fp32 with row stride ld; temperature [R], seeds [R], token_index [R] (null where all rows are greedy); top_k [R] int32 (0: all), top_p [R]
 // (1: all), min_p [R] (0: all), each may be null; out [R] int32.
+// cluster: CTAs per row (1, 2, 4, 8), 0 for the kernel's own choice.
 PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float* temperature, const unsigned long long* seeds,
                                   const int* token_index, const int* top_k, const float* top_p, const float* min_p, int* out, int n_rows,
-                                  int V, cudaStream_t stream) {
+                                  int V, int cluster, cudaStream_t stream) {
     if (n_rows <= 0) return 0;
     if (V <= 0 || (temperature && (!seeds || !token_index))) return PYRE_ERR_BAD_ARG;
+    if (cluster < 0 || cluster > MAX_CLUSTER || (cluster & (cluster - 1))) return PYRE_ERR_BAD_ARG;
     // CTAs per row: as many as keep two to an SM busy, and as two slices in an SM's shared memory ask for
-    int C = 1;
-    while (C < MAX_CLUSTER && ((n_rows * (long long)C < 2 * pyre_sm_count() && V > 2048 * C) || ceil_div(V, C) > 76 * 256)) C *= 2;
+    int C = cluster > 0 ? cluster : 1;
+    while (!cluster && C < MAX_CLUSTER && ((n_rows * (long long)C < 2 * pyre_sm_count() && V > 2048 * C) || ceil_div(V, C) > 76 * 256)) C *= 2;
     FilterParams p = {logits, ld, temperature, seeds, token_index, top_k, top_p, min_p, out, V, (ceil_div(V, C) + 3) / 4 * 4, 0};
     size_t bytes = (size_t)p.slice * 4 + 16;
     p.resident = bytes <= 190 * 1024;

@@ -38,7 +38,7 @@ SIGNATURES: dict[str, tuple[str, list]] = {
     "pyre_scale_rows": ("elementwise", [P, P, I, P, I, I, F, P]),
     "pyre_sample": ("sampling", [P, LL, P, P, P, P, I, I, P, P]),
     "pyre_sample_slices": ("sampling", [I]),
-    "pyre_sample_filtered": ("sampling", [P, LL, P, P, P, P, P, P, P, I, I, P]),
+    "pyre_sample_filtered": ("sampling", [P, LL, P, P, P, P, P, P, P, I, I, I, P]),
     "pyre_paged_attention_generic": ("attention_generic", [P, P, P, P, I, P, P, I, I, I, I, I, I, I, F, F, P, I, LL, P, I, I, P]),
     "pyre_sgemm_nt": ("gemm_f32", [P, LL, P, LL, P, LL, P, I, I, I, P]),
     "pyre_fixed_exponents": ("gemm_fixed", [P, LL, I, I, P, P, P]),

@@ -598,6 +598,9 @@ def delay(milliseconds: float) -> None:
     lib.call("pyre_delay", int(milliseconds * 1e6), _stream())
 
 
+_SAMPLE_CLUSTER = 0      # CTAs per row of ``pyre_sample_filtered``, 0 for the kernel's own choice (a row's token does not depend on it)
+
+
 def sample(logits: torch.Tensor, temperature: "torch.Tensor | None" = None, seeds: "torch.Tensor | None" = None,
            token_index: "torch.Tensor | None" = None, out: "torch.Tensor | None" = None, top_k: "torch.Tensor | None" = None,
            top_p: "torch.Tensor | None" = None, min_p: "torch.Tensor | None" = None) -> torch.Tensor:
@@ -632,7 +635,7 @@ def sample(logits: torch.Tensor, temperature: "torch.Tensor | None" = None, seed
         if not V:
             raise ValueError("rows of logits need an entry")
         lib.call("pyre_sample_filtered", logits.data_ptr(), logits.stride(0), temperature.data_ptr(), seeds.data_ptr(), token_index.data_ptr(), _ptr(top_k),
-                 _ptr(top_p), _ptr(min_p), out.data_ptr(), R, V, _stream())
+                 _ptr(top_p), _ptr(min_p), out.data_ptr(), R, V, _SAMPLE_CLUSTER, _stream())
         return out
     slices = lib.call_value("pyre_sample_slices", V)
     scratch = torch.empty(R * slices * 2, dtype=torch.int32, device=logits.device) if slices else None

@@ -176,6 +176,27 @@ def test_a_rows_token_does_not_depend_on_the_batch():
     assert torch.equal(call(table[10:50, 1:V + 1], *few), ids[10:50])
 
 
+@pytest.mark.parametrize("form", ["normal", "coarse", "flat", "equal", "peaked"])
+def test_any_number_of_ctas_per_row_gives_the_same(form, monkeypatch):
+    """Borders are found in whole numbers: 1 to 8 CTAs per row agree to the bit, on rows whose borders lie near the best token or far, or among ties."""
+    from pyre_b200.kernels import ops
+    R, V = 45, 60001
+    logits = torch.randn((R, V), generator=gen(77), device="cuda") * {"normal": 2, "coarse": 2, "flat": 0.01, "equal": 0, "peaked": 0.5}[form]
+    if form == "coarse":
+        logits = (logits * 2).round() / 2
+    if form == "peaked":
+        logits[:, 100:140] += 9
+    rule = rules(123, R)
+    want = None
+    for cluster in (0, 1, 2, 4, 8):
+        monkeypatch.setattr(ops, "_SAMPLE_CLUSTER", cluster)
+        ids = call(logits, *rule)
+        if want is None:
+            check(ids, logits, *rule)
+            want = ids
+        assert torch.equal(ids, want), cluster
+
+
 def test_draws_follow_the_distribution():
     """Many draws of one row: frequencies against the renormalised probabilities of the kept tokens.  4,096 draws; a count's deviation is at most
     sqrt(n / 4) = 32, so five of them bound each of the few counts with a chance of error below 1e-5."""
