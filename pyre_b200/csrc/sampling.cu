@@ -176,24 +176,27 @@ PYRE_API int pyre_sample(const float* logits, long long ld, const float* tempera
 // All three keep a prefix of the order.  The token is argmax over it of (l_i - max l) / T + g(seed, index, i), the noise of the kernels
 // above.  A row without a filter is chosen from as above, bit for bit; a NaN counts as -inf.
 //
-// A cluster of CTAs shares a row; each keeps its slice in shared memory where it fits.  Masses are whole numbers
-// (w 2^31, summed in 64 bits), so neither the order of the additions nor the cluster's size can move a border: results do not depend on them.
-//   1. max l.
-//   2. a histogram by distance from it in steps of 1/64 (count and mass per step; l decides the step alone and in order), of the tokens less than
-//      NEAR steps away; the others' mass stays in registers.  The step in which the k-th token or the p-th part of the mass lies follows.
-//   3. the tokens up to that step, some hundreds as a rule, go to the first CTA's list, and the others are done.  It ranks the ones of that step by
-//      (l, index): the border token; and once more for p after k.  Then noise for the tokens up to the border.
-// Where the border lies further away, or more tokens lie before it than the list holds (flat rows, rows of equal entries):
-//   2. the histogram of all tokens,
-//   3. the border step's tokens alone go to the list; if they are more than it holds, their span of (l, index) is cut into as many steps again, until
-//      they fit.
-//   4. all CTAs look for the tokens up to the border.
+// A cluster of CTAs shares a row; each keeps its slice in shared memory where two such CTAs fit on an SM, else it reads it again (out of L2).  Masses
+// are whole numbers (w 2^31, summed in 64 bits), so neither the order of the additions nor the cluster's size can move a border: results do
+// not depend on them.
+//   1. max l, and the largest entry that each thread has read.
+//   2. k: as many threads as k have read an entry of at least t, where t is the k-th of those (or somewhat below): no token below t is among the first k.  The
+//      tokens from t on, hardly more than k, go to the first CTA's list, and the other CTAs are done.  It ranks them by (l, index), which gives the
+//      border token of k and of p after k, and adds the noise.
+//   2'. p alone: a histogram of masses by distance (max l - l) / T in steps of 1/64 (l decides the step alone and in order) of the tokens less than NEAR steps
+//      away; the others' mass stays in registers.  It gives the step in which the p-th part of the mass lies, whose tokens go to the list and are
+//      ranked.  All CTAs look for the tokens up to the border.
+//   3'. The tokens up to the border are gathered before they get their noise: they are few in any 32 neighbours, and a token's noise is some
+//      hundred instructions.
+//   Where that does not do (the border lies further away, more equal entries than the list holds, k beyond the threads), `far_border` finds it: a histogram of
+//   all tokens, and the span of (l, index) in question cut into as many steps again until its tokens fit.
 // ---------------------------------------------------------------------------
 namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
-constexpr int F_THREADS = 512, F_WARPS = F_THREADS / 32, BINS = 2048, NEAR = F_THREADS, LISTED = 512, NEAR_LISTED = 2048, MAX_CLUSTER = 8;
+constexpr int F_THREADS = 512, F_WARPS = F_THREADS / 32, BINS = 2048, NEAR = 2 * F_THREADS, LISTED = 512, NEAR_LISTED = 2048, MAX_CLUSTER = 8;
 constexpr float BINS_PER_NAT = 64.f;
+constexpr int GATHERED = 6144;
 
 struct FilterParams {
     const float* logits;
@@ -210,7 +213,7 @@ struct FilterParams {
 };
 
 struct FilterShared {
-    unsigned near_count[NEAR], near_low[NEAR], near_high[NEAR];      // mass: high 2^32 + low
+    unsigned near_low[NEAR], near_high[NEAR];      // mass: high 2^32 + low
     union {
         struct {
             unsigned count[BINS], low[BINS], high[BINS];
@@ -219,6 +222,8 @@ struct FilterShared {
             u64 near_list[NEAR_LISTED];
             unsigned near_mass[NEAR_LISTED];
         };
+        float thread_most[MAX_CLUSTER][F_THREADS];
+        unsigned gathered[GATHERED];
     };
     u64 list[LISTED];
     unsigned list_mass[LISTED];
@@ -226,23 +231,288 @@ struct FilterShared {
     u64 warp_u64[2][F_WARPS];
     Best warp_best[F_WARPS];
     Best cluster_best[MAX_CLUSTER];
-    unsigned near_listed;
-    int near_step;                                    // the tokens up to this step are listed; < 0: too far or too many
+    unsigned listed;
+    unsigned near_own, near_pushed, near_base;        // the list: a CTA's own tokens from its end downwards, the other CTAs' from its start
+    unsigned n_gathered;
+    int near_step, near_kind;                         // what the first CTA has found: the step, and whether it will do (0: no)
+    float near_least;                                 // the smallest entry to list
     u64 rest;                                         // the mass beyond the near steps
     // the step that a search ended in (`above`: before it), or the border
     int step;
     u64 above_count, above_mass, inside, border, border_mass;
-    unsigned listed;
 };
 
-// A number whose order as an unsigned integer is that of the floats (-0 and +0 are one).
+// A number whose order as an unsigned integer is that of the floats (-0 and +0 are one), and back.
 __device__ __forceinline__ unsigned order_key(float l) {
     const unsigned u = __float_as_uint(l + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float entry_of(u64 key) {
+    const unsigned u = (unsigned)(key >> 32);
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
 __device__ __forceinline__ float entry(float l) { return l == l ? l : -INFINITY; }
+__device__ __forceinline__ unsigned mass_of(float d) { return __float2uint_rn(expf(-d) * 2147483648.f); }
+__device__ __forceinline__ int first_step(float d) { return (int)fminf(d * BINS_PER_NAT, (float)(BINS - 1)); }
+__device__ __forceinline__ void tally(unsigned* count, unsigned* low, unsigned* high, int b, unsigned f) {
+    atomicAdd(count + b, 1u);
+    const unsigned old = atomicAdd(low + b, f);
+    if (old + f < old) atomicAdd(high + b, 1u);
+}
 
-__global__ void __launch_bounds__(F_THREADS)
+// A CTA's part of a row.
+struct Slice {
+    FilterShared& sh;
+    cg::cluster_group cluster;
+    int C, rank, begin, n, head, body;      // entries: begin .. begin + n; up to a 16-byte boundary, and whole vectors after it
+    int turn;
+    const float* held;
+    float most, inv_t, top_p;
+
+    // (the distance of the largest entry is zero even where it is infinite or the temperature's inverse is)
+    __device__ __forceinline__ float distance(float l) const { return l == most ? 0.f : (most - l) * inv_t; }
+    __device__ __forceinline__ u64 composite(float l, int i) const { return (u64)order_key(l) << 32 | (unsigned)~(unsigned)(begin + i); }
+    __device__ __forceinline__ u64 share(u64 whole) const { return max(1ull, (u64)ceil((double)top_p * (double)whole)); }
+    // f(four entries as they are, the index of the first, how many count) for all of the slice
+    template <typename F> __device__ __forceinline__ void vectors(F f) const {
+        const int tid = threadIdx.x;
+        if (tid < head) f(make_float4(held[tid], -INFINITY, -INFINITY, -INFINITY), tid, 1);
+        constexpr int AHEAD = 4;
+        for (int i = tid; i < body; i += AHEAD * F_THREADS) {
+            float4 v[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+                if (i + q * F_THREADS < body) v[q] = *reinterpret_cast<const float4*>(held + head + 4 * (i + q * F_THREADS));
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+                if (i + q * F_THREADS < body) f(v[q], head + 4 * (i + q * F_THREADS), 4);
+        }
+        const int last = head + 4 * body + tid;
+        if (last < n) f(make_float4(held[last], -INFINITY, -INFINITY, -INFINITY), last, 1);
+    }
+    // f(entry as it is, its index)
+    template <typename F> __device__ __forceinline__ void entries(F f) const {
+        vectors([&](const float4& v, int i, int count) {
+            f(v.x, i);
+            if (count == 4) { f(v.y, i + 1); f(v.z, i + 2); f(v.w, i + 3); }
+        });
+    }
+    // Every CTA's pair of numbers (in its first C threads), known to all threads of the cluster afterwards in sh.slots[returned].
+    __device__ __forceinline__ int exchange(u64 a, u64 b) {
+        const int at = turn;
+        turn ^= 1;
+        if (threadIdx.x < C) {
+            FilterShared* other = cluster.map_shared_rank(&sh, threadIdx.x);
+            other->slots[at][rank][0] = a;
+            other->slots[at][rank][1] = b;
+        }
+        cluster.sync();
+        return at;
+    }
+    // Of the first CTA's `count` listed tokens (key(q), mass(q)), the one with which `target` tokens or `target` mass are reached, `above_*` lying before
+    // them all.
+    template <typename K, typename M>
+    __device__ __forceinline__ void rank_list(K key_of, M mass_at, int count, bool mass, u64 target, u64 above_count, u64 above_mass) const {
+        for (int q = threadIdx.x; q < count; q += F_THREADS) {
+            const u64 key = key_of(q), own = mass_at(q);
+            u64 c_at = above_count, m_at = above_mass;
+            for (int j = 0; j < count; ++j)
+                if (key_of(j) > key) { ++c_at; m_at += mass_at(j); }
+            if (mass ? m_at < target && m_at + own >= target : c_at + 1 == target) {
+                sh.border = key;
+                sh.border_mass = m_at + own;
+            }
+        }
+        __syncthreads();
+    }
+    __device__ void clear() const {
+        for (int b = threadIdx.x; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
+        __syncthreads();
+    }
+    __device__ u64 locate(bool mass, u64 target, u64 before_count, u64 before_mass, bool add);
+    __device__ void search(bool mass, u64 target, bool add);
+    __device__ void histogram() const {
+        clear();
+        entries([&](float l, int) {
+            const float d = distance(entry(l));
+            tally(sh.count, sh.low, sh.high, first_step(d), mass_of(d));
+        });
+    }
+};
+
+// Adds up the cluster's histograms and finds the step in which the sum (of counts or masses) reaches `target`: sh.step, .above_*, .inside in every
+// CTA.  Each CTA adds up a run of steps.  target 0: only the whole mass is wanted (returned).
+__device__ __noinline__ u64 Slice::locate(bool mass, u64 target, u64 before_count, u64 before_mass, bool add) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int run = BINS / C, per = (run + F_THREADS - 1) / F_THREADS, first = rank * run;
+    cluster.sync();
+    if (add && C > 1) {
+        for (int b = first + tid; b < first + run; b += F_THREADS) {
+            u64 sum = ((u64)sh.high[b] << 32) + sh.low[b];
+            unsigned count = sh.count[b];
+            for (int c = 1; c < C; ++c) {
+                const FilterShared* other = cluster.map_shared_rank(&sh, (rank + c) % C);
+                sum += ((u64)other->high[b] << 32) + other->low[b];
+                count += other->count[b];
+            }
+            sh.high[b] = (unsigned)(sum >> 32);
+            sh.low[b] = (unsigned)sum;
+            sh.count[b] = count;
+        }
+        __syncthreads();
+    }
+    // a thread's own steps, then the threads before it
+    u64 counts = 0, masses = 0;
+    for (int q = 0; q < per; ++q) {
+        const int b = tid * per + q;
+        if (b < run) {
+            counts += sh.count[first + b];
+            masses += ((u64)sh.high[first + b] << 32) + sh.low[first + b];
+        }
+    }
+    u64 c_up = counts, m_up = masses;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 a = __shfl_up_sync(0xffffffffu, c_up, o), b = __shfl_up_sync(0xffffffffu, m_up, o);
+        if (lane >= o) { c_up += a; m_up += b; }
+    }
+    if (lane == 31) { sh.warp_u64[0][warp] = c_up; sh.warp_u64[1][warp] = m_up; }
+    __syncthreads();
+    u64 c_all = 0, m_all = 0;
+    for (int w = 0; w < F_WARPS; ++w) {
+        if (w == warp) { c_up += c_all; m_up += m_all; }
+        c_all += sh.warp_u64[0][w];
+        m_all += sh.warp_u64[1][w];
+    }
+    const int at = exchange(c_all, m_all);
+    u64 c_before = before_count, m_before = before_mass, m_whole = before_mass;
+    for (int c = 0; c < C; ++c) {
+        if (c < rank) { c_before += sh.slots[at][c][0]; m_before += sh.slots[at][c][1]; }
+        m_whole += sh.slots[at][c][1];
+    }
+    if (target == 0) return m_whole;
+    u64 c_at = c_before + c_up - counts, m_at = m_before + m_up - masses;      // before the thread's own
+    if ((mass ? m_at : c_at) < target && (mass ? m_at + masses : c_at + counts) >= target) {
+        int b = tid * per;
+        for (;; ++b) {
+            const u64 c = sh.count[first + b], m = ((u64)sh.high[first + b] << 32) + sh.low[first + b];
+            if ((mass ? m_at + m : c_at + c) >= target) {
+                for (int q = 0; q < C; ++q) {
+                    FilterShared* other = cluster.map_shared_rank(&sh, q);
+                    other->step = first + b;
+                    other->above_count = c_at;
+                    other->above_mass = m_at;
+                    other->inside = c;
+                }
+                break;
+            }
+            c_at += c;
+            m_at += m;
+        }
+    }
+    cluster.sync();
+    return m_whole;
+}
+
+// From the histogram of all tokens (already added up where !add) to the border token: sh.border and, with everything before it, its mass, in every CTA.
+__device__ __noinline__ void Slice::search(bool mass, u64 target, bool add) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    locate(mass, target, 0, 0, add);
+    const int step0 = sh.step;
+    u64 from = 0, to = ~0ull;      // the span of (l, index) left
+    auto inside = [&](float l, int i) {
+        const u64 key = composite(l, i);
+        return first_step(distance(l)) == step0 && key >= from && key <= to;
+    };
+    for (int level = 0; sh.inside > LISTED && level < 7; ++level) {      // 64 bits, eleven a time
+        if (level == 0) {
+            u64 low = ~0ull, high = 0;
+            entries([&](float x, int i) {
+                const float l = entry(x);
+                if (inside(l, i)) {
+                    low = min(low, composite(l, i));
+                    high = max(high, composite(l, i));
+                }
+            });
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+                high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
+            }
+            __syncthreads();
+            if (lane == 0) { sh.warp_u64[0][warp] = low; sh.warp_u64[1][warp] = high; }
+            __syncthreads();
+            for (int w = 0; w < F_WARPS; ++w) {
+                low = min(low, sh.warp_u64[0][w]);
+                high = max(high, sh.warp_u64[1][w]);
+            }
+            const int at = exchange(low, high);
+            for (int c = 0; c < C; ++c) {
+                low = min(low, sh.slots[at][c][0]);
+                high = max(high, sh.slots[at][c][1]);
+            }
+            from = low;
+            to = high;
+        }
+        int shift = 0;
+        while ((to - from) >> shift >= BINS) ++shift;
+        const u64 before_count = sh.above_count, before_mass = sh.above_mass;
+        cluster.sync();      // all have read the last histogram and what it gave
+        clear();
+        entries([&](float x, int i) {
+            const float l = entry(x);
+            if (inside(l, i)) tally(sh.count, sh.low, sh.high, (int)((to - composite(l, i)) >> shift), mass_of(distance(l)));
+        });
+        locate(mass, target, before_count, before_mass, true);
+        to -= (u64)sh.step << shift;
+        from = max(from, to - ((1ull << shift) - 1));
+    }
+    // the tokens of the span, ranked by the first CTA
+    FilterShared* const lead = cluster.map_shared_rank(&sh, 0);
+    entries([&](float x, int i) {
+        const float l = entry(x);
+        if (inside(l, i)) {
+            const unsigned at = atomicAdd(&lead->listed, 1u);
+            if (at < LISTED) {
+                lead->list[at] = composite(l, i);
+                lead->list_mass[at] = mass_of(distance(l));
+            }
+        }
+    });
+    cluster.sync();
+    if (rank == 0) {
+        rank_list([&](int q) { return sh.list[q]; }, [&](int q) { return sh.list_mass[q]; }, min((int)sh.listed, LISTED), mass, target, sh.above_count,
+                  sh.above_mass);
+        if (tid == 0) sh.listed = 0;
+        if (tid > 0 && tid < C) {
+            FilterShared* other = cluster.map_shared_rank(&sh, tid);
+            other->border = sh.border;
+            other->border_mass = sh.border_mass;
+        }
+    }
+    cluster.sync();
+}
+
+// The border token wherever it lies (sh.border in every CTA).
+__device__ __noinline__ void far_border(Slice& s, int k, bool by_count, bool by_mass) {
+    s.histogram();
+    u64 whole = 0;
+    bool added = false;
+    if (by_count) {
+        s.search(false, (u64)k, true);
+        whole = s.sh.border_mass;
+        if (by_mass) {      // the histogram again (the search has added it up, or cut it into finer steps)
+            __syncthreads();
+            s.histogram();
+        }
+    } else {
+        whole = s.locate(true, 0, 0, 0, true);
+        added = true;
+    }
+    if (by_mass) s.search(true, s.share(whole), !added);
+}
+
+__global__ void __launch_bounds__(F_THREADS, 2)
 sample_filtered_kernel(const FilterParams p) {
     extern __shared__ float4 dyn[];
     __shared__ FilterShared sh;
@@ -251,6 +521,11 @@ sample_filtered_kernel(const FilterParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / C;
     pdl_trigger();
+    for (int b = tid; b < NEAR; b += F_THREADS) sh.near_low[b] = sh.near_high[b] = 0;
+    if (tid == 0) {
+        sh.listed = sh.near_own = sh.near_pushed = 0;
+        sh.rest = 0;
+    }
     cluster.sync();      // the others have started: their shared memory can be written to
     pdl_wait();
     const float* row = p.logits + (size_t)r * p.ld;
@@ -264,20 +539,9 @@ sample_filtered_kernel(const FilterParams p) {
     const float top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p ? fminf(p.min_p[r], 1.f) : 0.f;
     const bool by_count = k > 0 && k < p.V, by_mass = top_p < 1.f;
     const bool filtered = !greedy && (k > 0 || by_mass || min_p > 0.f);
+    const int head = min(n, (int)((4 - ((uintptr_t)(row + begin) >> 2)) & 3));
+    Slice s = {sh, cluster, C, rank, begin, n, head, (n - head) / 4, 0, row + begin, -INFINITY, inv_t, top_p};
 
-    int turn = 0;
-    // every CTA's pair of numbers, known to all threads of the cluster afterwards in sh.slots[returned]
-    auto exchange = [&](u64 a, u64 b) {      // a, b: in the first C threads
-        const int at = turn;
-        turn ^= 1;
-        if (tid < C) {
-            FilterShared* other = cluster.map_shared_rank(&sh, tid);
-            other->slots[at][rank][0] = a;
-            other->slots[at][rank][1] = b;
-        }
-        cluster.sync();
-        return at;
-    };
     auto best_of_block = [&](Best& best) {      // in thread 0
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
@@ -298,417 +562,314 @@ sample_filtered_kernel(const FilterParams p) {
     };
     Best best{-INFINITY, 0x7fffffff};
     if (!filtered) {
-        for (int i = tid; i < n; i += F_THREADS) {
-            float s = entry(row[begin + i]);
-            if (!greedy) s = __fadd_rn(__fmul_rn(s, inv_t), gumbel(seed, tix, (unsigned)(begin + i)));
-            if (s > best.score || best.index == 0x7fffffff) best = Best{s, begin + i};
-        }
+        s.entries([&](float l, int i) {
+            float v = entry(l);
+            if (!greedy) v = __fadd_rn(__fmul_rn(v, inv_t), gumbel(seed, tix, (unsigned)(begin + i)));
+            best = better(best, Best{v, begin + i});
+        });
         finish(best);
         return;
     }
 
     // 1. the slice, and the largest entry
-    const float* held = row + begin;
     float most = -INFINITY;
-    const int shift16 = (int)(((uintptr_t)held >> 2) & 3), head = min(n, (4 - shift16) & 3), body = (n - head) / 4;
-    // f(four entries, the index of the first) for all of the slice, by whole vectors but for its ends (of which the first entry alone counts)
-    auto vectors = [&](const float* src, auto f) {
-        if (tid < head) f(make_float4(entry(src[tid]), -INFINITY, -INFINITY, -INFINITY), tid, 1);
-        constexpr int AHEAD = 4;
-        for (int i = tid; i < body; i += AHEAD * F_THREADS) {
-            float4 v[AHEAD];
-#pragma unroll
-            for (int q = 0; q < AHEAD; ++q)
-                if (i + q * F_THREADS < body) v[q] = *reinterpret_cast<const float4*>(src + head + 4 * (i + q * F_THREADS));
-#pragma unroll
-            for (int q = 0; q < AHEAD; ++q)
-                if (i + q * F_THREADS < body)
-                    f(make_float4(entry(v[q].x), entry(v[q].y), entry(v[q].z), entry(v[q].w)), head + 4 * (i + q * F_THREADS), 4);
-        }
-        const int last = head + 4 * body + tid;
-        if (last < n) f(make_float4(entry(src[last]), -INFINITY, -INFINITY, -INFINITY), last, 1);
-    };
     {
-        float* const mine = reinterpret_cast<float*>(dyn) + shift16;      // the same place within 16 bytes
-        vectors(held, [&](const float4& v, int i, int count) {
-            most = fmaxf(most, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+        float* const mine = reinterpret_cast<float*>(dyn) + (((uintptr_t)s.held >> 2) & 3);      // the same place within 16 bytes
+        s.vectors([&](const float4& v, int i, int count) {
+            most = fmaxf(most, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));      // a NaN is passed over
             if (!p.resident) return;
             if (count == 4) *reinterpret_cast<float4*>(mine + i) = v;
             else mine[i] = v.x;
         });
-        if (p.resident) held = mine;
+        if (p.resident) s.held = mine;
     }
-    // f(entry, its index) for all of the slice
-    auto entries = [&](auto f) {
-        vectors(held, [&](const float4& v, int i, int count) {
-            f(v.x, i);
-            if (count == 4) { f(v.y, i + 1); f(v.z, i + 2); f(v.w, i + 3); }
-        });
-    };
+    const bool by_threads = by_count && k <= C * F_THREADS / 2;
+    if (by_threads) cluster.map_shared_rank(&sh, 0)->thread_most[rank][tid] = most;
     most = warp_max(most);
     if (lane == 0) sh.warp_best[warp].score = most;
-    sh.near_count[tid] = sh.near_low[tid] = sh.near_high[tid] = 0;
-    if (tid == 0) {
-        sh.listed = sh.near_listed = 0;
-        sh.rest = 0;
-    }
     __syncthreads();
     if (tid < C)
         for (int w = 0; w < F_WARPS; ++w) most = fmaxf(most, sh.warp_best[w].score);
     {
-        const int at = exchange(__float_as_uint(most), 0);
+        const int at = s.exchange(__float_as_uint(most), 0);
         for (int c = 0; c < C; ++c) most = fmaxf(most, __uint_as_float((unsigned)sh.slots[at][c][0]));
     }
-    // (the distance of the largest entry is zero even where it is infinite or the temperature's inverse is)
-    auto distance = [&](float l) { return l == most ? 0.f : (most - l) * inv_t; };
-    auto mass_of = [&](float d) { return __float2uint_rn(expf(-d) * 2147483648.f); };
-    auto first_step = [&](float d) { return (int)fminf(d * BINS_PER_NAT, (float)(BINS - 1)); };
-    auto composite = [&](float l, int i) { return (u64)order_key(l) << 32 | (unsigned)~(unsigned)(begin + i); };
-    auto tally = [&](int b, unsigned f) {
-        atomicAdd(&sh.count[b], 1u);
-        const unsigned old = atomicAdd(&sh.low[b], f);
-        if (old + f < old) atomicAdd(&sh.high[b], 1u);
-    };
-
-    // Adds up the cluster's histograms and finds the step in which the sum (of counts or masses) reaches `target`: sh.step, .above_*, .inside in every
-    // CTA.  Each CTA adds up a run of steps.  target 0: only the whole mass is wanted (returned).
-    auto locate = [&](bool mass, u64 target, u64 before_count, u64 before_mass, bool add) {
-        const int run = BINS / C, per = (run + F_THREADS - 1) / F_THREADS, first = rank * run;
-        cluster.sync();
-        if (add && C > 1) {
-            for (int b = first + tid; b < first + run; b += F_THREADS) {
-                u64 sum = ((u64)sh.high[b] << 32) + sh.low[b];
-                unsigned count = sh.count[b];
-                for (int c = 1; c < C; ++c) {
-                    const FilterShared* other = cluster.map_shared_rank(&sh, (rank + c) % C);
-                    sum += ((u64)other->high[b] << 32) + other->low[b];
-                    count += other->count[b];
-                }
-                sh.high[b] = (unsigned)(sum >> 32);
-                sh.low[b] = (unsigned)sum;
-                sh.count[b] = count;
-            }
-            __syncthreads();
-        }
-        // a thread's own steps, then the threads before it
-        u64 counts = 0, masses = 0;
-        for (int q = 0; q < per; ++q) {
-            const int b = tid * per + q;
-            if (b < run) {
-                counts += sh.count[first + b];
-                masses += ((u64)sh.high[first + b] << 32) + sh.low[first + b];
-            }
-        }
-        u64 c_up = counts, m_up = masses;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 a = __shfl_up_sync(0xffffffffu, c_up, o), b = __shfl_up_sync(0xffffffffu, m_up, o);
-            if (lane >= o) { c_up += a; m_up += b; }
-        }
-        if (lane == 31) { sh.warp_u64[0][warp] = c_up; sh.warp_u64[1][warp] = m_up; }
-        __syncthreads();
-        u64 c_all = 0, m_all = 0;
-        for (int w = 0; w < F_WARPS; ++w) {
-            if (w == warp) { c_up += c_all; m_up += m_all; }
-            c_all += sh.warp_u64[0][w];
-            m_all += sh.warp_u64[1][w];
-        }
-        const int at = exchange(c_all, m_all);
-        u64 c_before = before_count, m_before = before_mass, m_whole = before_mass;
-        for (int c = 0; c < C; ++c) {
-            if (c < rank) { c_before += sh.slots[at][c][0]; m_before += sh.slots[at][c][1]; }
-            m_whole += sh.slots[at][c][1];
-        }
-        if (target == 0) return m_whole;
-        u64 c_at = c_before + c_up - counts, m_at = m_before + m_up - masses;      // before the thread's own
-        if ((mass ? m_at : c_at) < target && (mass ? m_at + masses : c_at + counts) >= target) {
-            int b = tid * per;
-            for (;; ++b) {
-                const u64 c = sh.count[first + b], m = ((u64)sh.high[first + b] << 32) + sh.low[first + b];
-                if ((mass ? m_at + m : c_at + c) >= target) {
-                    for (int q = 0; q < C; ++q) {
-                        FilterShared* other = cluster.map_shared_rank(&sh, q);
-                        other->step = first + b;
-                        other->above_count = c_at;
-                        other->above_mass = m_at;
-                        other->inside = c;
-                    }
-                    break;
-                }
-                c_at += c;
-                m_at += m;
-            }
-        }
-        cluster.sync();
-        return m_whole;
-    };
-    // From the first histogram (already added up where !add) to the border token: sh.border and, with everything before it, its mass, in every CTA.
-    auto search = [&](bool mass, u64 target, bool add) {
-        locate(mass, target, 0, 0, add);
-        const int step0 = sh.step;
-        u64 from = 0, to = ~0ull;      // the span of (l, index) left
-        auto inside = [&](float l, int i) {
-            const u64 key = composite(l, i);
-            return first_step(distance(l)) == step0 && key >= from && key <= to;
-        };
-        bool spanned = false;
-        for (int level = 0; sh.inside > LISTED && level < 7; ++level) {      // 64 bits, eleven a time
-            if (!spanned) {
-                u64 low = ~0ull, high = 0;
-                entries([&](float l, int i) {
-                    if (inside(l, i)) {
-                        low = min(low, composite(l, i));
-                        high = max(high, composite(l, i));
-                    }
-                });
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
-                    high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
-                }
-                __syncthreads();
-                if (lane == 0) { sh.warp_u64[0][warp] = low; sh.warp_u64[1][warp] = high; }
-                __syncthreads();
-                for (int w = 0; w < F_WARPS; ++w) {
-                    low = min(low, sh.warp_u64[0][w]);
-                    high = max(high, sh.warp_u64[1][w]);
-                }
-                const int at = exchange(low, high);
-                for (int c = 0; c < C; ++c) {
-                    low = min(low, sh.slots[at][c][0]);
-                    high = max(high, sh.slots[at][c][1]);
-                }
-                from = low;
-                to = high;
-                spanned = true;
-            }
-            int shift = 0;
-            while ((to - from) >> shift >= BINS) ++shift;
-            const u64 before_count = sh.above_count, before_mass = sh.above_mass;
-            cluster.sync();      // all have read the last histogram and what it gave
-            for (int b = tid; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
-            __syncthreads();
-            entries([&](float l, int i) {
-                if (inside(l, i)) tally((int)((to - composite(l, i)) >> shift), mass_of(distance(l)));
-            });
-            locate(mass, target, before_count, before_mass, true);
-            to -= (u64)sh.step << shift;
-            from = max(from, to - ((1ull << shift) - 1));
-        }
-        // the tokens of the span, ranked by the first CTA
-        FilterShared* const lead = cluster.map_shared_rank(&sh, 0);
-        entries([&](float l, int i) {
-            if (inside(l, i)) {
-                const unsigned at = atomicAdd(&lead->listed, 1u);
-                if (at < LISTED) {
-                    lead->list[at] = composite(l, i);
-                    lead->list_mass[at] = mass_of(distance(l));
-                }
-            }
-        });
-        cluster.sync();
-        if (rank == 0) {
-            const int count = min((int)sh.listed, LISTED);
-            for (int q = tid; q < count; q += F_THREADS) {
-                const u64 key = sh.list[q], own = sh.list_mass[q];
-                u64 c_at = sh.above_count, m_at = sh.above_mass;
-                for (int j = 0; j < count; ++j)
-                    if (sh.list[j] > key) { ++c_at; m_at += sh.list_mass[j]; }
-                if (mass ? m_at < target && m_at + own >= target : c_at + 1 == target)
-                    for (int c = 0; c < C; ++c) {
-                        FilterShared* other = cluster.map_shared_rank(&sh, c);
-                        other->border = key;
-                        other->border_mass = m_at + own;
-                    }
-            }
-            __syncthreads();
-            if (tid == 0) sh.listed = 0;
-        }
-        cluster.sync();
-    };
-
-    u64 border = 0;
+    s.most = most;
     if (most == -INFINITY) {
         if (rank == 0 && tid == 0) p.out[r] = 0;      // nothing left to choose from
-        cluster.sync();
         return;
     }
-    auto clear = [&]() {
-        for (int b = tid; b < BINS; b += F_THREADS) sh.count[b] = sh.low[b] = sh.high[b] = 0;
-        __syncthreads();
-    };
-    auto share = [&](u64 whole) { return max(1ull, (u64)ceil((double)top_p * (double)whole)); };
     auto score = [&](float l, unsigned index) {
-        const float d = distance(l);
+        const float d = s.distance(l);
         if (min_p > 0.f && !(expf(-d) >= min_p)) return;
-        const float s = entry(__fadd_rn(-d, gumbel(seed, tix, index)));
-        best = better(best, Best{s, (int)index});
+        best = better(best, Best{entry(__fadd_rn(-d, gumbel(seed, tix, index))), (int)index});
     };
+    u64 border = 0;
     if (by_count || by_mass) {
         FilterShared* const lead = cluster.map_shared_rank(&sh, 0);
-        // 2. the near steps; what lies beyond them counts where the whole mass is wanted
-        u64 rest = 0;
-        entries([&](float l, int) {
-            const float d = distance(l);
-            if (d * BINS_PER_NAT < (float)NEAR) {
-                const int b = first_step(d);
-                const unsigned f = mass_of(d);
-                atomicAdd(&sh.near_count[b], 1u);
-                const unsigned old = atomicAdd(&sh.near_low[b], f);
-                if (old + f < old) atomicAdd(&sh.near_high[b], 1u);
+        // The tokens with entries from `least` to `largest` go to the first CTA's list: its own from the end downwards, the others' by way of lists of
+        // their own from the start on (one counter for all of them would be waited for in turn).
+        auto list = [&](float least, float largest) {
+            s.vectors([&](const float4& v, int i, int count) {
+                if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least)) return;
+                const float l[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (q < count && l[q] >= least && l[q] <= largest) {
+                        const unsigned at = atomicAdd(&sh.near_own, 1u);
+                        if (at < NEAR_LISTED) {
+                            sh.near_list[NEAR_LISTED - 1 - at] = s.composite(l[q], i + q);
+                            sh.near_mass[NEAR_LISTED - 1 - at] = mass_of(s.distance(l[q]));
+                        }
+                    }
+            });
+            __syncthreads();
+            if (rank != 0) {
+                const unsigned count = sh.near_own;
+                if (tid == 0 && count) sh.near_base = atomicAdd(&lead->near_pushed, count);
+                __syncthreads();
+                for (unsigned q = tid; q < count && q < NEAR_LISTED; q += F_THREADS)
+                    if (sh.near_base + q < NEAR_LISTED) {
+                        lead->near_list[sh.near_base + q] = sh.near_list[NEAR_LISTED - 1 - q];
+                        lead->near_mass[sh.near_base + q] = sh.near_mass[NEAR_LISTED - 1 - q];
+                    }
             }
-            else if (!by_count && d < 23.f) rest += mass_of(d);      // (below 2^-32 beyond)
-        });
-        if (!by_count) {
+            cluster.sync();
+        };
+        // (the first CTA's) how many there are, and where the q-th one is
+        auto listed = [&]() { return (int)(sh.near_pushed + sh.near_own); };
+        auto place = [&](int q) { return q < (int)sh.near_pushed ? q : NEAR_LISTED - 1 - (q - (int)sh.near_pushed); };
+        auto choose = [&](int count) {      // among the listed ones, by the first CTA
+            const u64 border = sh.border;
+            for (int q = tid; q < count; q += F_THREADS) {
+                const u64 key = sh.near_list[place(q)];
+                if (key >= border) score(entry_of(key), ~(unsigned)key);
+            }
+            best_of_block(best);
+            if (tid == 0) p.out[r] = best.index == 0x7fffffff ? 0 : best.index;
+        };
+        int kind = 0;
+        if (by_threads) {
+            // 2. t, by the first CTA
+            if (rank == 0) {
+                const int values = C * F_THREADS;
+                const float* const all = &sh.thread_most[0][0];
+                float least = INFINITY;
+                for (int q = tid; q < values; q += F_THREADS)
+                    if (all[q] > -INFINITY) least = fminf(least, all[q]);
+                least = -warp_max(-least);
+                if (lane == 0) sh.warp_best[warp].score = least;
+                __syncthreads();
+                for (int w = 0; w < F_WARPS; ++w) least = fminf(least, sh.warp_best[w].score);
+                // steps from the largest to the least of them; those up to the step with which they are k
+                const float width = (most - least) * (1.f / (NEAR - 1));
+                auto step_of = [&](float v) { return width > 0.f ? (int)fminf((most - v) / width, (float)(NEAR - 1)) : 0; };
+                for (int q = tid; q < values; q += F_THREADS)
+                    if (all[q] > -INFINITY) atomicAdd(&sh.near_low[step_of(all[q])], 1u);
+                if (tid == 0) sh.step = -1;
+                __syncthreads();
+                const int mine = sh.near_low[2 * tid] + sh.near_low[2 * tid + 1];      // two steps a thread
+                int up = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, up, o);
+                    if (lane >= o) up += x;
+                }
+                if (lane == 31) sh.warp_u64[0][warp] = up;
+                __syncthreads();
+                for (int w = 0; w < warp; ++w) up += (int)sh.warp_u64[0][w];
+                if (up >= k && up - mine < k) sh.step = 2 * tid + 1;
+                __syncthreads();
+                float t = INFINITY;
+                for (int q = tid; q < values; q += F_THREADS)
+                    if (all[q] > -INFINITY && step_of(all[q]) <= sh.step) t = fminf(t, all[q]);
+                t = -warp_max(-t);
+                __syncthreads();
+                if (lane == 0) sh.warp_best[warp].score = t;
+                __syncthreads();
+                if (tid < C) {
+                    for (int w = 0; w < F_WARPS; ++w) t = fminf(t, sh.warp_best[w].score);
+                    FilterShared* other = cluster.map_shared_rank(&sh, tid);
+                    other->near_least = t;
+                    other->near_kind = sh.step >= 0 && most < INFINITY ? 2 : 0;
+                }
+            }
+            cluster.sync();
+            if (sh.near_kind == 2) {
+                const float t = sh.near_least;
+                list(t, most);
+                const int count = rank == 0 ? listed() : 0;
+                if (rank == 0 && tid < C) cluster.map_shared_rank(&sh, tid)->near_kind = count <= 2 * F_THREADS ? 3 : 0;
+                cluster.sync();
+                if (sh.near_kind == 3) {
+                    if (rank != 0) return;      // nothing of the others' is read any more
+                    // each token's place, and the mass before it: the k-th one, then the one with which p of the mass is reached
+                    u64 keys[2], before[2], own[2];
+                    int places[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int q = tid + h * F_THREADS;
+                        keys[h] = q < count ? sh.near_list[place(q)] : 0;
+                        own[h] = q < count ? sh.near_mass[place(q)] : 0;
+                        before[h] = 0;
+                        places[h] = 0;
+                        if (q < count)
+                            for (int j = 0; j < count; ++j)
+                                if (sh.near_list[place(j)] > keys[h]) { ++places[h]; before[h] += sh.near_mass[place(j)]; }
+                        if (q < count && places[h] + 1 == k) {
+                            sh.border = keys[h];
+                            sh.border_mass = before[h] + own[h];
+                        }
+                    }
+                    __syncthreads();
+                    if (by_mass) {
+                        const u64 target = s.share(sh.border_mass);
+                        __syncthreads();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            if (tid + h * F_THREADS < count && before[h] < target && before[h] + own[h] >= target) sh.border = keys[h];
+                        __syncthreads();
+                    }
+                    choose(count);
+                    return;
+                }
+            }
+        } else if (!by_count && most < INFINITY && inv_t < 1e37f && inv_t > 0.f) {
+            // 2'. the near steps, and the mass beyond them
+            const float scale = inv_t * BINS_PER_NAT;      // a power of two apart: distances in steps are rounded as they are
+            u64 rest = 0;
+            s.entries([&](float l, int) {
+                const float d = (most - l) * scale;      // (a NaN's is one, and lies on neither side)
+                if (d < 23.f * BINS_PER_NAT) {           // (below 2^-32 beyond)
+                    const unsigned f = mass_of(d * (1.f / BINS_PER_NAT));
+                    if (d < (float)NEAR) {
+                        const unsigned old = atomicAdd(&sh.near_low[(int)d], f);
+                        if (old + f < old) atomicAdd(&sh.near_high[(int)d], 1u);
+                    } else rest += f;
+                }
+            });
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
             if (lane == 0 && rest) atomicAdd(&lead->rest, rest);
-        }
-        __syncthreads();
-        if (rank != 0) {
-            const unsigned count = sh.near_count[tid], low = sh.near_low[tid];
-            if (count) {
-                atomicAdd(&lead->near_count[tid], count);
-                const unsigned old = atomicAdd(&lead->near_low[tid], low);
-                const unsigned high = sh.near_high[tid] + (old + low < old);
-                if (high) atomicAdd(&lead->near_high[tid], high);
-            }
-        }
-        cluster.sync();
-        // the steps' sums up to and with each one of the first CTA's threads', and the search among them
-        u64 counts = 0, masses = 0, c_up = 0, m_up = 0, target = k;
-        auto near_step = [&](bool mass, u64 target) {      // all threads of the first CTA; the step in sh.step, what is before it in sh.above_*
-            if (tid == 0) sh.step = -1;
             __syncthreads();
-            if ((mass ? m_up : c_up) >= target && (mass ? m_up - masses : c_up - counts) < target) {
-                sh.step = tid;
-                sh.above_count = c_up - counts;
-                sh.above_mass = m_up - masses;
-                sh.inside = counts;
-            }
-            __syncthreads();
-        };
-        if (rank == 0) {
-            counts = c_up = sh.near_count[tid];
-            masses = m_up = ((u64)sh.near_high[tid] << 32) + sh.near_low[tid];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 x = __shfl_up_sync(0xffffffffu, c_up, o), y = __shfl_up_sync(0xffffffffu, m_up, o);
-                if (lane >= o) { c_up += x; m_up += y; }
-            }
-            if (lane == 31) { sh.warp_u64[0][warp] = c_up; sh.warp_u64[1][warp] = m_up; }
-            __syncthreads();
-            u64 m_all = 0;
-            for (int w = 0; w < F_WARPS; ++w) {
-                if (w < warp) { c_up += sh.warp_u64[0][w]; m_up += sh.warp_u64[1][w]; }
-                m_all += sh.warp_u64[1][w];
-            }
-            if (!by_count) target = share(m_all + sh.rest);
-            near_step(!by_count, target);
-            if (tid < C) {
-                const bool fits = sh.step >= 0 && sh.above_count + sh.inside <= NEAR_LISTED;
-                cluster.map_shared_rank(&sh, tid)->near_step = fits ? sh.step : -1;
-            }
-        }
-        cluster.sync();
-        const int near = sh.near_step;
-        if (near >= 0) {
-            // 3. the tokens up to that step
-            entries([&](float l, int i) {
-                if (distance(l) * BINS_PER_NAT < (float)(near + 1)) {
-                    const unsigned at = atomicAdd(&lead->near_listed, 1u);
-                    if (at < NEAR_LISTED) {
-                        lead->near_list[at] = composite(l, i);
-                        lead->near_mass[at] = mass_of(distance(l));
-                    }
+            if (rank != 0)
+                for (int b = tid; b < NEAR; b += F_THREADS) {
+                    const unsigned low = sh.near_low[b];
+                    if (low) {
+                        const unsigned old = atomicAdd(&lead->near_low[b], low);
+                        const unsigned high = sh.near_high[b] + (old + low < old);
+                        if (high) atomicAdd(&lead->near_high[b], high);
+                    } else if (sh.near_high[b]) atomicAdd(&lead->near_high[b], sh.near_high[b]);
                 }
-            });
             cluster.sync();
-            if (rank != 0) return;      // nothing of theirs is read any more
-            const int listed = min((int)sh.near_listed, NEAR_LISTED);
-            auto value = [&](u64 key) {
-                const unsigned u = (unsigned)(key >> 32);
-                return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
-            };
-            // the border token, from the ones of sh.step alone where they fit into the short list, else from all listed ones
-            auto rank_step = [&](bool mass, u64 target) {
-                const bool brief = sh.inside <= LISTED;
-                if (brief) {
-                    for (int q = tid; q < listed; q += F_THREADS) {
-                        const u64 key = sh.near_list[q];
-                        if (first_step(distance(value(key))) == sh.step) {
-                            const unsigned at = atomicAdd(&sh.listed, 1u);
-                            if (at < LISTED) {
-                                sh.list[at] = key;
-                                sh.list_mass[at] = sh.near_mass[q];
+            u64 target = 0;
+            if (rank == 0) {
+                // two steps a thread: the sums up to and with them
+                u64 masses[2], up = 0;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) up += masses[q] = ((u64)sh.near_high[2 * tid + q] << 32) + sh.near_low[2 * tid + q];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 x = __shfl_up_sync(0xffffffffu, up, o);
+                    if (lane >= o) up += x;
+                }
+                if (lane == 31) sh.warp_u64[0][warp] = up;
+                if (tid == 0) sh.step = -1;
+                __syncthreads();
+                u64 all = 0;
+                for (int w = 0; w < F_WARPS; ++w) {
+                    if (w < warp) up += sh.warp_u64[0][w];
+                    all += sh.warp_u64[0][w];
+                }
+                target = s.share(all + sh.rest);
+#pragma unroll
+                for (int q = 1; q >= 0; --q) {
+                    if (up >= target && up - masses[q] < target) {
+                        sh.step = 2 * tid + q;
+                        sh.above_mass = up - masses[q];
+                    }
+                    up -= masses[q];
+                }
+                __syncthreads();
+                if (tid < C) cluster.map_shared_rank(&sh, tid)->near_step = sh.step;
+            }
+            cluster.sync();
+            const int step = sh.near_step;
+            if (step >= 0) {
+                // the entries of the step lie within these, rounding and all; its tokens alone are ranked
+                const float T_step = T * (1.f / BINS_PER_NAT), slack = 4e-7f * (fabsf(most) + (float)(step + 1) * T_step);
+                list(most - (float)(step + 1) * T_step - slack, most - (float)step * T_step + slack);
+                if (rank == 0) {
+                    const int count = listed();
+                    if (count <= NEAR_LISTED) {
+                        for (int q = tid; q < count; q += F_THREADS) {
+                            const u64 key = sh.near_list[place(q)];
+                            if ((int)((most - entry_of(key)) * scale) == step) {
+                                const unsigned at = atomicAdd(&sh.listed, 1u);
+                                if (at < LISTED) {
+                                    sh.list[at] = key;
+                                    sh.list_mass[at] = sh.near_mass[place(q)];
+                                }
                             }
                         }
                     }
                     __syncthreads();
-                }
-                const int count = brief ? min((int)sh.listed, LISTED) : listed;
-                const u64* const keys = brief ? sh.list : sh.near_list;
-                const unsigned* const of = brief ? sh.list_mass : sh.near_mass;
-                for (int q = tid; q < count; q += F_THREADS) {
-                    const u64 key = keys[q], own = of[q];
-                    u64 c_at = brief ? sh.above_count : 0, m_at = brief ? sh.above_mass : 0;
-                    for (int j = 0; j < count; ++j)
-                        if (keys[j] > key) { ++c_at; m_at += of[j]; }
-                    if (mass ? m_at < target && m_at + own >= target : c_at + 1 == target) {
-                        sh.border = key;
-                        sh.border_mass = m_at + own;
+                    const bool fits = count <= NEAR_LISTED && sh.listed <= LISTED;
+                    if (fits)
+                        s.rank_list([&](int q) { return sh.list[q]; }, [&](int q) { return sh.list_mass[q]; }, (int)sh.listed, true, target, 0, sh.above_mass);
+                    if (tid < C) {
+                        FilterShared* other = cluster.map_shared_rank(&sh, tid);
+                        other->border = sh.border;
+                        other->near_kind = fits;
                     }
                 }
-                __syncthreads();
-                if (tid == 0) sh.listed = 0;
-                __syncthreads();
-            };
-            rank_step(!by_count, target);
-            if (by_count && by_mass) {
-                target = share(sh.border_mass);
-                near_step(true, target);
-                rank_step(true, target);
+                cluster.sync();
+                kind = sh.near_kind;
             }
-            const u64 border = sh.border;
-            for (int q = tid; q < listed; q += F_THREADS) {
-                const u64 key = sh.near_list[q];
-                if (key >= border) score(value(key), ~(unsigned)key);
-            }
-            best_of_block(best);
-            if (tid == 0) p.out[r] = best.index == 0x7fffffff ? 0 : best.index;
-            return;
         }
-        // (flat rows) all steps
-        auto histogram = [&]() {
-            clear();
-            entries([&](float l, int) {
-                const float d = distance(l);
-                tally(first_step(d), mass_of(d));
-            });
-        };
-        histogram();
-        u64 whole = 0;
-        bool added = false;
-        if (by_count) {
-            search(false, (u64)k, true);
-            border = sh.border;
-            whole = sh.border_mass;
-            if (by_mass) {      // the first histogram again (the search has added it up, or cut it into finer steps)
-                __syncthreads();
-                histogram();
-            }
-        } else {
-            whole = locate(true, 0, 0, 0, true);
-            added = true;
+        if (kind == 0) {
+            __syncthreads();
+            if (tid == 0) sh.listed = 0;
+            Slice copy = s;      // (its address is taken: the original stays in registers)
+            far_border(copy, k, by_count, by_mass);
         }
-        if (by_mass) {
-            search(true, share(whole), !added);
-            border = sh.border;
-        }
+        border = sh.border;
     }
-    entries([&](float l, int i) {
-        if (composite(l, i) >= border) score(l, (unsigned)(begin + i));
-    });
+    const float border_l = border ? entry_of(border) : -INFINITY;
+    // (what is likely to be as far as min_p allows is looked at closely; a NaN is not)
+    const float far = min_p > 0.f ? 0.01f - logf(min_p) : INFINITY;
+    // 3'. gathered, then worked on
+    constexpr int ROUND = GATHERED / 4;      // vectors
+    for (int from = 0; from == 0 || from < s.body; from += ROUND) {
+        __syncthreads();
+        if (tid == 0) sh.n_gathered = 0;
+        __syncthreads();
+        auto gather = [&](float l, int i) {
+            if (l >= border_l && s.distance(l) <= far && s.composite(l, i) >= border) {
+                const unsigned at = atomicAdd(&sh.n_gathered, 1u);
+                if (at < GATHERED) sh.gathered[at] = i;
+            }
+        };
+        for (int i = from + tid; i < s.body && i < from + ROUND; i += F_THREADS) {
+            const float4 v = *reinterpret_cast<const float4*>(s.held + s.head + 4 * i);
+            if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= border_l)) continue;
+            const int at = s.head + 4 * i;
+            gather(v.x, at);
+            gather(v.y, at + 1);
+            gather(v.z, at + 2);
+            gather(v.w, at + 3);
+        }
+        __syncthreads();
+        const int count = min((int)sh.n_gathered, GATHERED);
+        for (int q = tid; q < count; q += F_THREADS) score(s.held[sh.gathered[q]], begin + sh.gathered[q]);
+    }
+    // the ends of the slice, off its vectors
+    auto end = [&](int i) {
+        const float l = s.held[i];
+        if (l >= border_l && s.distance(l) <= far && s.composite(l, i) >= border) score(l, begin + i);
+    };
+    if (tid < head) end(tid);
+    if (head + 4 * s.body + tid < n) end(head + 4 * s.body + tid);
     finish(best);
 }
 }  // namespace
@@ -722,17 +883,19 @@ PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float
     if (n_rows <= 0) return 0;
     if (V <= 0 || (temperature && (!seeds || !token_index))) return PYRE_ERR_BAD_ARG;
     if (cluster < 0 || cluster > MAX_CLUSTER || (cluster & (cluster - 1))) return PYRE_ERR_BAD_ARG;
-    // CTAs per row: as many as keep two to an SM busy, and as two slices in an SM's shared memory ask for
+    // CTAs per row: as many as find room, two to an SM.  152,064 entries, first k and p: 64 rows on 1 / 2 / 4 / 8 CTAs each 43 / 32 / 26 / 45 us, one row
+    // 26 / 19 / 15 / 13 us, 256 rows 67 / 69 / 80 / 136 us.
     int C = cluster > 0 ? cluster : 1;
-    while (!cluster && C < MAX_CLUSTER && ((n_rows * (long long)C < 2 * pyre_sm_count() && V > 2048 * C) || ceil_div(V, C) > 76 * 256)) C *= 2;
+    while (!cluster && C < MAX_CLUSTER && n_rows * 2ll * C <= 2 * pyre_sm_count() && V > 2048 * C) C *= 2;
     FilterParams p = {logits, ld, temperature, seeds, token_index, top_k, top_p, min_p, out, V, (ceil_div(V, C) + 3) / 4 * 4, 0};
+    constexpr int RESIDENT = 77 * 1024;      // two CTAs on an SM
     size_t bytes = (size_t)p.slice * 4 + 16;
-    p.resident = bytes <= 190 * 1024;
+    p.resident = bytes <= RESIDENT;
     if (!p.resident) bytes = 0;
     static bool configured[PYRE_MAX_DEVICES] = {};      // the attribute is per device
     bool& done = configured[pyre_current_device()];
     if (!done) {
-        const cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 190 * 1024);
+        const cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RESIDENT);
         if (e != cudaSuccess) return (int)e;
         done = true;
     }
