@@ -194,7 +194,7 @@ PYRE_API int pyre_sample(const float* logits, long long ld, const float* tempera
 namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
-constexpr int F_THREADS = 512, F_WARPS = F_THREADS / 32, BINS = 2048, NEAR = 2 * F_THREADS, LISTED = 512, NEAR_LISTED = 2048, MAX_CLUSTER = 8;
+constexpr int F_THREADS = 512, F_WARPS = F_THREADS / 32, BINS = 2048, NEAR = 2 * F_THREADS, LISTED = 512, NEAR_LISTED = 2048, MAX_CLUSTER = 16;
 constexpr float BINS_PER_NAT = 64.f;
 constexpr int GATHERED = 6144;
 
@@ -222,7 +222,7 @@ struct FilterShared {
             u64 near_list[NEAR_LISTED];
             unsigned near_mass[NEAR_LISTED];
         };
-        float thread_most[MAX_CLUSTER][F_THREADS];
+        float thread_most[MAX_CLUSTER * F_THREADS / 2];
         unsigned gathered[GATHERED];
     };
     u64 list[LISTED];
@@ -239,7 +239,7 @@ struct FilterShared {
     u64 rest;                                         // the mass beyond the near steps
     // the step that a search ended in (`above`: before it), or the border
     int step;
-    u64 above_count, above_mass, inside, border, border_mass;
+    u64 above_count, above_mass, inside, border, border_mass, target;
 };
 
 // A number whose order as an unsigned integer is that of the floats (-0 and +0 are one), and back.
@@ -252,7 +252,8 @@ __device__ __forceinline__ float entry_of(u64 key) {
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 __device__ __forceinline__ float entry(float l) { return l == l ? l : -INFINITY; }
-__device__ __forceinline__ unsigned mass_of(float d) { return __float2uint_rn(expf(-d) * 2147483648.f); }
+// exp(-d) 2^31 as a whole number (1.44 d is off by 2^-24 of it, so a mass by 1e-7 d)
+__device__ __forceinline__ unsigned mass_of(float d) { return __float2uint_rn(exp2f(fmaf(d, -1.44269504f, 31.f))); }
 __device__ __forceinline__ int first_step(float d) { return (int)fminf(d * BINS_PER_NAT, (float)(BINS - 1)); }
 __device__ __forceinline__ void tally(unsigned* count, unsigned* low, unsigned* high, int b, unsigned f) {
     atomicAdd(count + b, 1u);
@@ -297,6 +298,59 @@ struct Slice {
             if (count == 4) { f(v.y, i + 1); f(v.z, i + 2); f(v.w, i + 3); }
         });
     }
+    // put(place, entry, its index) for the whole vectors from `from` to `to` whose entries lie from `least` to `largest`; the places are taken from
+    // `counter`, a warp's at once (no thread may be elsewhere).
+    template <typename F> __device__ __forceinline__ void pick(int from, int to, float least, float largest, unsigned* counter, F put) const {
+        const int lane = threadIdx.x & 31;
+        constexpr int AHEAD = 4;
+        for (int i0 = from + (threadIdx.x & ~31); i0 < to; i0 += AHEAD * F_THREADS) {
+            float4 v[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int i = i0 + q * F_THREADS + lane;
+                v[q] = i < to ? *reinterpret_cast<const float4*>(held + head + 4 * i) : make_float4(NAN, NAN, NAN, NAN);
+            }
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v[q].x, v[q].y), fmaxf(v[q].z, v[q].w)) >= least)) continue;
+                const float l[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+                unsigned hits[4], before = 0;
+                int total = 0;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    hits[c] = __ballot_sync(0xffffffffu, l[c] >= least && l[c] <= largest);
+                    total += __popc(hits[c]);
+                }
+                if (!total) continue;
+                if (lane == 0) before = atomicAdd(counter, (unsigned)total);
+                before = __shfl_sync(0xffffffffu, before, 0);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (hits[c] >> lane & 1) put(before + __popc(hits[c] & ((1u << lane) - 1)), l[c], head + 4 * (i0 + q * F_THREADS + lane) + c);
+                    before += __popc(hits[c]);
+                }
+            }
+        }
+    }
+    // ... and for the entries off whole vectors
+    template <typename F> __device__ __forceinline__ void pick_ends(float least, float largest, unsigned* counter, F put) const {
+        auto end = [&](int i) {
+            if (held[i] >= least && held[i] <= largest) put(atomicAdd(counter, 1u), held[i], i);
+        };
+        const int tid = threadIdx.x;
+        if (tid < head) end(tid);
+        if (head + 4 * body + tid < n) end(head + 4 * body + tid);
+    }
+    // f(entry, its index) for the entries from `least` to `largest`
+    template <typename F> __device__ __forceinline__ void between(float least, float largest, F f) const {
+        vectors([&](const float4& v, int i, int count) {
+            if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least)) return;
+            const float l[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (q < count && l[q] >= least && l[q] <= largest) f(l[q], i + q);
+        });
+    }
     // Every CTA's pair of numbers (in its first C threads), known to all threads of the cluster afterwards in sh.slots[returned].
     __device__ __forceinline__ int exchange(u64 a, u64 b) {
         const int at = turn;
@@ -316,6 +370,7 @@ struct Slice {
         for (int q = threadIdx.x; q < count; q += F_THREADS) {
             const u64 key = key_of(q), own = mass_at(q);
             u64 c_at = above_count, m_at = above_mass;
+#pragma unroll 8
             for (int j = 0; j < count; ++j)
                 if (key_of(j) > key) { ++c_at; m_at += mass_at(j); }
             if (mass ? m_at < target && m_at + own >= target : c_at + 1 == target) {
@@ -330,7 +385,11 @@ struct Slice {
         __syncthreads();
     }
     __device__ u64 locate(bool mass, u64 target, u64 before_count, u64 before_mass, bool add);
-    __device__ void search(bool mass, u64 target, bool add);
+    __device__ void refine(bool mass, u64 target, float least, float largest);
+    __device__ __forceinline__ void search(bool mass, u64 target, bool add) {      // from the histogram of all tokens (already added up where !add)
+        locate(mass, target, 0, 0, add);
+        refine(mass, target, -INFINITY, INFINITY);
+    }
     __device__ void histogram() const {
         clear();
         entries([&](float l, int) {
@@ -414,21 +473,24 @@ __device__ __noinline__ u64 Slice::locate(bool mass, u64 target, u64 before_coun
     return m_whole;
 }
 
-// From the histogram of all tokens (already added up where !add) to the border token: sh.border and, with everything before it, its mass, in every CTA.
-__device__ __noinline__ void Slice::search(bool mass, u64 target, bool add) {
+// From the step in which the target lies (sh.step, .above_*, .inside in every CTA; its entries lie from `least` to `largest`) to the border token: sh.border and, with everything before it, its
+// mass, in every CTA.
+__device__ __noinline__ void Slice::refine(bool mass, u64 target, float least, float largest) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    locate(mass, target, 0, 0, add);
     const int step0 = sh.step;
     u64 from = 0, to = ~0ull;      // the span of (l, index) left
     auto inside = [&](float l, int i) {
         const u64 key = composite(l, i);
         return first_step(distance(l)) == step0 && key >= from && key <= to;
     };
+    auto each = [&](auto f) {
+        if (least == -INFINITY) entries([&](float x, int i) { f(entry(x), i); });
+        else between(least, largest, f);
+    };
     for (int level = 0; sh.inside > LISTED && level < 7; ++level) {      // 64 bits, eleven a time
         if (level == 0) {
             u64 low = ~0ull, high = 0;
-            entries([&](float x, int i) {
-                const float l = entry(x);
+            each([&](float l, int i) {
                 if (inside(l, i)) {
                     low = min(low, composite(l, i));
                     high = max(high, composite(l, i));
@@ -459,8 +521,7 @@ __device__ __noinline__ void Slice::search(bool mass, u64 target, bool add) {
         const u64 before_count = sh.above_count, before_mass = sh.above_mass;
         cluster.sync();      // all have read the last histogram and what it gave
         clear();
-        entries([&](float x, int i) {
-            const float l = entry(x);
+        each([&](float l, int i) {
             if (inside(l, i)) tally(sh.count, sh.low, sh.high, (int)((to - composite(l, i)) >> shift), mass_of(distance(l)));
         });
         locate(mass, target, before_count, before_mass, true);
@@ -469,8 +530,7 @@ __device__ __noinline__ void Slice::search(bool mass, u64 target, bool add) {
     }
     // the tokens of the span, ranked by the first CTA
     FilterShared* const lead = cluster.map_shared_rank(&sh, 0);
-    entries([&](float x, int i) {
-        const float l = entry(x);
+    each([&](float l, int i) {
         if (inside(l, i)) {
             const unsigned at = atomicAdd(&lead->listed, 1u);
             if (at < LISTED) {
@@ -583,8 +643,17 @@ sample_filtered_kernel(const FilterParams p) {
         });
         if (p.resident) s.held = mine;
     }
-    const bool by_threads = by_count && k <= C * F_THREADS / 2;
-    if (by_threads) cluster.map_shared_rank(&sh, 0)->thread_most[rank][tid] = most;
+    // (of 16 CTAs two threads' together)
+    const int values = min(C * F_THREADS, MAX_CLUSTER * F_THREADS / 2);
+    const bool by_threads = by_count && k <= values / 2;
+    if (by_threads) {
+        float* const all = cluster.map_shared_rank(&sh, 0)->thread_most;
+        if (C < MAX_CLUSTER) all[rank * F_THREADS + tid] = most;
+        else {
+            const float two = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            if (!(tid & 1)) all[(rank * F_THREADS + tid) / 2] = two;
+        }
+    }
     most = warp_max(most);
     if (lane == 0) sh.warp_best[warp].score = most;
     __syncthreads();
@@ -610,19 +679,14 @@ sample_filtered_kernel(const FilterParams p) {
         // The tokens with entries from `least` to `largest` go to the first CTA's list: its own from the end downwards, the others' by way of lists of
         // their own from the start on (one counter for all of them would be waited for in turn).
         auto list = [&](float least, float largest) {
-            s.vectors([&](const float4& v, int i, int count) {
-                if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least)) return;
-                const float l[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (q < count && l[q] >= least && l[q] <= largest) {
-                        const unsigned at = atomicAdd(&sh.near_own, 1u);
-                        if (at < NEAR_LISTED) {
-                            sh.near_list[NEAR_LISTED - 1 - at] = s.composite(l[q], i + q);
-                            sh.near_mass[NEAR_LISTED - 1 - at] = mass_of(s.distance(l[q]));
-                        }
-                    }
-            });
+            auto put = [&](unsigned at, float l, int i) {
+                if (at < NEAR_LISTED) {
+                    sh.near_list[NEAR_LISTED - 1 - at] = s.composite(l, i);
+                    sh.near_mass[NEAR_LISTED - 1 - at] = mass_of(s.distance(l));
+                }
+            };
+            s.pick(0, s.body, least, largest, &sh.near_own, put);
+            s.pick_ends(least, largest, &sh.near_own, put);
             __syncthreads();
             if (rank != 0) {
                 const unsigned count = sh.near_own;
@@ -652,8 +716,7 @@ sample_filtered_kernel(const FilterParams p) {
         if (by_threads) {
             // 2. t, by the first CTA
             if (rank == 0) {
-                const int values = C * F_THREADS;
-                const float* const all = &sh.thread_most[0][0];
+                const float* const all = sh.thread_most;
                 float least = INFINITY;
                 for (int q = tid; q < values; q += F_THREADS)
                     if (all[q] > -INFINITY) least = fminf(least, all[q]);
@@ -699,26 +762,31 @@ sample_filtered_kernel(const FilterParams p) {
                 const float t = sh.near_least;
                 list(t, most);
                 const int count = rank == 0 ? listed() : 0;
-                if (rank == 0 && tid < C) cluster.map_shared_rank(&sh, tid)->near_kind = count <= 2 * F_THREADS ? 3 : 0;
+                if (rank == 0 && tid < C) cluster.map_shared_rank(&sh, tid)->near_kind = count <= NEAR ? 3 : 0;
                 cluster.sync();
                 if (sh.near_kind == 3) {
                     if (rank != 0) return;      // nothing of the others' is read any more
                     // each token's place, and the mass before it: the k-th one, then the one with which p of the mass is reached
                     u64 keys[2], before[2], own[2];
-                    int places[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int q = tid + h * F_THREADS;
                         keys[h] = q < count ? sh.near_list[place(q)] : 0;
                         own[h] = q < count ? sh.near_mass[place(q)] : 0;
                         before[h] = 0;
-                        places[h] = 0;
-                        if (q < count)
-                            for (int j = 0; j < count; ++j)
-                                if (sh.near_list[place(j)] > keys[h]) { ++places[h]; before[h] += sh.near_mass[place(j)]; }
-                        if (q < count && places[h] + 1 == k) {
-                            sh.border = keys[h];
-                            sh.border_mass = before[h] + own[h];
+                        int places = 0;
+                        if (q < count) {
+                            const int pushed = (int)sh.near_pushed;
+#pragma unroll 4
+                            for (int j = 0; j < pushed; ++j)
+                                if (sh.near_list[j] > keys[h]) { ++places; before[h] += sh.near_mass[j]; }
+#pragma unroll 4
+                            for (int j = NEAR_LISTED - (count - pushed); j < NEAR_LISTED; ++j)
+                                if (sh.near_list[j] > keys[h]) { ++places; before[h] += sh.near_mass[j]; }
+                            if (places + 1 == k) {
+                                sh.border = keys[h];
+                                sh.border_mass = before[h] + own[h];
+                            }
                         }
                     }
                     __syncthreads();
@@ -763,9 +831,10 @@ sample_filtered_kernel(const FilterParams p) {
                 }
             cluster.sync();
             u64 target = 0;
-            if (rank == 0) {
-                // two steps a thread: the sums up to and with them
-                u64 masses[2], up = 0;
+            // (the first CTA) the near step in which the sum of the masses from `above` on reaches the target, which is p of the whole if there is none
+            // yet: sh.step, and what is before it in sh.above_mass
+            auto locate_near = [&](u64 above) {
+                u64 masses[2], up = 0;      // two steps a thread: the sums up to and with them
 #pragma unroll
                 for (int q = 0; q < 2; ++q) up += masses[q] = ((u64)sh.near_high[2 * tid + q] << 32) + sh.near_low[2 * tid + q];
 #pragma unroll
@@ -781,7 +850,8 @@ sample_filtered_kernel(const FilterParams p) {
                     if (w < warp) up += sh.warp_u64[0][w];
                     all += sh.warp_u64[0][w];
                 }
-                target = s.share(all + sh.rest);
+                if (target == 0) target = s.share(all + sh.rest);
+                up += above;
 #pragma unroll
                 for (int q = 1; q >= 0; --q) {
                     if (up >= target && up - masses[q] < target) {
@@ -791,6 +861,9 @@ sample_filtered_kernel(const FilterParams p) {
                     up -= masses[q];
                 }
                 __syncthreads();
+            };
+            if (rank == 0) {
+                locate_near(0);
                 if (tid < C) cluster.map_shared_rank(&sh, tid)->near_step = sh.step;
             }
             cluster.sync();
@@ -798,13 +871,66 @@ sample_filtered_kernel(const FilterParams p) {
             if (step >= 0) {
                 // the entries of the step lie within these, rounding and all; its tokens alone are ranked
                 const float T_step = T * (1.f / BINS_PER_NAT), slack = 4e-7f * (fabsf(most) + (float)(step + 1) * T_step);
-                list(most - (float)(step + 1) * T_step - slack, most - (float)step * T_step + slack);
+                const float least = most - (float)(step + 1) * T_step - slack, largest = most - (float)step * T_step + slack;
+                list(least, largest);
                 if (rank == 0) {
                     const int count = listed();
-                    if (count <= NEAR_LISTED) {
+                    const bool fits = count <= NEAR_LISTED;
+                    const u64 before = sh.above_mass;
+                    if (fits) {
+                        // the span of (l, index) that the step's tokens take, cut into steps until few are left (each is compared with each then)
+                        auto in_step = [&](u64 key) { return (int)((most - entry_of(key)) * scale) == step; };
+                        u64 from = ~0ull, to = 0, above = sh.above_mass;
+                        if (count > 192) {
+                            for (int q = tid; q < count; q += F_THREADS) {
+                                const u64 key = sh.near_list[place(q)];
+                                if (in_step(key)) { from = min(from, key); to = max(to, key); }
+                            }
+#pragma unroll
+                            for (int o = 16; o > 0; o >>= 1) {
+                                from = min(from, __shfl_xor_sync(0xffffffffu, from, o));
+                                to = max(to, __shfl_xor_sync(0xffffffffu, to, o));
+                            }
+                            if (lane == 0) { sh.warp_u64[0][warp] = from; sh.warp_u64[1][warp] = to; }
+                            __syncthreads();
+                            for (int w = 0; w < F_WARPS; ++w) {
+                                from = min(from, sh.warp_u64[0][w]);
+                                to = max(to, sh.warp_u64[1][w]);
+                            }
+                        } else {
+                            from = 0;
+                            to = ~0ull;
+                        }
+                        auto left = [&](u64 key) { return key >= from && key <= to && in_step(key); };
+                        for (int level = 0; level < 7 && count > 192; ++level) {
+                            int own = 0;
+                            for (int q = tid; q < count; q += F_THREADS) own += left(sh.near_list[place(q)]);
+                            own = __reduce_add_sync(0xffffffffu, own);
+                            if (lane == 0) sh.warp_u64[0][warp] = own;
+                            for (int b = tid; b < NEAR; b += F_THREADS) sh.near_low[b] = sh.near_high[b] = 0;
+                            __syncthreads();
+                            int few = 0;
+                            for (int w = 0; w < F_WARPS; ++w) few += (int)sh.warp_u64[0][w];
+                            if (few <= 64) break;
+                            int shift = 0;
+                            while ((to - from) >> shift >= NEAR) ++shift;
+                            for (int q = tid; q < count; q += F_THREADS) {
+                                const u64 key = sh.near_list[place(q)];
+                                if (!left(key)) continue;
+                                const int b = (int)((to - key) >> shift);
+                                const unsigned f = sh.near_mass[place(q)], old = atomicAdd(&sh.near_low[b], f);
+                                if (old + f < old) atomicAdd(&sh.near_high[b], 1u);
+                            }
+                            __syncthreads();
+                            locate_near(above);
+                            above = sh.above_mass;
+                            to -= (u64)sh.step << shift;
+                            from = max(from, to - ((1ull << shift) - 1));
+                            __syncthreads();
+                        }
                         for (int q = tid; q < count; q += F_THREADS) {
                             const u64 key = sh.near_list[place(q)];
-                            if ((int)((most - entry_of(key)) * scale) == step) {
+                            if (left(key)) {
                                 const unsigned at = atomicAdd(&sh.listed, 1u);
                                 if (at < LISTED) {
                                     sh.list[at] = key;
@@ -812,71 +938,64 @@ sample_filtered_kernel(const FilterParams p) {
                                 }
                             }
                         }
+                        __syncthreads();
+                        s.rank_list([&](int q) { return sh.list[q]; }, [&](int q) { return sh.list_mass[q]; }, min((int)sh.listed, LISTED), true, target, 0, above);
                     }
-                    __syncthreads();
-                    const bool fits = count <= NEAR_LISTED && sh.listed <= LISTED;
-                    if (fits)
-                        s.rank_list([&](int q) { return sh.list[q]; }, [&](int q) { return sh.list_mass[q]; }, (int)sh.listed, true, target, 0, sh.above_mass);
+                    if (tid == 0) sh.listed = 0;
                     if (tid < C) {
                         FilterShared* other = cluster.map_shared_rank(&sh, tid);
                         other->border = sh.border;
-                        other->near_kind = fits;
+                        other->near_kind = fits ? 1 : 2;
+                        other->step = step;
+                        other->above_mass = before;
+                        other->above_count = 0;
+                        other->inside = LISTED + 1;
+                        other->target = target;
                     }
                 }
                 cluster.sync();
                 kind = sh.near_kind;
+                if (kind == 2) {      // more (equal entries, as a rule) than the list holds
+                    Slice copy = s;
+                    copy.refine(true, sh.target, least, largest);
+                }
             }
         }
         if (kind == 0) {
             __syncthreads();
-            if (tid == 0) sh.listed = 0;
             Slice copy = s;      // (its address is taken: the original stays in registers)
             far_border(copy, k, by_count, by_mass);
         }
         border = sh.border;
     }
-    const float border_l = border ? entry_of(border) : -INFINITY;
-    // (what is likely to be as far as min_p allows is looked at closely; a NaN is not)
-    const float far = min_p > 0.f ? 0.01f - logf(min_p) : INFINITY;
-    // 3'. gathered, then worked on
-    constexpr int ROUND = GATHERED / 4;      // vectors
+    // 3'. gathered, then worked on.  What min_p may leave lies within a little more than -log(min_p) T of the largest entry.
+    float least = border ? entry_of(border) : -INFINITY;
+    if (min_p > 0.f) least = fmaxf(least, most - (0.01f - logf(min_p)) * T - 4e-7f * fabsf(most));
+    auto put = [&](unsigned at, float, int i) {
+        if (at < GATHERED) sh.gathered[at] = i;
+    };
+    constexpr int ROUND = GATHERED / 4 - F_THREADS / 4;      // vectors, so that the ends fit too
     for (int from = 0; from == 0 || from < s.body; from += ROUND) {
         __syncthreads();
         if (tid == 0) sh.n_gathered = 0;
         __syncthreads();
-        auto gather = [&](float l, int i) {
-            if (l >= border_l && s.distance(l) <= far && s.composite(l, i) >= border) {
-                const unsigned at = atomicAdd(&sh.n_gathered, 1u);
-                if (at < GATHERED) sh.gathered[at] = i;
-            }
-        };
-        for (int i = from + tid; i < s.body && i < from + ROUND; i += F_THREADS) {
-            const float4 v = *reinterpret_cast<const float4*>(s.held + s.head + 4 * i);
-            if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= border_l)) continue;
-            const int at = s.head + 4 * i;
-            gather(v.x, at);
-            gather(v.y, at + 1);
-            gather(v.z, at + 2);
-            gather(v.w, at + 3);
-        }
+        s.pick(from, min(s.body, from + ROUND), least, INFINITY, &sh.n_gathered, put);
+        if (from == 0) s.pick_ends(least, INFINITY, &sh.n_gathered, put);
         __syncthreads();
         const int count = min((int)sh.n_gathered, GATHERED);
-        for (int q = tid; q < count; q += F_THREADS) score(s.held[sh.gathered[q]], begin + sh.gathered[q]);
+        for (int q = tid; q < count; q += F_THREADS) {
+            const int i = sh.gathered[q];
+            const float l = s.held[i];
+            if (s.composite(l, i) >= border) score(l, begin + i);
+        }
     }
-    // the ends of the slice, off its vectors
-    auto end = [&](int i) {
-        const float l = s.held[i];
-        if (l >= border_l && s.distance(l) <= far && s.composite(l, i) >= border) score(l, begin + i);
-    };
-    if (tid < head) end(tid);
-    if (head + 4 * s.body + tid < n) end(head + 4 * s.body + tid);
     finish(best);
 }
 }  // namespace
 
 // logits [R, V] fp32 with row stride ld; temperature [R], seeds [R], token_index [R] (null where all rows are greedy); top_k [R] int32 (0: all), top_p [R]
 // (1: all), min_p [R] (0: all), each may be null; out [R] int32.
-// cluster: CTAs per row (1, 2, 4, 8), 0 for the kernel's own choice.
+// cluster: CTAs per row (1, 2, 4, 8, 16), 0 for the kernel's own choice.
 PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float* temperature, const unsigned long long* seeds,
                                   const int* token_index, const int* top_k, const float* top_p, const float* min_p, int* out, int n_rows,
                                   int V, int cluster, cudaStream_t stream) {
@@ -895,7 +1014,8 @@ PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float
     static bool configured[PYRE_MAX_DEVICES] = {};      // the attribute is per device
     bool& done = configured[pyre_current_device()];
     if (!done) {
-        const cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RESIDENT);
+        cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RESIDENT);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return (int)e;
         done = true;
     }

@@ -178,7 +178,7 @@ def test_a_rows_token_does_not_depend_on_the_batch():
 
 @pytest.mark.parametrize("form", ["normal", "coarse", "flat", "equal", "peaked"])
 def test_any_number_of_ctas_per_row_gives_the_same(form, monkeypatch):
-    """Borders are found in whole numbers: 1 to 8 CTAs per row agree to the bit, on rows whose borders lie near the best token or far, or among ties."""
+    """Borders are found in whole numbers: 1 to 16 CTAs per row agree to the bit, on rows whose borders lie near the best token or far, or among ties."""
     from pyre_b200.kernels import ops
     R, V = 45, 60001
     logits = torch.randn((R, V), generator=gen(77), device="cuda") * {"normal": 2, "coarse": 2, "flat": 0.01, "equal": 0, "peaked": 0.5}[form]
@@ -188,7 +188,7 @@ def test_any_number_of_ctas_per_row_gives_the_same(form, monkeypatch):
         logits[:, 100:140] += 9
     rule = rules(123, R)
     want = None
-    for cluster in (0, 1, 2, 4, 8):
+    for cluster in (0, 1, 2, 4, 8, 16):
         monkeypatch.setattr(ops, "_SAMPLE_CLUSTER", cluster)
         ids = call(logits, *rule)
         if want is None:
