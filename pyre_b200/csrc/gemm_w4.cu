@@ -6,9 +6,12 @@
 // The inner sums are exact (32-bit integers: |sum| <= 16 * 8 * 127 * 128 < 2^21, a weight's half byte stays in the upper half of its byte, which
 // makes it sixteen times as large and spares the sign's extension), the outer ones in float, by ascending group in each of a CTA's warps,
 // then over the warps in order.
+#include <cooperative_groups.h>
+
 #include "tensor_core.cuh"
 
 namespace {
+namespace cg = cooperative_groups;
 constexpr int GROUP = 128;
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -26,73 +29,194 @@ struct W4Params {
     const __nv_bfloat16* scales;  // [G][N]
     void* out;                    // [M][N]
     int M, N, G;
+    int* err_flag;
 };
 
-constexpr int WARPS = 8;
+constexpr int ERR_TIMEOUT = 2;
+constexpr int FEATURES = 128, W_BYTES = FEATURES * GROUP / 2;      // of a tile
 
-// A CTA owns 16 features and NT tiles of 8 tokens; its warps take the groups in turn.  Lane l of a warp holds 32 neighbouring elements (the
-// l % 4th quarter of the group) of features l / 4 and l / 4 + 8 and of token l / 4: which k an MMA step sums over is free as long as
-// both operands agree.
-template <int NT, typename T>
-__global__ void __launch_bounds__(WARPS * 32)
-w4_few_kernel(const W4Params p) {
-    __shared__ float sums[WARPS][NT * 4][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, c = lane & 3;
-    const int f0 = blockIdx.x * 16, t0 = blockIdx.y * NT * 8;
-    const int fa = min(f0 + quad, p.N - 1), fb = min(f0 + quad + 8, p.N - 1);
-    const size_t pitch = (size_t)p.G * GROUP;
-    const uint8_t* wa = p.packed + fa * (pitch / 2) + c * 16;
-    const uint8_t* wb = p.packed + fb * (pitch / 2) + c * 16;
-    const uint8_t* x[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) x[n] = p.rows + (size_t)min(t0 + n * 8 + quad, p.M - 1) * pitch + c * 32;
-    pdl_trigger();
-    pdl_wait();
-    float total[NT][4] = {};
-    for (int g = warp; g < p.G; g += WARPS) {
-        const uint4 a4 = *reinterpret_cast<const uint4*>(wa + (size_t)g * (GROUP / 2));
-        const uint4 b4 = *reinterpret_cast<const uint4*>(wb + (size_t)g * (GROUP / 2));
-        const float sa = __bfloat162float(p.scales[(size_t)g * p.N + fa]) * 0.0625f;
-        const float sb = __bfloat162float(p.scales[(size_t)g * p.N + fb]) * 0.0625f;
-        const uint32_t a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const uint4 x0 = *reinterpret_cast<const uint4*>(x[n] + (size_t)g * GROUP);
-            const uint4 x1 = *reinterpret_cast<const uint4*>(x[n] + (size_t)g * GROUP + 16);
-            const uint32_t xv[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-            int d[4] = {};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mma_s8(d, lower(a[j]), lower(b[j]), upper(a[j]), upper(b[j]), xv[2 * j], xv[2 * j + 1]);
-            const float* s = p.row_scales + (size_t)g * p.ld_scales;
-            const float s0 = s[min(t0 + n * 8 + 2 * c, p.M - 1)], s1 = s[min(t0 + n * 8 + 2 * c + 1, p.M - 1)];
-            total[n][0] = fmaf((float)d[0] * s0, sa, total[n][0]);
-            total[n][1] = fmaf((float)d[1] * s1, sa, total[n][1]);
-            total[n][2] = fmaf((float)d[2] * s0, sb, total[n][2]);
-            total[n][3] = fmaf((float)d[3] * s1, sb, total[n][3]);
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sums[warp][n * 4 + i][lane] = total[n][i];
-    __syncthreads();
-    for (int e = warp; e < NT * 4; e += WARPS) {
-        float v = sums[0][e][lane];
-        for (int w = 1; w < WARPS; ++w) v += sums[w][e][lane];
-        const int t = t0 + (e >> 2) * 8 + 2 * c + (e & 1), f = f0 + quad + (e & 2) * 4;
-        if (t < p.M && f < p.N) ElemOps<T>::store((T*)p.out + (size_t)t * p.N + f, v);
-    }
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err_flag) {
+    return mbar_wait_or<ERR_TIMEOUT>(bar, parity, abort_flag, err_flag);
+}
+// ... that does not look at the abort flag: for copies and MMAs in flight, before the CTA gives its memory back.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity) && clock64() - t0 < PYRE_WAIT_CYCLES) {}
 }
 
-template <typename T>
-int launch_few(const W4Params& p, cudaStream_t stream) {
-    const int tiles = ceil_div(p.M, 8), nt = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
-    const dim3 grid(ceil_div(p.N, 16), ceil_div(tiles, nt));
-    if (nt == 4) pyre_launch(w4_few_kernel<4, T>, grid, dim3(WARPS * 32), 0, stream, p);
-    else if (nt == 2) pyre_launch(w4_few_kernel<2, T>, grid, dim3(WARPS * 32), 0, stream, p);
-    else pyre_launch(w4_few_kernel<1, T>, grid, dim3(WARPS * 32), 0, stream, p);
-    PYRE_LAUNCH_CHECK();
-    return 0;
+// ---------------------------------------------------------------------------
+// Few rows: a stream of weights from memory.  A CTA owns 128 features and up to 8 NT tokens; the CTAs of a cluster share a tile's K.
+//   warp 8, one thread : TMA.  A group of 128 k at a time into a ring of STAGES: the weights as they are packed, the tokens' bytes.
+//   warp 9             : the group's scales, of the features (a sixteenth of them: the integers are sixteen times as large) and of the tokens.
+//   warps 0..7         : two sets of four that take the groups in turn; a warp owns 32 features.  Lane l holds 32 neighbouring elements (the l % 4th quarter
+//                        of the group) of features l / 4 + 0, 8, 16, 24 and of token l / 4: which k an MMA step sums over is free as long as both
+//                        operands agree.
+// The sets' and the cluster's shares meet in shared memory and are added in order.
+// ---------------------------------------------------------------------------
+constexpr int STREAM_THREADS = 320, STREAM_STAGES = 8;
+
+template <int NT> struct Stream {
+    static constexpr int X_BYTES = NT * 8 * GROUP;
+    static constexpr int STAGE = W_BYTES + X_BYTES;                                                   // multiples of 1,024: the swizzles' patterns
+    static constexpr int SCALES = STREAM_STAGES * STAGE, SCALE = (FEATURES + NT * 8) * 4;             // [stage][features, tokens] floats
+    static constexpr int BARS = SCALES + STREAM_STAGES * SCALE;
+    static constexpr int TOTAL = BARS + STREAM_STAGES * 16 + 16 + 1024;
+    static_assert(2 * NT * 8 * FEATURES * 4 <= SCALES, "the sets' sums take the ring's place");
+};
+
+template <int NT, typename T>
+__global__ void __launch_bounds__(STREAM_THREADS, 2)
+w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const W4Params p, int per_cta) {
+    using L = Stream<NT>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t full = base + L::BARS, empty = full + 8 * STREAM_STAGES;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::BARS + 16 * STREAM_STAGES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int f0 = blockIdx.x / C * FEATURES, t0 = blockIdx.y * NT * 8;
+    const int first = rank * per_cta, n = max(0, min(per_cta, p.G - first));
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < STREAM_STAGES; ++s) { mbar_init(full + 8 * s, 2); mbar_init(empty + 8 * s, 4); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_trigger();
+    bool ok = true;
+    if (warp == 8) {
+        if (lane == 0) {
+            const int early = min(n, STREAM_STAGES);      // the weights depend on no earlier kernel
+            int asked = 0;
+            auto weights = [&](int i) {
+                const int s = i % STREAM_STAGES;
+                mbar_expect_tx(full + 8 * s, L::STAGE);
+                tma_load_2d(base + s * L::STAGE, &map_w, full + 8 * s, (first + i) * (GROUP / 2), f0);
+            };
+            for (int i = 0; i < early; ++i) weights(i);
+            pdl_wait();
+            for (int i = 0; i < n; ++i) {
+                const int s = i % STREAM_STAGES;
+                if (i >= early) {
+                    if (!(ok = mbar_wait(empty + 8 * s, ((i / STREAM_STAGES) & 1) ^ 1, abort_flag, p.err_flag))) break;
+                    weights(i);
+                }
+                tma_load_2d(base + s * L::STAGE + W_BYTES, &map_x, full + 8 * s, (first + i) * GROUP, t0);
+                asked = i + 1;
+            }
+            if (!ok)      // a wait ran out: the copies in flight end first
+                for (int i = max(0, asked - STREAM_STAGES); i < asked; ++i) mbar_drain(full + 8 * (i % STREAM_STAGES), (i / STREAM_STAGES) & 1);
+        }
+    } else if (warp == 9) {
+        constexpr int BATCH = 4, F = FEATURES / 32, X = (NT * 8 + 31) / 32;
+        bool waited = false;
+        for (int i0 = 0; i0 < n && ok; i0 += BATCH) {
+            float v[BATCH][F + X];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j)
+#pragma unroll
+                for (int q = 0; q < F; ++q)
+                    v[j][q] = __bfloat162float(p.scales[(size_t)(first + min(i0 + j, n - 1)) * p.N + min(f0 + q * 32 + lane, p.N - 1)]) * 0.0625f;
+            if (!waited) pdl_wait();
+            waited = true;
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j)
+#pragma unroll
+                for (int q = 0; q < X; ++q)
+                    v[j][F + q] = p.row_scales[(size_t)(first + min(i0 + j, n - 1)) * p.ld_scales + min(t0 + q * 32 + lane, p.M - 1)];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const int i = i0 + j, s = i % STREAM_STAGES;
+                if (i >= n) break;
+                ok = mbar_wait(empty + 8 * s, ((i / STREAM_STAGES) & 1) ^ 1, abort_flag, p.err_flag) && ok;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                float* const to = reinterpret_cast<float*>(gen + L::SCALES + s * L::SCALE);
+#pragma unroll
+                for (int q = 0; q < F; ++q) to[q * 32 + lane] = v[j][q];
+#pragma unroll
+                for (int q = 0; q < X; ++q)
+                    if (q * 32 + lane < NT * 8) to[FEATURES + q * 32 + lane] = v[j][F + q];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + 8 * s);
+            }
+        }
+        if (!waited) pdl_wait();
+    } else {
+        const int set = warp >> 2, row0 = (warp & 3) * 32, quad = lane >> 2, c = lane & 3;
+        float total[NT][2][4] = {};
+        for (int i = set; i < n; i += 2) {
+            const int s = i % STREAM_STAGES;
+            ok = mbar_wait(full + 8 * s, (i / STREAM_STAGES) & 1, abort_flag, p.err_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint32_t stage = base + s * L::STAGE;
+            uint32_t a[4][4];      // rows quad + 0, 8, 16, 24
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = row0 + q * 8 + quad;      // 64-byte swizzle: a chunk of 16 bytes by bits 7 and 8
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a[q][0]), "=r"(a[q][1]), "=r"(a[q][2]), "=r"(a[q][3])
+                             : "r"(stage + row * 64 + ((c ^ ((row >> 1) & 3)) << 4)) : "memory");
+            }
+            const float* const scales = reinterpret_cast<const float*>(gen + L::SCALES + s * L::SCALE);
+            float sw[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sw[q] = scales[row0 + q * 8 + quad];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const uint32_t src = stage + W_BYTES + (t * 8 + quad) * GROUP;      // 128-byte swizzle: a chunk of 16 bytes by bits 7 to 9
+                uint32_t x[8];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                             : "r"(src + (((2 * c) ^ quad) << 4)) : "memory");
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
+                             : "r"(src + (((2 * c + 1) ^ quad) << 4)) : "memory");
+                const float2 sx = *reinterpret_cast<const float2*>(scales + FEATURES + t * 8 + 2 * c);
+                int d[2][4] = {};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        mma_s8(d[h], lower(a[2 * h][j]), lower(a[2 * h + 1][j]), upper(a[2 * h][j]), upper(a[2 * h + 1][j]), x[2 * j], x[2 * j + 1]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    total[t][h][0] = fmaf((float)d[h][0] * sx.x, sw[2 * h], total[t][h][0]);
+                    total[t][h][1] = fmaf((float)d[h][1] * sx.y, sw[2 * h], total[t][h][1]);
+                    total[t][h][2] = fmaf((float)d[h][2] * sx.x, sw[2 * h + 1], total[t][h][2]);
+                    total[t][h][3] = fmaf((float)d[h][3] * sx.y, sw[2 * h + 1], total[t][h][3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + 8 * s);
+        }
+        // [set][token][feature]; the ring is free once both sets are through it
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        float* const sums = reinterpret_cast<float*>(gen) + set * NT * 8 * FEATURES;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sums[(t * 8 + 2 * c + (e & 1)) * FEATURES + row0 + h * 16 + (e >> 1) * 8 + quad] = total[t][h][e];
+    }
+    const bool failed = __syncthreads_or(!ok);
+    if (C > 1) cluster.sync();
+    if (!failed) {
+        // (a CTA that gave up raised the error word: what the others write is not looked at)
+        const int tokens = min(NT * 8, p.M - t0);
+        for (int i = rank * STREAM_THREADS + threadIdx.x; i < tokens * FEATURES; i += C * STREAM_THREADS) {
+            const int f = f0 + i % FEATURES;
+            float v = 0.f;
+            for (int q = 0; q < C; ++q) {
+                const float* const sums = reinterpret_cast<const float*>(C > 1 ? cluster.map_shared_rank(gen, q) : gen);
+                v += sums[i] + sums[NT * 8 * FEATURES + i];
+            }
+            if (f < p.N) ElemOps<T>::store((T*)p.out + (size_t)(t0 + i / FEATURES) * p.N + f, v);
+        }
+    }
+    if (C > 1) cluster.sync();      // the others' sums are read
 }
 
 // ---------------------------------------------------------------------------
@@ -106,11 +230,9 @@ int launch_few(const W4Params& p, cudaStream_t stream) {
 //                        feature and added to float sums in registers, by ascending group.
 // An output tile whose K is shared among CTAs (few tiles) leaves float shares, added up in order by whoever reads them.
 // ---------------------------------------------------------------------------
-constexpr int ERR_TIMEOUT = 2;
-constexpr int FEATURES = 128, MANY_THREADS = 768, EPI_WARP0 = 8, EPI_WARPS = 16, A_COLS = 32;
+constexpr int MANY_THREADS = 768, EPI_WARP0 = 8, EPI_WARPS = 16, A_COLS = 32;
 constexpr int W_STAGES = 6, STAGES = 6;               // packed weights; both operands of the MMAs
 constexpr int BATCH = 4, S_STAGES = 2;                // groups whose scales come at a time
-constexpr int W_BYTES = FEATURES * GROUP / 2;
 
 struct ManyParams {
     const float* row_scales;
@@ -124,14 +246,6 @@ struct ManyParams {
     int* err_flag;
 };
 
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err_flag) {
-    return mbar_wait_or<ERR_TIMEOUT>(bar, parity, abort_flag, err_flag);
-}
-// ... that does not look at the abort flag: for copies and MMAs in flight, before the CTA gives its memory back.
-__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity) && clock64() - t0 < PYRE_WAIT_CYCLES) {}
-}
 __device__ __forceinline__ bool elect_one() {
     uint32_t one;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
@@ -483,7 +597,7 @@ bool byte_map(CUtensorMap* map, const void* p, int rows, long long pitch, int wi
 }
 
 template <int TN, typename T>
-int launch_many(const W4Params& w, int splits, int* err_flag, cudaStream_t stream) {
+int launch_many(const W4Params& w, int splits, cudaStream_t stream) {
     using L = Many<TN>;
     static bool configured_on[PYRE_MAX_DEVICES] = {};      // the attribute is per device
     bool& configured = configured_on[pyre_current_device()];
@@ -494,7 +608,7 @@ int launch_many(const W4Params& w, int splits, int* err_flag, cudaStream_t strea
     }
     CUtensorMap mw, mx;
     if (!byte_map(&mw, w.packed, w.N, 64ll * w.G, 64, FEATURES) || !byte_map(&mx, w.rows, w.M, 128ll * w.G, 128, TN)) return PYRE_ERR_BAD_ARG;
-    ManyParams p = {w.row_scales, w.ld_scales, w.scales, w.out, w.M, w.N, w.G, ceil_div(w.M, TN), 0, splits, ceil_div(w.G, splits), w.N % (16 / (int)sizeof(T)) == 0 && !((uintptr_t)w.out & 15), err_flag};
+    ManyParams p = {w.row_scales, w.ld_scales, w.scales, w.out, w.M, w.N, w.G, ceil_div(w.M, TN), 0, splits, ceil_div(w.G, splits), w.N % (16 / (int)sizeof(T)) == 0 && !((uintptr_t)w.out & 15), w.err_flag};
     const long long tiles = (long long)p.tiles_m * ceil_div(w.N, FEATURES);
     if (tiles * splits > 0x7fffffffll) return PYRE_ERR_UNSUPPORTED;
     p.tiles = (int)tiles;
@@ -504,7 +618,52 @@ int launch_many(const W4Params& w, int splits, int* err_flag, cudaStream_t strea
     PYRE_LAUNCH_CHECK();
     return 0;
 }
-constexpr int FEW = 32;      // rows up to here take the other kernel
+
+// CTAs that share a tile's K: as many as find room on the SMs, each with four groups at least.
+template <int NT, typename T>
+int launch_stream(const W4Params& p, cudaStream_t stream) {
+    using L = Stream<NT>;
+    static bool configured_on[PYRE_MAX_DEVICES] = {};      // the attribute is per device
+    bool& configured = configured_on[pyre_current_device()];
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(w4_stream_kernel<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    CUtensorMap mw, mx;
+    if (!byte_map(&mw, p.packed, p.N, 64ll * p.G, 64, FEATURES) || !byte_map(&mx, p.rows, p.M, 128ll * p.G, 128, NT * 8)) return PYRE_ERR_BAD_ARG;
+    const int tiles = ceil_div(p.N, FEATURES), rows = ceil_div(p.M, NT * 8), room = 2 * pyre_sm_count();
+    int C = 1;
+    while (C < 8 && 2ll * C * tiles * rows <= room && p.G >= 8 * C) C *= 2;
+    const int per = ceil_div(p.G, C);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)rows);
+    cfg.blockDim = dim3(STREAM_THREADS);
+    cfg.dynamicSmemBytes = L::TOTAL;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pyre_pdl_enabled() ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_stream_kernel<NT, T>, mw, mx, p, per);
+    if (e != cudaSuccess) return (int)e;
+    PYRE_LAUNCH_CHECK();
+    return 0;
+}
+template <typename T>
+int launch_few(const W4Params& p, cudaStream_t stream) {
+    switch (ceil_div(p.M, 8)) {
+        case 1: return launch_stream<1, T>(p, stream);
+        case 2: return launch_stream<2, T>(p, stream);
+        case 3: return launch_stream<3, T>(p, stream);
+        default: return launch_stream<4, T>(p, stream);
+    }
+}
+constexpr int FEW = 32;      // rows up to here take the stream
 
 // A warp per group of a feature: s = bf16(max |w| / 7), q = rint(w / s) within -8 .. 7.  A group of zeros (or below 2^-100) has s = 0, one with an
 // infinity or a NaN s = NaN.
@@ -593,8 +752,8 @@ PYRE_API int pyre_w4_linear(const void* rows, const float* row_scales, long long
     if (G <= 0 || ((uintptr_t)rows & 15) || ((uintptr_t)packed & 15)) return PYRE_ERR_BAD_ARG;
     if (dtype != PYRE_F32 && dtype != PYRE_BF16) return PYRE_ERR_BAD_ARG;
     if (splits < 1 || (splits > 1 && (M <= FEW || dtype != PYRE_F32 || (splits - 1) * ceil_div(G, splits) >= G))) return PYRE_ERR_BAD_ARG;
-    const W4Params p = {(const uint8_t*)rows, row_scales, ld_scales, (const uint8_t*)packed, (const __nv_bfloat16*)scales, out, M, N, G};
+    const W4Params p = {(const uint8_t*)rows, row_scales, ld_scales, (const uint8_t*)packed, (const __nv_bfloat16*)scales, out, M, N, G, err_flag};
     if (M <= FEW) return dtype == PYRE_F32 ? launch_few<float>(p, stream) : launch_few<__nv_bfloat16>(p, stream);
-    if (M <= 64) return dtype == PYRE_F32 ? launch_many<64, float>(p, splits, err_flag, stream) : launch_many<64, __nv_bfloat16>(p, splits, err_flag, stream);
-    return dtype == PYRE_F32 ? launch_many<128, float>(p, splits, err_flag, stream) : launch_many<128, __nv_bfloat16>(p, splits, err_flag, stream);
+    if (M <= 64) return dtype == PYRE_F32 ? launch_many<64, float>(p, splits, stream) : launch_many<64, __nv_bfloat16>(p, splits, stream);
+    return dtype == PYRE_F32 ? launch_many<128, float>(p, splits, stream) : launch_many<128, __nv_bfloat16>(p, splits, stream);
 }

@@ -179,16 +179,16 @@ PYRE_API int pyre_sample(const float* logits, long long ld, const float* tempera
 // A cluster of CTAs shares a row; each keeps its slice in shared memory where two such CTAs fit on an SM, else it reads it again (out of L2).  Masses
 // are whole numbers (w 2^31, summed in 64 bits), so neither the order of the additions nor the cluster's size can move a border: results do
 // not depend on them.
-//   1. max l, and the largest entry that each thread has read.
-//   2. k: as many threads as k have read an entry of at least t, where t is the k-th of those (or somewhat below): no token below t is among the first k.  The
-//      tokens from t on, hardly more than k, go to the first CTA's list, and the other CTAs are done.  It ranks them by (l, index), which gives the
-//      border token of k and of p after k, and adds the noise.
+//   1. max l, and the largest entry of each block of 128: what follows reads the blocks again that hold entries it looks for.
+//   2. k: as many blocks as k have an entry of at least t, where t is the k-th of their largest ones (or somewhat below): no token below t is among the first
+//      k.  The tokens from t on, hardly more than k, go to the first CTA's list, and the other CTAs are done.  It ranks them by (l, index), which
+//      gives the border token of k and of p after k, and adds the noise.
 //   2'. p alone: a histogram of masses by distance (max l - l) / T in steps of 1/64 (l decides the step alone and in order) of the tokens less than NEAR steps
 //      away; the others' mass stays in registers.  It gives the step in which the p-th part of the mass lies, whose tokens go to the list and are
 //      ranked.  All CTAs look for the tokens up to the border.
 //   3'. The tokens up to the border are gathered before they get their noise: they are few in any 32 neighbours, and a token's noise is some
 //      hundred instructions.
-//   Where that does not do (the border lies further away, more equal entries than the list holds, k beyond the threads), `far_border` finds it: a histogram of
+//   Where that does not do (the border lies further away, more equal entries than the list holds, k beyond the blocks), `far_border` finds it: a histogram of
 //   all tokens, and the span of (l, index) in question cut into as many steps again until its tokens fit.
 // ---------------------------------------------------------------------------
 namespace {
@@ -196,7 +196,7 @@ namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 constexpr int F_THREADS = 512, F_WARPS = F_THREADS / 32, BINS = 2048, NEAR = 2 * F_THREADS, LISTED = 512, NEAR_LISTED = 2048, MAX_CLUSTER = 16;
 constexpr float BINS_PER_NAT = 64.f;
-constexpr int GATHERED = 6144;
+constexpr int GATHERED = 6144, BLOCKS = 1216, ALL_BLOCKS = 4096;      // of a CTA, of a row
 
 struct FilterParams {
     const float* logits;
@@ -222,9 +222,10 @@ struct FilterShared {
             u64 near_list[NEAR_LISTED];
             unsigned near_mass[NEAR_LISTED];
         };
-        float thread_most[MAX_CLUSTER * F_THREADS / 2];
+        float all_most[ALL_BLOCKS];
         unsigned gathered[GATHERED];
     };
+    float block_most[BLOCKS];
     u64 list[LISTED];
     unsigned list_mass[LISTED];
     u64 slots[2][MAX_CLUSTER][2];                     // what the cluster's CTAs tell each other
@@ -266,6 +267,7 @@ struct Slice {
     FilterShared& sh;
     cg::cluster_group cluster;
     int C, rank, begin, n, head, body;      // entries: begin .. begin + n; up to a 16-byte boundary, and whole vectors after it
+    int blocks;                             // whose largest entries are known
     int turn;
     const float* held;
     float most, inv_t, top_p;
@@ -298,40 +300,46 @@ struct Slice {
             if (count == 4) { f(v.y, i + 1); f(v.z, i + 2); f(v.w, i + 3); }
         });
     }
-    // put(place, entry, its index) for the whole vectors from `from` to `to` whose entries lie from `least` to `largest`; the places are taken from
-    // `counter`, a warp's at once (no thread may be elsewhere).
+    // put(place, entry, its index) for the entries from `least` to `largest` in the blocks (of 32 whole vectors) from `from` to `to`; the places are taken
+    // from `counter`, a warp's at once (no thread may be elsewhere).
     template <typename F> __device__ __forceinline__ void pick(int from, int to, float least, float largest, unsigned* counter, F put) const {
         const int lane = threadIdx.x & 31;
         constexpr int AHEAD = 4;
-        for (int i0 = from + (threadIdx.x & ~31); i0 < to; i0 += AHEAD * F_THREADS) {
-            float4 v[AHEAD];
+        for (int b0 = from + (threadIdx.x >> 5); b0 < to; b0 += 32 * F_WARPS) {      // a warp's blocks lie F_WARPS apart
+            const int b = b0 + lane * F_WARPS;
+            unsigned hit = __ballot_sync(0xffffffffu, b < to && (b >= blocks || sh.block_most[b] >= least));
+            while (hit) {
+                float4 v[AHEAD];
+                int at[AHEAD];
 #pragma unroll
-            for (int q = 0; q < AHEAD; ++q) {
-                const int i = i0 + q * F_THREADS + lane;
-                v[q] = i < to ? *reinterpret_cast<const float4*>(held + head + 4 * i) : make_float4(NAN, NAN, NAN, NAN);
-            }
-#pragma unroll
-            for (int q = 0; q < AHEAD; ++q) {
-                if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v[q].x, v[q].y), fmaxf(v[q].z, v[q].w)) >= least)) continue;
-                const float l[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
-                unsigned hits[4], before = 0;
-                int total = 0;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    hits[c] = __ballot_sync(0xffffffffu, l[c] >= least && l[c] <= largest);
-                    total += __popc(hits[c]);
+                for (int q = 0; q < AHEAD; ++q) {
+                    at[q] = hit ? 32 * (b0 + (__ffs(hit) - 1) * F_WARPS) + lane : body;
+                    hit &= hit - 1;
+                    v[q] = at[q] < body ? *reinterpret_cast<const float4*>(held + head + 4 * at[q]) : make_float4(NAN, NAN, NAN, NAN);
                 }
-                if (!total) continue;
-                if (lane == 0) before = atomicAdd(counter, (unsigned)total);
-                before = __shfl_sync(0xffffffffu, before, 0);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (hits[c] >> lane & 1) put(before + __popc(hits[c] & ((1u << lane) - 1)), l[c], head + 4 * (i0 + q * F_THREADS + lane) + c);
-                    before += __popc(hits[c]);
+                for (int q = 0; q < AHEAD; ++q) {
+                    const float l[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+                    unsigned hits[4], before = 0;
+                    int total = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        hits[c] = __ballot_sync(0xffffffffu, l[c] >= least && l[c] <= largest);
+                        total += __popc(hits[c]);
+                    }
+                    if (!total) continue;
+                    if (lane == 0) before = atomicAdd(counter, (unsigned)total);
+                    before = __shfl_sync(0xffffffffu, before, 0);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (hits[c] >> lane & 1) put(before + __popc(hits[c] & ((1u << lane) - 1)), l[c], head + 4 * at[q] + c);
+                        before += __popc(hits[c]);
+                    }
                 }
             }
         }
     }
+    __device__ __forceinline__ int all_blocks() const { return (body + 31) / 32; }
     // ... and for the entries off whole vectors
     template <typename F> __device__ __forceinline__ void pick_ends(float least, float largest, unsigned* counter, F put) const {
         auto end = [&](int i) {
@@ -600,7 +608,7 @@ sample_filtered_kernel(const FilterParams p) {
     const bool by_count = k > 0 && k < p.V, by_mass = top_p < 1.f;
     const bool filtered = !greedy && (k > 0 || by_mass || min_p > 0.f);
     const int head = min(n, (int)((4 - ((uintptr_t)(row + begin) >> 2)) & 3));
-    Slice s = {sh, cluster, C, rank, begin, n, head, (n - head) / 4, 0, row + begin, -INFINITY, inv_t, top_p};
+    Slice s = {sh, cluster, C, rank, begin, n, head, (n - head) / 4, 0, 0, row + begin, -INFINITY, inv_t, top_p};
 
     auto best_of_block = [&](Best& best) {      // in thread 0
 #pragma unroll
@@ -635,24 +643,40 @@ sample_filtered_kernel(const FilterParams p) {
     float most = -INFINITY;
     {
         float* const mine = reinterpret_cast<float*>(dyn) + (((uintptr_t)s.held >> 2) & 3);      // the same place within 16 bytes
-        s.vectors([&](const float4& v, int i, int count) {
-            most = fmaxf(most, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));      // a NaN is passed over
-            if (!p.resident) return;
-            if (count == 4) *reinterpret_cast<float4*>(mine + i) = v;
-            else mine[i] = v.x;
-        });
+        auto end = [&](int i) {
+            most = fmaxf(most, s.held[i]);      // a NaN is passed over
+            if (p.resident) mine[i] = s.held[i];
+        };
+        if (tid < head) end(tid);
+        if (head + 4 * s.body + tid < n) end(head + 4 * s.body + tid);
+        constexpr int AHEAD = 4;
+        s.blocks = min(s.all_blocks(), BLOCKS);
+        for (int b0 = warp; b0 < s.all_blocks(); b0 += AHEAD * F_WARPS) {
+            float4 v[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int i = 32 * (b0 + q * F_WARPS) + lane;
+                v[q] = i < s.body ? *reinterpret_cast<const float4*>(s.held + head + 4 * i) : make_float4(NAN, NAN, NAN, NAN);
+            }
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int b = b0 + q * F_WARPS, i = 32 * b + lane;
+                const float four = entry(fmaxf(fmaxf(v[q].x, v[q].y), fmaxf(v[q].z, v[q].w)));
+                most = fmaxf(most, four);
+                const unsigned key = __reduce_max_sync(0xffffffffu, order_key(four));
+                if (lane == 0 && b < s.blocks) sh.block_most[b] = entry_of((u64)key << 32);
+                if (p.resident && i < s.body) *reinterpret_cast<float4*>(mine + head + 4 * i) = v[q];
+            }
+        }
         if (p.resident) s.held = mine;
     }
-    // (of 16 CTAs two threads' together)
-    const int values = min(C * F_THREADS, MAX_CLUSTER * F_THREADS / 2);
-    const bool by_threads = by_count && k <= values / 2;
-    if (by_threads) {
-        float* const all = cluster.map_shared_rank(&sh, 0)->thread_most;
-        if (C < MAX_CLUSTER) all[rank * F_THREADS + tid] = most;
-        else {
-            const float two = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            if (!(tid & 1)) all[(rank * F_THREADS + tid) / 2] = two;
-        }
+    // the blocks' largest entries, side by side in the first CTA
+    const int per_cta = (p.slice + 127) / 128 + 1;
+    const bool by_blocks = by_count && C * per_cta <= ALL_BLOCKS && per_cta <= BLOCKS && k <= p.V / 256;
+    if (by_blocks) {
+        __syncthreads();
+        float* const all = cluster.map_shared_rank(&sh, 0)->all_most;
+        for (int b = tid; b < per_cta; b += F_THREADS) all[rank * per_cta + b] = b < s.blocks ? sh.block_most[b] : -INFINITY;
     }
     most = warp_max(most);
     if (lane == 0) sh.warp_best[warp].score = most;
@@ -685,7 +709,7 @@ sample_filtered_kernel(const FilterParams p) {
                     sh.near_mass[NEAR_LISTED - 1 - at] = mass_of(s.distance(l));
                 }
             };
-            s.pick(0, s.body, least, largest, &sh.near_own, put);
+            s.pick(0, s.all_blocks(), least, largest, &sh.near_own, put);
             s.pick_ends(least, largest, &sh.near_own, put);
             __syncthreads();
             if (rank != 0) {
@@ -713,10 +737,11 @@ sample_filtered_kernel(const FilterParams p) {
             if (tid == 0) p.out[r] = best.index == 0x7fffffff ? 0 : best.index;
         };
         int kind = 0;
-        if (by_threads) {
+        if (by_blocks) {
             // 2. t, by the first CTA
             if (rank == 0) {
-                const float* const all = sh.thread_most;
+                const float* const all = sh.all_most;
+                const int values = C * per_cta;
                 float least = INFINITY;
                 for (int q = tid; q < values; q += F_THREADS)
                     if (all[q] > -INFINITY) least = fminf(least, all[q]);
@@ -974,12 +999,12 @@ sample_filtered_kernel(const FilterParams p) {
     auto put = [&](unsigned at, float, int i) {
         if (at < GATHERED) sh.gathered[at] = i;
     };
-    constexpr int ROUND = GATHERED / 4 - F_THREADS / 4;      // vectors, so that the ends fit too
-    for (int from = 0; from == 0 || from < s.body; from += ROUND) {
+    constexpr int ROUND = GATHERED / 128 - 1;      // blocks, and the ends
+    for (int from = 0; from == 0 || from < s.all_blocks(); from += ROUND) {
         __syncthreads();
         if (tid == 0) sh.n_gathered = 0;
         __syncthreads();
-        s.pick(from, min(s.body, from + ROUND), least, INFINITY, &sh.n_gathered, put);
+        s.pick(from, min(s.all_blocks(), from + ROUND), least, INFINITY, &sh.n_gathered, put);
         if (from == 0) s.pick_ends(least, INFINITY, &sh.n_gathered, put);
         __syncthreads();
         const int count = min((int)sh.n_gathered, GATHERED);
@@ -1002,8 +1027,8 @@ PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float
     if (n_rows <= 0) return 0;
     if (V <= 0 || (temperature && (!seeds || !token_index))) return PYRE_ERR_BAD_ARG;
     if (cluster < 0 || cluster > MAX_CLUSTER || (cluster & (cluster - 1))) return PYRE_ERR_BAD_ARG;
-    // CTAs per row: as many as find room, two to an SM.  152,064 entries, first k and p: 64 rows on 1 / 2 / 4 / 8 CTAs each 43 / 32 / 26 / 45 us, one row
-    // 26 / 19 / 15 / 13 us, 256 rows 67 / 69 / 80 / 136 us.
+    // CTAs per row: as many as find room, two to an SM.  152,064 entries, us on 1 / 2 / 4 / 8 CTAs a row: 1 row, k 22 / 16 / 13 / 12 (16 CTAs: 11); 64 rows,
+    // k 40 / 29 / 23 / 58, p 234 / 133 / 82 / 140; 256 rows, k 49 / 59 / 73 / 192, p 316 / 251 / 244 / 503.
     int C = cluster > 0 ? cluster : 1;
     while (!cluster && C < MAX_CLUSTER && n_rows * 2ll * C <= 2 * pyre_sm_count() && V > 2048 * C) C *= 2;
     FilterParams p = {logits, ld, temperature, seeds, token_index, top_k, top_p, min_p, out, V, (ceil_div(V, C) + 3) / 4 * 4, 0};
