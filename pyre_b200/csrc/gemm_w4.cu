@@ -46,22 +46,23 @@ __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
 
 // ---------------------------------------------------------------------------
 // Few rows: a stream of weights from memory.  A CTA owns 128 features and up to 8 NT tokens; the CTAs of a cluster share a tile's K.
-//   warp 8, one thread : TMA.  A group of 128 k at a time into a ring of STAGES: the weights as they are packed, the tokens' bytes.
-//   warp 9             : the group's scales, of the features (a sixteenth of them: the integers are sixteen times as large) and of the tokens.
-//   warps 0..7         : two sets of four that take the groups in turn; a warp owns 32 features.  Lane l holds 32 neighbouring elements (the l % 4th quarter
-//                        of the group) of features l / 4 + 0, 8, 16, 24 and of token l / 4: which k an MMA step sums over is free as long as both
+//   warp 8, one thread : TMA.  Two groups of 128 k at a time into a ring of STAGES: the weights as they are packed, the tokens' bytes.  (A copy of one group
+//                        has rows of 64 bytes, which hold up its engine: 24 x 5,120 x 27,648 took 22.6 us with them, ROWS128 with two.)
+//   warp 9             : the groups' scales, of the features (a sixteenth of them: the integers are sixteen times as large) and of the tokens.
+//   warps 0..7         : two sets of four that take the stages in turn; a warp owns 32 features.  Lane l holds 32 neighbouring elements (the l % 4th quarter
+//                        of the group) of four features and of token l / 4: which k an MMA step sums over is free as long as both
 //                        operands agree.
 // The sets' and the cluster's shares meet in shared memory and are added in order.
 // ---------------------------------------------------------------------------
-constexpr int STREAM_THREADS = 320, STREAM_STAGES = 8;
+constexpr int STREAM_THREADS = 320, STREAM_STAGES = 4, PAIR = 2;
 
 template <int NT> struct Stream {
-    static constexpr int X_BYTES = NT * 8 * GROUP;
-    static constexpr int STAGE = W_BYTES + X_BYTES;                                                   // multiples of 1,024: the swizzles' patterns
-    static constexpr int SCALES = STREAM_STAGES * STAGE, SCALE = (FEATURES + NT * 8) * 4;             // [stage][features, tokens] floats
-    static constexpr int BARS = SCALES + STREAM_STAGES * SCALE;
+    static constexpr int X_BYTES = NT * 8 * GROUP;                                                    // a group's
+    static constexpr int STAGE = PAIR * (W_BYTES + X_BYTES);                                          // multiples of 1,024: the swizzles' patterns
+    static constexpr int SCALES = STREAM_STAGES * STAGE, SCALE = (FEATURES + NT * 8) * 4;             // [stage][group][features, tokens] floats
+    static constexpr int BARS = SCALES + STREAM_STAGES * PAIR * SCALE;
     static constexpr int TOTAL = BARS + STREAM_STAGES * 16 + 16 + 1024;
-    static_assert(2 * NT * 8 * FEATURES * 4 <= SCALES, "the sets' sums take the ring's place");
+    static_assert(2 * NT * 8 * FEATURES * 4 <= SCALES && 2 * (TOTAL + 1024) <= 233472 && STREAM_STAGES % 2 == 0, "the sets' sums take the ring's place; two CTAs");
 };
 
 template <int NT, typename T>
@@ -77,7 +78,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int f0 = blockIdx.x / C * FEATURES, t0 = blockIdx.y * NT * 8;
-    const int first = rank * per_cta, n = max(0, min(per_cta, p.G - first));
+    const int first = rank * per_cta, n = max(0, min(per_cta, p.G - first)), steps = (n + PAIR - 1) / PAIR;      // per_cta is even
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -89,32 +90,34 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     bool ok = true;
     if (warp == 8) {
         if (lane == 0) {
-            const int early = min(n, STREAM_STAGES);      // the weights depend on no earlier kernel
+            const int early = min(steps, STREAM_STAGES);      // the weights depend on no earlier kernel
             int asked = 0;
             auto weights = [&](int i) {
                 const int s = i % STREAM_STAGES;
                 mbar_expect_tx(full + 8 * s, L::STAGE);
-                tma_load_2d(base + s * L::STAGE, &map_w, full + 8 * s, (first + i) * (GROUP / 2), f0);
+                tma_load_2d(base + s * L::STAGE, &map_w, full + 8 * s, (first + PAIR * i) * (GROUP / 2), f0);
             };
             for (int i = 0; i < early; ++i) weights(i);
             pdl_wait();
-            for (int i = 0; i < n; ++i) {
+            for (int i = 0; i < steps; ++i) {
                 const int s = i % STREAM_STAGES;
                 if (i >= early) {
                     if (!(ok = mbar_wait(empty + 8 * s, ((i / STREAM_STAGES) & 1) ^ 1, abort_flag, p.err_flag))) break;
                     weights(i);
                 }
-                tma_load_2d(base + s * L::STAGE + W_BYTES, &map_x, full + 8 * s, (first + i) * GROUP, t0);
+                for (int h = 0; h < PAIR; ++h)      // (beyond the last group: zeros)
+                    tma_load_2d(base + s * L::STAGE + PAIR * W_BYTES + h * L::X_BYTES, &map_x, full + 8 * s, (first + PAIR * i + h) * GROUP, t0);
                 asked = i + 1;
             }
             if (!ok)      // a wait ran out: the copies in flight end first
                 for (int i = max(0, asked - STREAM_STAGES); i < asked; ++i) mbar_drain(full + 8 * (i % STREAM_STAGES), (i / STREAM_STAGES) & 1);
         }
     } else if (warp == 9) {
-        constexpr int BATCH = 4, F = FEATURES / 32, X = (NT * 8 + 31) / 32;
+        constexpr int BATCH = 4, F = FEATURES / 32;
+        static_assert(BATCH % PAIR == 0 && NT <= 4, "whole stages, a lane per token");
         bool waited = false;
         for (int i0 = 0; i0 < n && ok; i0 += BATCH) {
-            float v[BATCH][F + X];
+            float v[BATCH][F], x[BATCH];
 #pragma unroll
             for (int j = 0; j < BATCH; ++j)
 #pragma unroll
@@ -123,69 +126,71 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             if (!waited) pdl_wait();
             waited = true;
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j)
-#pragma unroll
-                for (int q = 0; q < X; ++q)
-                    v[j][F + q] = p.row_scales[(size_t)(first + min(i0 + j, n - 1)) * p.ld_scales + min(t0 + q * 32 + lane, p.M - 1)];
+            for (int j = 0; j < BATCH; ++j) x[j] = p.row_scales[(size_t)(first + min(i0 + j, n - 1)) * p.ld_scales + min(t0 + lane, p.M - 1)];
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
-                const int i = i0 + j, s = i % STREAM_STAGES;
-                if (i >= n) break;
-                ok = mbar_wait(empty + 8 * s, ((i / STREAM_STAGES) & 1) ^ 1, abort_flag, p.err_flag) && ok;
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                float* const to = reinterpret_cast<float*>(gen + L::SCALES + s * L::SCALE);
+                const int i = (i0 + j) / PAIR, s = i % STREAM_STAGES;
+                if (i >= steps) break;
+                if (j % PAIR == 0) {
+                    ok = mbar_wait(empty + 8 * s, ((i / STREAM_STAGES) & 1) ^ 1, abort_flag, p.err_flag) && ok;
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                float* const to = reinterpret_cast<float*>(gen + L::SCALES + (s * PAIR + j % PAIR) * L::SCALE);
 #pragma unroll
                 for (int q = 0; q < F; ++q) to[q * 32 + lane] = v[j][q];
-#pragma unroll
-                for (int q = 0; q < X; ++q)
-                    if (q * 32 + lane < NT * 8) to[FEATURES + q * 32 + lane] = v[j][F + q];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full + 8 * s);
+                if (lane < NT * 8) to[FEATURES + lane] = x[j];
+                if (j % PAIR == PAIR - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full + 8 * s);
+                }
             }
         }
         if (!waited) pdl_wait();
     } else {
         const int set = warp >> 2, row0 = (warp & 3) * 32, quad = lane >> 2, c = lane & 3;
+        // The feature of a lane among eight: neighbouring lanes of four read rows four apart, whose swizzles are different.
+        const int row8 = (quad >> 1) | (quad & 1) << 2;
         float total[NT][2][4] = {};
-        for (int i = set; i < n; i += 2) {
+        for (int i = set; i < steps; i += 2) {
             const int s = i % STREAM_STAGES;
             ok = mbar_wait(full + 8 * s, (i / STREAM_STAGES) & 1, abort_flag, p.err_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const uint32_t stage = base + s * L::STAGE;
-            uint32_t a[4][4];      // rows quad + 0, 8, 16, 24
+            const int groups = min(PAIR, n - PAIR * i);
+            for (int g = 0; g < groups; ++g) {
+                uint32_t a[4][4];      // features row8 + 0, 8, 16, 24
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = row0 + q * 8 + quad;      // 64-byte swizzle: a chunk of 16 bytes by bits 7 and 8
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a[q][0]), "=r"(a[q][1]), "=r"(a[q][2]), "=r"(a[q][3])
-                             : "r"(stage + row * 64 + ((c ^ ((row >> 1) & 3)) << 4)) : "memory");
-            }
-            const float* const scales = reinterpret_cast<const float*>(gen + L::SCALES + s * L::SCALE);
-            float sw[4];
+                for (int q = 0; q < 4; ++q)      // 128-byte swizzle: a chunk of 16 bytes by bits 7 to 9
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a[q][0]), "=r"(a[q][1]), "=r"(a[q][2]), "=r"(a[q][3])
+                                 : "r"(stage + (row0 + q * 8 + row8) * 128 + (((4 * g + c) ^ row8) << 4)) : "memory");
+                const float* const scales = reinterpret_cast<const float*>(gen + L::SCALES + (s * PAIR + g) * L::SCALE);
+                float sw[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) sw[q] = scales[row0 + q * 8 + quad];
+                for (int q = 0; q < 4; ++q) sw[q] = scales[row0 + q * 8 + row8];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint32_t src = stage + W_BYTES + (t * 8 + quad) * GROUP;      // 128-byte swizzle: a chunk of 16 bytes by bits 7 to 9
-                uint32_t x[8];
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                             : "r"(src + (((2 * c) ^ quad) << 4)) : "memory");
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
-                             : "r"(src + (((2 * c + 1) ^ quad) << 4)) : "memory");
-                const float2 sx = *reinterpret_cast<const float2*>(scales + FEATURES + t * 8 + 2 * c);
-                int d[2][4] = {};
+                for (int t = 0; t < NT; ++t) {
+                    const uint32_t src = stage + PAIR * W_BYTES + g * L::X_BYTES + (t * 8 + quad) * GROUP;
+                    uint32_t x[8];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                                 : "r"(src + (((2 * c) ^ quad) << 4)) : "memory");
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
+                                 : "r"(src + (((2 * c + 1) ^ quad) << 4)) : "memory");
+                    const float2 sx = *reinterpret_cast<const float2*>(scales + FEATURES + t * 8 + 2 * c);
+                    int d[2][4] = {};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        mma_s8(d[h], lower(a[2 * h][j]), lower(a[2 * h + 1][j]), upper(a[2 * h][j]), upper(a[2 * h + 1][j]), x[2 * j], x[2 * j + 1]);
+                        for (int h = 0; h < 2; ++h)
+                            mma_s8(d[h], lower(a[2 * h][j]), lower(a[2 * h + 1][j]), upper(a[2 * h][j]), upper(a[2 * h + 1][j]), x[2 * j], x[2 * j + 1]);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    total[t][h][0] = fmaf((float)d[h][0] * sx.x, sw[2 * h], total[t][h][0]);
-                    total[t][h][1] = fmaf((float)d[h][1] * sx.y, sw[2 * h], total[t][h][1]);
-                    total[t][h][2] = fmaf((float)d[h][2] * sx.x, sw[2 * h + 1], total[t][h][2]);
-                    total[t][h][3] = fmaf((float)d[h][3] * sx.y, sw[2 * h + 1], total[t][h][3]);
+                    for (int h = 0; h < 2; ++h) {
+                        total[t][h][0] = fmaf((float)d[h][0] * sx.x, sw[2 * h], total[t][h][0]);
+                        total[t][h][1] = fmaf((float)d[h][1] * sx.y, sw[2 * h], total[t][h][1]);
+                        total[t][h][2] = fmaf((float)d[h][2] * sx.x, sw[2 * h + 1], total[t][h][2]);
+                        total[t][h][3] = fmaf((float)d[h][3] * sx.y, sw[2 * h + 1], total[t][h][3]);
+                    }
                 }
             }
             __syncwarp();
@@ -199,7 +204,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sums[(t * 8 + 2 * c + (e & 1)) * FEATURES + row0 + h * 16 + (e >> 1) * 8 + quad] = total[t][h][e];
+                for (int e = 0; e < 4; ++e) sums[(t * 8 + 2 * c + (e & 1)) * FEATURES + row0 + h * 16 + (e >> 1) * 8 + row8] = total[t][h][e];
     }
     const bool failed = __syncthreads_or(!ok);
     if (C > 1) cluster.sync();
@@ -631,11 +636,11 @@ int launch_stream(const W4Params& p, cudaStream_t stream) {
         configured = true;
     }
     CUtensorMap mw, mx;
-    if (!byte_map(&mw, p.packed, p.N, 64ll * p.G, 64, FEATURES) || !byte_map(&mx, p.rows, p.M, 128ll * p.G, 128, NT * 8)) return PYRE_ERR_BAD_ARG;
+    if (!byte_map(&mw, p.packed, p.N, 64ll * p.G, 128, FEATURES) || !byte_map(&mx, p.rows, p.M, 128ll * p.G, 128, NT * 8)) return PYRE_ERR_BAD_ARG;
     const int tiles = ceil_div(p.N, FEATURES), rows = ceil_div(p.M, NT * 8), room = 2 * pyre_sm_count();
     int C = 1;
     while (C < 8 && 2ll * C * tiles * rows <= room && p.G >= 8 * C) C *= 2;
-    const int per = ceil_div(p.G, C);
+    const int per = ceil_div(ceil_div(p.G, C), PAIR) * PAIR;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)rows);
     cfg.blockDim = dim3(STREAM_THREADS);
