@@ -15,7 +15,7 @@ namespace cg = cooperative_groups;
 constexpr int GROUP = 128;
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t lower(uint32_t w) { return (w << 4) & 0xf0f0f0f0u; }
@@ -55,6 +55,7 @@ __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
 // The sets' and the cluster's shares meet in shared memory and are added in order.
 // ---------------------------------------------------------------------------
 constexpr int STREAM_THREADS = 320, STREAM_STAGES = 4, PAIR = 2;
+constexpr int ROW = FEATURES + 4;      // of a token's sums: what a warp stores at once falls on different banks
 
 template <int NT> struct Stream {
     static constexpr int X_BYTES = NT * 8 * GROUP;                                                    // a group's
@@ -62,12 +63,12 @@ template <int NT> struct Stream {
     static constexpr int SCALES = STREAM_STAGES * STAGE, SCALE = (FEATURES + NT * 8) * 4;             // [stage][group][features, tokens] floats
     static constexpr int BARS = SCALES + STREAM_STAGES * PAIR * SCALE;
     static constexpr int TOTAL = BARS + STREAM_STAGES * 16 + 16 + 1024;
-    static_assert(2 * NT * 8 * FEATURES * 4 <= SCALES && 2 * (TOTAL + 1024) <= 233472 && STREAM_STAGES % 2 == 0, "the sets' sums take the ring's place; two CTAs");
+    static_assert(2 * NT * 8 * ROW * 4 <= SCALES && 2 * (TOTAL + 1024) <= 233472 && STREAM_STAGES % 2 == 0, "the sets' sums take the ring's place; two CTAs");
 };
 
 template <int NT, typename T>
 __global__ void __launch_bounds__(STREAM_THREADS, 2)
-w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const W4Params p, int per_cta) {
+w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const W4Params p) {
     using L = Stream<NT>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -78,7 +79,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int f0 = blockIdx.x / C * FEATURES, t0 = blockIdx.y * NT * 8;
-    const int first = rank * per_cta, n = max(0, min(per_cta, p.G - first)), steps = (n + PAIR - 1) / PAIR;      // per_cta is even
+    const int first = (int)((long long)rank * p.G / C), n = (int)((rank + 1ll) * p.G / C) - first, steps = (n + PAIR - 1) / PAIR;      // four groups at least
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -90,6 +91,8 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     bool ok = true;
     if (warp == 8) {
         if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
             const int early = min(steps, STREAM_STAGES);      // the weights depend on no earlier kernel
             int asked = 0;
             auto weights = [&](int i) {
@@ -157,33 +160,34 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             ok = mbar_wait(full + 8 * s, (i / STREAM_STAGES) & 1, abort_flag, p.err_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const uint32_t stage = base + s * L::STAGE;
+            const uint8_t* const stage = gen + s * L::STAGE;
             const int groups = min(PAIR, n - PAIR * i);
             for (int g = 0; g < groups; ++g) {
-                uint32_t a[4][4];      // features row8 + 0, 8, 16, 24
+                // features row8 + 0, 8, 16, 24: the lower and the upper halves of 16 bytes
+                uint32_t lo[4][4], hi[4][4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q)      // 128-byte swizzle: a chunk of 16 bytes by bits 7 to 9
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a[q][0]), "=r"(a[q][1]), "=r"(a[q][2]), "=r"(a[q][3])
-                                 : "r"(stage + (row0 + q * 8 + row8) * 128 + (((4 * g + c) ^ row8) << 4)) : "memory");
+                for (int q = 0; q < 4; ++q) {      // 128-byte swizzle: a chunk of 16 bytes by bits 7 to 9
+                    const uint4 w = *reinterpret_cast<const uint4*>(stage + (row0 + q * 8 + row8) * 128 + (((4 * g + c) ^ row8) << 4));
+                    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { lo[q][j] = lower(word[j]); hi[q][j] = upper(word[j]); }
+                }
                 const float* const scales = reinterpret_cast<const float*>(gen + L::SCALES + (s * PAIR + g) * L::SCALE);
                 float sw[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) sw[q] = scales[row0 + q * 8 + row8];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const uint32_t src = stage + PAIR * W_BYTES + g * L::X_BYTES + (t * 8 + quad) * GROUP;
-                    uint32_t x[8];
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                                 : "r"(src + (((2 * c) ^ quad) << 4)) : "memory");
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
-                                 : "r"(src + (((2 * c + 1) ^ quad) << 4)) : "memory");
+                    const uint8_t* const src = stage + PAIR * W_BYTES + g * L::X_BYTES + (t * 8 + quad) * GROUP;
+                    const uint4 x0 = *reinterpret_cast<const uint4*>(src + (((2 * c) ^ quad) << 4));
+                    const uint4 x1 = *reinterpret_cast<const uint4*>(src + (((2 * c + 1) ^ quad) << 4));
+                    const uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
                     const float2 sx = *reinterpret_cast<const float2*>(scales + FEATURES + t * 8 + 2 * c);
                     int d[2][4] = {};
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            mma_s8(d[h], lower(a[2 * h][j]), lower(a[2 * h + 1][j]), upper(a[2 * h][j]), upper(a[2 * h + 1][j]), x[2 * j], x[2 * j + 1]);
+                        for (int h = 0; h < 2; ++h) mma_s8(d[h], lo[2 * h][j], lo[2 * h + 1][j], hi[2 * h][j], hi[2 * h + 1][j], x[2 * j], x[2 * j + 1]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         total[t][h][0] = fmaf((float)d[h][0] * sx.x, sw[2 * h], total[t][h][0]);
@@ -198,27 +202,39 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
         // [set][token][feature]; the ring is free once both sets are through it
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        float* const sums = reinterpret_cast<float*>(gen) + set * NT * 8 * FEATURES;
+        float* const sums = reinterpret_cast<float*>(gen) + set * NT * 8 * ROW;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sums[(t * 8 + 2 * c + (e & 1)) * FEATURES + row0 + h * 16 + (e >> 1) * 8 + row8] = total[t][h][e];
+                for (int e = 0; e < 4; ++e) sums[(t * 8 + 2 * c + (e & 1)) * ROW + row0 + h * 16 + (e >> 1) * 8 + row8] = total[t][h][e];
     }
     const bool failed = __syncthreads_or(!ok);
     if (C > 1) cluster.sync();
     if (!failed) {
         // (a CTA that gave up raised the error word: what the others write is not looked at)
         const int tokens = min(NT * 8, p.M - t0);
-        for (int i = rank * STREAM_THREADS + threadIdx.x; i < tokens * FEATURES; i += C * STREAM_THREADS) {
-            const int f = f0 + i % FEATURES;
-            float v = 0.f;
+        const bool vec = p.N % 4 == 0 && !((uintptr_t)p.out & (4 * sizeof(T) - 1));
+        for (int i = rank * STREAM_THREADS + threadIdx.x; i < tokens * (FEATURES / 4); i += C * STREAM_THREADS) {
+            const int t = i / (FEATURES / 4), f = i % (FEATURES / 4) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int q = 0; q < C; ++q) {
-                const float* const sums = reinterpret_cast<const float*>(C > 1 ? cluster.map_shared_rank(gen, q) : gen);
-                v += sums[i] + sums[NT * 8 * FEATURES + i];
+                const float* const sums = reinterpret_cast<const float*>(C > 1 ? cluster.map_shared_rank(gen, q) : gen) + t * ROW + f;
+                const float4 a = *reinterpret_cast<const float4*>(sums), b = *reinterpret_cast<const float4*>(sums + NT * 8 * ROW);
+                v.x += a.x + b.x;
+                v.y += a.y + b.y;
+                v.z += a.z + b.z;
+                v.w += a.w + b.w;
             }
-            if (f < p.N) ElemOps<T>::store((T*)p.out + (size_t)(t0 + i / FEATURES) * p.N + f, v);
+            T* const out = (T*)p.out + (size_t)(t0 + t) * p.N + f0 + f;
+            const Vec<T, 4> rounded = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+            if (vec) {
+                if (f0 + f < p.N) store_vec<T, 4>(out, rounded);
+            } else
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (f0 + f + k < p.N) out[k] = rounded.v[k];
         }
     }
     if (C > 1) cluster.sync();      // the others' sums are read
@@ -640,7 +656,6 @@ int launch_stream(const W4Params& p, cudaStream_t stream) {
     const int tiles = ceil_div(p.N, FEATURES), rows = ceil_div(p.M, NT * 8), room = 2 * pyre_sm_count();
     int C = 1;
     while (C < 8 && 2ll * C * tiles * rows <= room && p.G >= 8 * C) C *= 2;
-    const int per = ceil_div(ceil_div(p.G, C), PAIR) * PAIR;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)rows);
     cfg.blockDim = dim3(STREAM_THREADS);
@@ -654,7 +669,7 @@ int launch_stream(const W4Params& p, cudaStream_t stream) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pyre_pdl_enabled() ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_stream_kernel<NT, T>, mw, mx, p, per);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_stream_kernel<NT, T>, mw, mx, p);
     if (e != cudaSuccess) return (int)e;
     PYRE_LAUNCH_CHECK();
     return 0;
