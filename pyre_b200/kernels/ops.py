@@ -141,6 +141,17 @@ class Rows8:
             raise ValueError(f"scales must be float32 {(groups, rows.shape[0])}, got {scales.dtype} {tuple(scales.shape)}")
         self.rows, self.scales, self.width, self.dtype = rows, scales, width, dtype
 
+    @classmethod
+    def empty(cls, n_rows: int, width: int, device, dtype: torch.dtype) -> "Rows8":
+        """Uninitialised rows for a kernel to fill."""
+        out = cls.__new__(cls)
+        groups = -(-width // GROUP8)
+        # (sizes as plain arguments: a tuple costs a microsecond more)
+        out.rows = torch.empty(n_rows, groups * GROUP8, dtype=torch.int8, device=device)
+        out.scales = torch.empty(groups, n_rows, dtype=torch.float32, device=device)
+        out.width, out.dtype = width, dtype
+        return out
+
     @property
     def shape(self):
         return torch.Size((self.rows.shape[0], self.width))
@@ -195,9 +206,9 @@ def materialize(t: "torch.Tensor | PartialSums | DeferredProduct | ScaledRows | 
     norm's output may take."""
     if isinstance(t, Rows8):
         _check_rows8(t)
-        T, K = t.shape
-        out = torch.empty((T, K), dtype=t.dtype, device=t.rows.device)
-        lib.call("pyre_rows8_values", t.rows.data_ptr(), t.scales.data_ptr(), t.scales.stride(0), out.data_ptr(), T, K, _dt(t.dtype), _stream())
+        rows, T, K = t.rows, t.rows.shape[0], t.width
+        out = torch.empty(T, K, dtype=t.dtype, device=rows.device)
+        lib.call("pyre_rows8_values", rows.data_ptr(), t.scales.data_ptr(), t.scales.stride(0), out.data_ptr(), T, K, _dt(t.dtype), _stream())
         return out
     if isinstance(t, NormedBranch):
         t = t.formed()
@@ -254,6 +265,9 @@ def _ptr(t: "torch.Tensor | None") -> "int | None":
 
 
 def _check(t: torch.Tensor, name: str, dtype=None, dim: "int | None" = None) -> None:
+    if t.is_cuda and (dtype is None or t.dtype is dtype) and (dim is None or t.dim() == dim) and t.is_contiguous() \
+            and t.device.index == _current_device():
+        return
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (pyre_b200 has no CPU path)")
     require_current_device(t.device, name)
@@ -372,17 +386,13 @@ def add_rmsnorm(x: torch.Tensor, delta: "torch.Tensor | None", weight: torch.Ten
 
 
 def _check_rows8(x: Rows8) -> None:
-    if not x.rows.is_cuda or not x.scales.is_cuda or x.scales.device != x.rows.device:
+    rows, scales = x.rows, x.scales
+    if not rows.is_cuda or scales.device != rows.device:
         raise ValueError("rows in 8 bits and their scales must lie on one CUDA device (pyre_b200 has no CPU path)")
-    require_current_device(x.rows.device, "x")
-    if not x.rows.is_contiguous() or x.rows.data_ptr() % 16 or (x.scales.shape[1] > 1 and x.scales.stride(1) != 1):
+    if rows.get_device() != _current_device():
+        require_current_device(rows.device, "x")
+    if not rows.is_contiguous() or rows.data_ptr() % 16 or (scales.shape[1] > 1 and scales.stride(1) != 1):
         raise ValueError("rows in 8 bits must be contiguous and start on a 16-byte boundary, their scales contiguous along the tokens")
-
-
-def _rows8_out(T: int, width: int, device, dtype: torch.dtype) -> Rows8:
-    groups = -(-width // GROUP8)
-    return Rows8(torch.empty((T, groups * GROUP8), dtype=torch.int8, device=device), torch.empty((groups, T), dtype=torch.float32, device=device),
-                 width, dtype)
 
 
 def add_rmsnorm_rows8(x: torch.Tensor, delta: "torch.Tensor | PartialSums | DeferredProduct | None", weight: torch.Tensor, eps: float,
@@ -391,27 +401,28 @@ def add_rmsnorm_rows8(x: torch.Tensor, delta: "torch.Tensor | PartialSums | Defe
     fp32 residual stream and takes the sum as there; ``delta`` has the activation dtype ``dtype`` or is a lazy form of a branch output.
     Each 128 neighbouring elements of a row share the scale max |.| / 127, so the values are off by at most half of it: the norm is
     not rounded to ``dtype`` in between."""
-    delta = formed(delta)
     _check(x, "x", torch.float32, 2)
     _check(weight, "weight", torch.float32, 1)
     T, H = x.shape
     if weight.shape[0] != H:
         raise ValueError(f"norm weight has {weight.shape[0]} entries, rows have {H}")
-    if delta is not None and tuple(delta.shape) != (T, H):
+    if not isinstance(delta, torch.Tensor):
+        delta = formed(delta)
+    if delta is not None and delta.shape != (T, H):
         raise ValueError(f"delta shape {tuple(delta.shape)} != x shape {(T, H)}")
-    if isinstance(delta, DeferredProduct):
-        delta = delta.partials()
     parts, n_parts = None, 0
-    if isinstance(delta, PartialSums):
-        parts, n_parts, delta = delta.parts, delta.n, None
-    elif delta is not None:
+    if isinstance(delta, torch.Tensor):
         _check(delta, "delta", dtype, 2)
+    elif delta is not None:
+        if isinstance(delta, DeferredProduct):
+            delta = delta.partials()
+        parts, n_parts, delta = (delta.parts, delta.n, None) if isinstance(delta, PartialSums) else (None, 0, delta)
     n_rows = T
     if rows is not None:
         _check(rows, "rows", torch.int32, 1)
         n_rows = rows.shape[0]
         update_x = False
-    out = _rows8_out(n_rows, H, x.device, dtype)
+    out = Rows8.empty(n_rows, H, x.device, dtype)
     lib.call("pyre_norm_rows8", x.data_ptr(), _ptr(delta), _ptr(parts), n_parts, T * H, weight.data_ptr(), out.rows.data_ptr(), out.scales.data_ptr(),
              _ptr(rows), n_rows, H, float(eps), int(bool(update_x and (delta is not None or parts is not None))), _dt(dtype), _stream())
     return out
@@ -423,7 +434,7 @@ def quantize_rows8(x: torch.Tensor) -> Rows8:
         raise ValueError("x must be a CUDA matrix with contiguous rows")
     require_current_device(x.device, "x")
     T, K = x.shape
-    out = _rows8_out(T, K, x.device, x.dtype)
+    out = Rows8.empty(T, K, x.device, x.dtype)
     lib.call("pyre_rows8", x.data_ptr(), x.stride(0), out.rows.data_ptr(), out.scales.data_ptr(), T, K, 0, 0, 0.0, _dt(x.dtype), _stream())
     return out
 
@@ -436,7 +447,7 @@ def gate_rows8(gate_up: torch.Tensor, kind: str = "silu", limit: float = 0.0) ->
         raise ValueError("gate_up must have an even number of columns")
     if kind not in GATE_KINDS:
         raise UnsupportedSize(f"gate activation {kind!r}: this kernel knows {sorted(GATE_KINDS)}")
-    out = _rows8_out(T, two_i // 2, gate_up.device, gate_up.dtype)
+    out = Rows8.empty(T, two_i // 2, gate_up.device, gate_up.dtype)
     lib.call("pyre_rows8", gate_up.data_ptr(), two_i, out.rows.data_ptr(), out.scales.data_ptr(), T, two_i // 2, 1, {"silu": 0, "relu": 1, "clamped": 2}[kind],
              float(limit), _dt(gate_up.dtype), _stream())
     return out
@@ -463,22 +474,33 @@ def linear4(x: "torch.Tensor | Rows8", w: Weight4, out_dtype: "torch.dtype | Non
     if not isinstance(x, Rows8):
         x = quantize_rows8(materialize(x))
     _check_rows8(x)
-    T, K = x.shape
-    N, K2 = w.shape
-    if K != K2:
-        raise ValueError(f"inner sizes differ: x is [{T}, {K}], w is [{N}, {K2}]")
-    require_current_device(w.packed.device, "w")
-    dtype = out_dtype or x.dtype
-    groups = w.scales.shape[0]
-    splits = lib.call_value("pyre_w4_splits", T, N, groups)
+    rows, scales, packed = x.rows, x.scales, w.packed
+    T, K, N = rows.shape[0], x.width, packed.shape[0]
+    if K != w.width:
+        raise ValueError(f"inner sizes differ: x is [{T}, {K}], w is [{N}, {w.width}]")
+    if packed.device != rows.device:
+        require_current_device(packed.device, "w")
+    dtype, groups = out_dtype or x.dtype, scales.shape[0]
+    splits = _w4_splits(T, N, groups, rows.get_device()) if T > W4_STREAM_ROWS else 1
     shares = partials_ok or splits > 1
-    out = torch.empty((splits, T, N) if shares else (T, N), dtype=torch.float32 if shares else dtype, device=x.rows.device)
-    lib.call("pyre_w4_linear", x.rows.data_ptr(), x.scales.data_ptr(), x.scales.stride(0), w.packed.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
-             T, N, groups, splits, _dt(out.dtype), device_error_flag(x.rows.device).data_ptr(), _stream())
+    if shares:
+        out = torch.empty(splits, T, N, dtype=torch.float32, device=rows.device)
+    else:
+        out = torch.empty(T, N, dtype=dtype, device=rows.device)
+    lib.call("pyre_w4_linear", rows.data_ptr(), scales.data_ptr(), scales.stride(0), packed.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
+             T, N, groups, splits, _dt(out.dtype), device_error_flag(rows.device).data_ptr(), _stream())
     if not shares:
         return out
     out = PartialSums(out, dtype)
     return out if partials_ok else materialize(out)
+
+
+W4_STREAM_ROWS = 32      # up to here ``pyre_w4_linear`` shares K within clusters (csrc/gemm_w4.cu: FEW)
+
+
+@functools.lru_cache(maxsize=4096)
+def _w4_splits(T: int, N: int, groups: int, device: int) -> int:
+    return lib.call_value("pyre_w4_splits", T, N, groups)
 
 
 def add_residual(x: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:
@@ -622,11 +644,12 @@ def sample(logits: torch.Tensor, temperature: "torch.Tensor | None" = None, seed
         if not (temperature.shape[0] == seeds.shape[0] == token_index.shape[0] == R):
             raise ValueError("temperature, seeds and token_index need one entry per row")
     if out is None:
-        out = torch.empty((R,), dtype=torch.int32, device=logits.device)
+        out = torch.empty(R, dtype=torch.int32, device=logits.device)
     if top_k is not None or top_p is not None or min_p is not None:
-        require_current_device(logits.device, "logits")
         if temperature is None:
             raise ValueError("top_k, top_p and min_p go with a temperature (0 for rows that take the best token)")
+        if logits.get_device() != _current_device():
+            require_current_device(logits.device, "logits")
         for t, name, dtype in ((top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32), (out, "out", torch.int32)):
             if t is not None:
                 _check(t, name, dtype, 1)
