@@ -281,7 +281,13 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint32_t tmem_a, uint64
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr));
+}
+// The loads before have arrived.  It takes their registers, so that nothing is done with them ahead of it (and what is not from tensor memory may be).
+__device__ __forceinline__ void tmem_wait16(int* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
@@ -529,16 +535,24 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     int v[COLS];
 #pragma unroll
                     for (int c = 0; c < COLS; c += 16) tmem_ld16(tmem + lanes + d * TN + col0 + c, v + c);
-                    const uint64_t scale = pack2(*sw, *sw);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    const float ws = *sw;
+                    const uint64_t scale = pack2(ws, ws);
+                    uint64_t x[COLS / 2];
+#pragma unroll
+                    for (int q = 0; q < COLS; q += 4) {
+                        const ulonglong2 x4 = *reinterpret_cast<const ulonglong2*>(sx + q);
+                        x[q / 2] = x4.x;
+                        x[q / 2 + 1] = x4.y;
+                    }
+#pragma unroll
+                    for (int c = 0; c < COLS; c += 16) tmem_wait16(v + c);
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(acc_empty + 8 * d);
 #pragma unroll
                     for (int q = 0; q < COLS; q += 4) {
-                        const ulonglong2 x4 = *reinterpret_cast<const ulonglong2*>(sx + q);
-                        sum[q / 2] = fma2(mul2(pack2((float)v[q], (float)v[q + 1]), x4.x), scale, sum[q / 2]);
-                        sum[q / 2 + 1] = fma2(mul2(pack2((float)v[q + 2], (float)v[q + 3]), x4.y), scale, sum[q / 2 + 1]);
+                        sum[q / 2] = fma2(mul2(pack2((float)v[q], (float)v[q + 1]), x[q / 2]), scale, sum[q / 2]);
+                        sum[q / 2 + 1] = fma2(mul2(pack2((float)v[q + 2], (float)v[q + 3]), x[q / 2 + 1]), scale, sum[q / 2 + 1]);
                     }
                 }
                 __syncwarp();
