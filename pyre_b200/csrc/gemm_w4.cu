@@ -247,11 +247,11 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 //                        is where the MMAs take their A operand from.
 //   warp 1, one thread : four MMAs (kind::i8, 32 k each) a group, into one of two accumulators of 32-bit integers.
 //   warps 2, 3         : the scales of four groups at a time, of features and of tokens, to shared memory.
-//   warps 8..23        : a thread owns a feature and a quarter of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
+//   warps 8..15        : a thread owns a feature and half of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
 //                        feature and added to float sums in registers, by ascending group.
 // An output tile whose K is shared among CTAs (few tiles) leaves float shares, added up in order by whoever reads them.
 // ---------------------------------------------------------------------------
-constexpr int MANY_THREADS = 768, EPI_WARP0 = 8, EPI_WARPS = 16, A_COLS = 32;
+constexpr int MANY_THREADS = 512, EPI_WARP0 = 8, EPI_WARPS = 8, A_COLS = 32;
 constexpr int W_STAGES = 6, STAGES = 6;               // packed weights; both operands of the MMAs
 constexpr int BATCH = 4, S_STAGES = 2;                // groups whose scales come at a time
 
@@ -508,8 +508,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         }
         if (!waited) pdl_wait();
     } else {
-        constexpr int COLS = TN / 4;
-        static_assert(EPI_WARPS == 16 && COLS % 16 == 0, "four warps side by side, whole loads from tensor memory");
+        constexpr int COLS = TN / 2;
+        static_assert(EPI_WARPS == 8 && COLS % 16 == 0, "two warps side by side, whole loads from tensor memory");
         const int quarter = warp & 3, row = quarter * 32 + lane, col0 = ((warp - EPI_WARP0) >> 2) * COLS;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         pdl_wait();
@@ -532,27 +532,28 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    int v[COLS];
-#pragma unroll
-                    for (int c = 0; c < COLS; c += 16) tmem_ld16(tmem + lanes + d * TN + col0 + c, v + c);
+                    const uint32_t from = tmem + lanes + d * TN + col0;
+                    int v[2][16];
+                    tmem_ld16(from, v[0]);
                     const float ws = *sw;
                     const uint64_t scale = pack2(ws, ws);
-                    uint64_t x[COLS / 2];
 #pragma unroll
-                    for (int q = 0; q < COLS; q += 4) {
-                        const ulonglong2 x4 = *reinterpret_cast<const ulonglong2*>(sx + q);
-                        x[q / 2] = x4.x;
-                        x[q / 2 + 1] = x4.y;
-                    }
+                    for (int c = 0; c < COLS; c += 16) {
+                        int* const now = v[(c / 16) & 1];
+                        tmem_wait16(now);
+                        if (c + 16 < COLS) tmem_ld16(from + c + 16, v[(c / 16 + 1) & 1]);      // on its way while this one is worked on
+                        else {
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(acc_empty + 8 * d);
+                        }
 #pragma unroll
-                    for (int c = 0; c < COLS; c += 16) tmem_wait16(v + c);
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty + 8 * d);
-#pragma unroll
-                    for (int q = 0; q < COLS; q += 4) {
-                        sum[q / 2] = fma2(mul2(pack2((float)v[q], (float)v[q + 1]), x[q / 2]), scale, sum[q / 2]);
-                        sum[q / 2 + 1] = fma2(mul2(pack2((float)v[q + 2], (float)v[q + 3]), x[q / 2 + 1]), scale, sum[q / 2 + 1]);
+                        for (int q = 0; q < 16; q += 4) {
+                            const ulonglong2 x4 = *reinterpret_cast<const ulonglong2*>(sx + c + q);
+                            uint64_t &s0 = sum[(c + q) / 2], &s1 = sum[(c + q) / 2 + 1];
+                            s0 = fma2(mul2(pack2((float)now[q], (float)now[q + 1]), x4.x), scale, s0);
+                            s1 = fma2(mul2(pack2((float)now[q + 2], (float)now[q + 3]), x4.y), scale, s1);
+                        }
                     }
                 }
                 __syncwarp();
