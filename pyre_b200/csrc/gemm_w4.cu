@@ -7,7 +7,6 @@
 // makes it sixteen times as large and spares the sign's extension), the outer ones in float, by ascending group in each of a CTA's warps,
 // then over the warps in order.
 #include <cooperative_groups.h>
-#include <cuda_fp16.h>
 
 #include "tensor_core.cuh"
 
@@ -243,11 +242,11 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 
 // ---------------------------------------------------------------------------
 // Many rows, on the 5th-generation tensor cores.  A CTA owns 128 features (the MMA's rows) and TN tokens and takes a group of 128 k at a time:
-//   warp 0, one thread : TMA.  The group's weights as they are packed (128 x 64 bytes) into one ring, the tokens' bytes (TN x 128) into another.
+//   warps 0, 3, a thread each : TMA.  The tokens' bytes of a group (TN x 128) into one ring, its weights as they are packed (128 x 64) into another.
 //   warps 4..7         : a thread owns a feature: 64 bytes of a group to 128 (two masks and a shift per eight), stored to tensor memory, which
 //                        is where the MMAs take their A operand from.
 //   warp 1, one thread : four MMAs (kind::i8, 32 k each) a group, into one of two accumulators of 32-bit integers.
-//   warps 2, 3         : the scales of four groups at a time, of features and of tokens, to shared memory.
+//   warp 2             : the scales of four groups at a time, of features and of tokens, to shared memory.
 //   warps 8..15        : a thread owns a feature and half of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
 //                        feature and added to float sums in registers, by ascending group.
 // An output tile whose K is shared among CTAs (few tiles) leaves float shares, added up in order by whoever reads them.
@@ -385,7 +384,7 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         *abort_flag = 0;
         for (int s = 0; s < W_STAGES; ++s) { mbar_init(w_full + 8 * s, 1); mbar_init(w_empty + 8 * s, 4); }
         for (int s = 0; s < STAGES; ++s) { mbar_init(ab_full + 8 * s, 5); mbar_init(ab_empty + 8 * s, 1); }
-        for (int s = 0; s < S_STAGES; ++s) { mbar_init(s_full + 8 * s, 2); mbar_init(s_empty + 8 * s, EPI_WARPS); }
+        for (int s = 0; s < S_STAGES; ++s) { mbar_init(s_full + 8 * s, 1); mbar_init(s_empty + 8 * s, EPI_WARPS); }
         for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, EPI_WARPS); }
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -411,45 +410,30 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     };
 
     int f0, t0, split, first, n;
-    if (warp == 0) {
+    if (warp == 0 || warp == 3) {
         if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
+            // the weights have a thread of their own: they are converted, so they are wanted well before the rows are
+            const bool rows = warp == 0;
+            const CUtensorMap* const map = rows ? &map_x : &map_w;
+            const uint32_t full = rows ? ab_full : w_full, empty = rows ? ab_empty : w_empty, stages = rows ? STAGES : W_STAGES;
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
             bool waited = false, ok = true;
-            int it = 0, w_asked = 0, x_asked = 0;
+            uint32_t it = 0;
             for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
                 range(item, f0, t0, split, first, n);
-                auto weights = [&](int i) {
-                    const int at = it + i, s = at % W_STAGES;
-                    if (!mbar_wait(w_empty + 8 * s, ((at / W_STAGES) & 1) ^ 1, abort_flag, p.err_flag)) return false;
-                    mbar_expect_tx(w_full + 8 * s, W_BYTES);
-                    tma_load_2d(base + L::W_OFF + s * W_BYTES, &map_w, w_full + 8 * s, (first + i) * (GROUP / 2), f0);
-                    w_asked = at + 1;
-                    return true;
-                };
-                int done = 0;
-                if (!waited) {
-                    // the weights depend on no earlier kernel
-                    done = min(n, W_STAGES);
-                    for (int i = 0; i < done; ++i) weights(i);
-                    pdl_wait();
-                    waited = true;
+                for (int i = 0; i < n; ++i) {
+                    if (!waited && (rows || it == W_STAGES)) { pdl_wait(); waited = true; }      // (the weights depend on no earlier kernel)
+                    const uint32_t s = it % stages;
+                    if (!(ok = mbar_wait(empty + 8 * s, ((it / stages) & 1) ^ 1, abort_flag, p.err_flag))) break;
+                    mbar_expect_tx(full + 8 * s, rows ? L::X_BYTES : W_BYTES);
+                    if (rows) tma_load_2d(base + L::X_OFF + s * L::X_BYTES, map, full + 8 * s, (first + i) * GROUP, t0);
+                    else tma_load_2d(base + L::W_OFF + s * W_BYTES, map, full + 8 * s, (first + i) * (GROUP / 2), f0);
+                    ++it;
                 }
-                for (int i = 0; i < n && ok; ++i) {
-                    const int at = it + i, s = at % STAGES;
-                    if (i >= done && !(ok = weights(i))) break;
-                    if (!(ok = mbar_wait(ab_empty + 8 * s, ((at / STAGES) & 1) ^ 1, abort_flag, p.err_flag))) break;
-                    mbar_expect_tx(ab_full + 8 * s, L::X_BYTES);
-                    tma_load_2d(base + L::X_OFF + s * L::X_BYTES, &map_x, ab_full + 8 * s, (first + i) * GROUP, t0);
-                    x_asked = at + 1;
-                }
-                it += n;
             }
             if (!waited) pdl_wait();
-            if (!ok) {      // a wait ran out: the copies in flight end first
-                for (int at = max(0, w_asked - W_STAGES); at < w_asked; ++at) mbar_drain(w_full + 8 * (at % W_STAGES), (at / W_STAGES) & 1);
-                for (int at = max(0, x_asked - STAGES); at < x_asked; ++at) mbar_drain(ab_full + 8 * (at % STAGES), (at / STAGES) & 1);
-            }
+            if (!ok)      // a wait ran out: the copies in flight end first
+                for (uint32_t at = it > stages ? it - stages : 0; at < it; ++at) mbar_drain(full + 8 * (at % stages), (at / stages) & 1);
         }
     } else if (warp == 1) {
         // D 32-bit integers (2 at bit 4), A and B signed bytes (1 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24
@@ -485,8 +469,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             mbar_drain(drained, 0);
         }
         __syncwarp();
-    } else if (warp < 4) {
-        // warp 2: the tokens' scales, warp 3: the features' (a sixteenth of them: the integers are sixteen times as large)
+    } else if (warp == 2) {
+        // the scales of the tokens, and of the features (a sixteenth of them: the integers are sixteen times as large)
         bool ok = true;
         int bt = 0;
         pdl_wait();
@@ -494,25 +478,27 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             range(item, f0, t0, split, first, n);
             for (int i0 = 0; i0 < n && ok; i0 += BATCH, ++bt) {
                 const int s = bt % S_STAGES;
-                constexpr int PER_LANE = FEATURES / 32;
-                float v[BATCH][PER_LANE];
+                constexpr int F = FEATURES / 32, X = TN / 32;
+                float x[BATCH][X], w[BATCH][F];
 #pragma unroll
                 for (int j = 0; j < BATCH; ++j) {
                     const size_t g = first + min(i0 + j, n - 1);
 #pragma unroll
-                    for (int q = 0; q < PER_LANE; ++q) {
-                        if (warp == 2) v[j][q] = q * 32 < TN ? p.row_scales[g * p.ld_scales + min(t0 + q * 32 + lane, p.M - 1)] : 0.f;
-                        else v[j][q] = __bfloat162float(p.scales[g * p.N + min(f0 + q * 32 + lane, p.N - 1)]) * 0.0625f;
-                    }
+                    for (int q = 0; q < X; ++q) x[j][q] = p.row_scales[g * p.ld_scales + min(t0 + q * 32 + lane, p.M - 1)];
+#pragma unroll
+                    for (int q = 0; q < F; ++q) w[j][q] = __bfloat162float(p.scales[g * p.N + min(f0 + q * 32 + lane, p.N - 1)]) * 0.0625f;
                 }
                 ok = mbar_wait(s_empty + 8 * s, ((bt / S_STAGES) & 1) ^ 1, abort_flag, p.err_flag);
                 ok = __all_sync(0xffffffffu, ok);
-                float* const to = reinterpret_cast<float*>(gen + (warp == 2 ? L::SX_OFF + s * BATCH * TN * 4 : L::SW_OFF + s * BATCH * FEATURES * 4));
+                float* const sx = reinterpret_cast<float*>(gen + L::SX_OFF) + s * BATCH * TN + lane;
+                float* const sw = reinterpret_cast<float*>(gen + L::SW_OFF) + s * BATCH * FEATURES + lane;
 #pragma unroll
-                for (int j = 0; j < BATCH; ++j)
+                for (int j = 0; j < BATCH; ++j) {
 #pragma unroll
-                    for (int q = 0; q < PER_LANE; ++q)
-                        if (warp == 3 || q * 32 < TN) to[j * (warp == 2 ? TN : FEATURES) + q * 32 + lane] = v[j][q];
+                    for (int q = 0; q < X; ++q) sx[j * TN + q * 32] = x[j][q];
+#pragma unroll
+                    for (int q = 0; q < F; ++q) sw[j * FEATURES + q * 32] = w[j][q];
+                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_full + 8 * s);
             }
@@ -614,322 +600,6 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     }
 }
 
-// ---------------------------------------------------------------------------
-// Very many rows with a bfloat16 result.  Above, each group costs a conversion, a product and a multiplication with addition per output, and its hand-over
-// from the tensor cores to the sums: they are used for a fifth of the time.  Here the scales are in the operands, as half floats, and the sums stay in
-// tensor memory for all of K:
-//   a weight times its scale is a whole number of at most 8 times eight bits, which a half float holds exactly;
-//   an element of a row times its scale is rounded to eleven bits, an eighth of the result's rounding (2-norm: 1.4e-4 against 1.1e-3 for bfloat16).
-// Scales of a feature in a tile, and of a token, are put on a power of two of their own (the largest in [2^11, 2^12) and [2^3, 2^4)); others lose more bits (as
-// subnormals) only below 2^-24 of it.  The powers come back at the end.
-//   in front           : `w4_half_rows_kernel`, the rows as half floats and their powers.
-//   warps 0, 2, a thread each : TMA, of the rows (two copies of 64 k a group), of the weights.
-//   warp 3             : the features' powers of two of the tile to come, then their scales, four groups at a time.
-//   warps 4..19        : four sets of four take the groups in turn; a thread owns a feature: 64 bytes of a group to 256: a byte under the half float 1024's
-//                        upper byte is 1024 and its lower or 16 times its upper half, from which the constant and the bias are taken off, and
-//                        which the scale multiplies; all exactly.
-//   warp 1, one thread : eight MMAs (kind::f16, 16 k each) a group, into one of two accumulators, a tile each.
-//   warps 20..27       : a thread owns a feature and half of the tokens: the accumulator of a tile while the next one fills.
-// ---------------------------------------------------------------------------
-constexpr int HALF_THREADS = 896, HALF_SETS = 4, HALF_EPI0 = 4 + 4 * HALF_SETS, HALF_EPI = 8, HALF_W_STAGES = 8, HALF_STAGES = 4, HALF_A_COLS = 64, HALF_TN = 128;
-constexpr int HALF_X_BYTES = HALF_TN * GROUP * 2;
-constexpr int HALF_ROWS = 256, HALF_GROUPS = 16;      // from so many rows and groups on
-
-// D (tensor memory, floats) += A (tensor memory, half floats) * B (shared memory, half floats)
-__device__ __forceinline__ void umma_half(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
-__device__ __forceinline__ __half2 bits_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
-// Eight packed elements times m (m16: a sixteenth of it) -> four pairs of half floats.
-__device__ __forceinline__ void halves_of(uint32_t w, __half2 m, __half2 m16, uint32_t* out) {
-    const __half2 low_bias = bits_half2(0x64086408u), high_bias = bits_half2(0x64806480u);      // 1032 = 1024 + 8, 1152 = 1024 + 16 * 8
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t b = __byte_perm(w, 0x64646464u, h ? 0x4342 : 0x4140);      // two bytes, each under 0x64
-        out[h] = half2_bits(__hmul2(__hsub2(bits_half2((b & 0xff0fff0fu) ^ 0x00080008u), low_bias), m));
-        out[2 + h] = half2_bits(__hmul2(__hsub2(bits_half2((b & 0xfff0fff0u) ^ 0x00800080u), high_bias), m16));
-    }
-}
-// The exponent e with which v 2^-e lies in [2^above, 2^(above + 1)), within what floats hold (0 has one too; bits of a float, its sign taken off).
-__device__ __forceinline__ int power_of(uint32_t bits, int above) { return max(-110, min(254, (int)(bits >> 23)) - above - 127); }
-
-struct Half {
-    static constexpr int W_OFF = 0, X_OFF = HALF_W_STAGES * W_BYTES, SW_OFF = X_OFF + HALF_STAGES * HALF_X_BYTES;      // [stage][group][feature] half floats
-    static constexpr int POW_OFF = SW_OFF + S_STAGES * BATCH * FEATURES * 2;        // [tile's parity][feature] floats
-    static constexpr int OUT_OFF = POW_OFF + 2 * FEATURES * 4;                      // [warp][16 tokens][32 features] floats
-    static constexpr int BARS = OUT_OFF + HALF_EPI * 512 * 4;
-    static constexpr int N_BARS = 2 * (HALF_W_STAGES + HALF_STAGES + S_STAGES + 2) + 1;
-    static constexpr int TOTAL = BARS + N_BARS * 8 + 24 + 1024;
-    static constexpr int A_COL0 = 2 * HALF_TN;
-    static_assert(A_COL0 + HALF_STAGES * HALF_A_COLS <= 512 && TOTAL <= 232448 && OUT_OFF % 16 == 0, "fits");
-    // A wait by parity cannot tell a phase from the one two before it: with as many stages as sets, or a multiple, a stage is always the same set's.
-    static_assert(HALF_W_STAGES % HALF_SETS == 0 && HALF_STAGES % HALF_SETS == 0, "see above");
-    // Warp 3 is at most two batches and the rings' stages ahead of the MMAs, those at most a tile ahead of the epilogue (two accumulators): two places for
-    // the powers do if it waits for the tile before the last one (acc_empty).
-};
-
-__global__ void __launch_bounds__(HALF_THREADS, 1)
-w4_half_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ ManyParams p, const float* token_powers) {
-    using L = Half;
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t w_full = base + L::BARS, w_empty = w_full + 8 * HALF_W_STAGES;
-    const uint32_t ab_full = w_empty + 8 * HALF_W_STAGES, ab_empty = ab_full + 8 * HALF_STAGES;
-    const uint32_t sw_full = ab_empty + 8 * HALF_STAGES, sw_empty = sw_full + 8 * S_STAGES;
-    const uint32_t acc_full = sw_empty + 8 * S_STAGES, acc_empty = acc_full + 16, drained = acc_empty + 16;
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::BARS + L::N_BARS * 8);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::BARS + L::N_BARS * 8 + 8);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-    if (threadIdx.x == 0) {
-        *abort_flag = 0;
-        for (int s = 0; s < HALF_W_STAGES; ++s) { mbar_init(w_full + 8 * s, 1); mbar_init(w_empty + 8 * s, 4); }
-        for (int s = 0; s < HALF_STAGES; ++s) { mbar_init(ab_full + 8 * s, 5); mbar_init(ab_empty + 8 * s, 1); }
-        for (int s = 0; s < S_STAGES; ++s) { mbar_init(sw_full + 8 * s, 1); mbar_init(sw_empty + 8 * s, 4 * HALF_SETS); }
-        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, HALF_EPI); }
-        mbar_init(drained, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 1) {
-        __syncwarp();
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *tmem_slot;
-    pdl_trigger();
-
-    if (warp == 0 || warp == 2) {
-        if (lane == 0) {
-            // the weights have a thread of their own: they are converted, so they are wanted well before the rows are
-            const bool rows = warp == 0;
-            const CUtensorMap* const map = rows ? &map_x : &map_w;
-            const uint32_t full = rows ? ab_full : w_full, empty = rows ? ab_empty : w_empty, stages = rows ? HALF_STAGES : HALF_W_STAGES;
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-            bool waited = false, ok = true;
-            uint32_t it = 0;
-            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
-                const int f0 = tile / p.tiles_m * FEATURES, t0 = tile % p.tiles_m * HALF_TN;
-                for (int i = 0; i < p.G && ok; ++i) {
-                    if (!waited && (rows || it == HALF_W_STAGES)) { pdl_wait(); waited = true; }      // (the weights depend on no earlier kernel)
-                    const uint32_t s = it % stages;
-                    if (!(ok = mbar_wait(empty + 8 * s, ((it / stages) & 1) ^ 1, abort_flag, p.err_flag))) break;
-                    if (rows) {
-                        mbar_expect_tx(full + 8 * s, HALF_X_BYTES);
-                        for (int h = 0; h < 2; ++h)
-                            tma_load_2d(base + L::X_OFF + s * HALF_X_BYTES + h * (HALF_X_BYTES / 2), map, full + 8 * s, i * GROUP + h * 64, t0);
-                    } else {
-                        mbar_expect_tx(full + 8 * s, W_BYTES);
-                        tma_load_2d(base + L::W_OFF + s * W_BYTES, map, full + 8 * s, i * (GROUP / 2), f0);
-                    }
-                    ++it;
-                }
-            }
-            if (!waited) pdl_wait();
-            if (!ok)      // a wait ran out: the copies in flight end first
-                for (uint32_t at = it > stages ? it - stages : 0; at < it; ++at) mbar_drain(full + 8 * (at % stages), (at / stages) & 1);
-        }
-    } else if (warp == 1) {
-        // D floats (1 at bit 4), A and B half floats (0 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24
-        constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(HALF_TN >> 3) << 17) | ((uint32_t)(FEATURES >> 4) << 24);
-        const uint64_t db0 = umma_desc(base + L::X_OFF);
-        const bool elected = elect_one();      // the whole warp goes through the loop, so that the operands stay in uniform registers
-        int it = 0, j = 0;
-        bool ok = true;
-        pdl_wait();      // no bounded wait should have to last as long as the kernels before
-        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++j) {
-            const int d = j & 1;
-            ok = mbar_wait(acc_empty + 8 * d, ((j >> 1) & 1) ^ 1, abort_flag, p.err_flag);
-            for (int i = 0; i < p.G; ++i, ++it) {
-                const int s = it % HALF_STAGES;
-                ok = mbar_wait(ab_full + 8 * s, (it / HALF_STAGES) & 1, abort_flag, p.err_flag) && ok;
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t db = db0 + s * (HALF_X_BYTES >> 4);
-                const uint32_t a = tmem + L::A_COL0 + s * HALF_A_COLS;
-                if (elected) {
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)      // 32 bytes of k further; the second copy after four
-                        umma_half(tmem + d * HALF_TN, a + 8 * q, db + 2 * (q & 3) + (q >> 2) * (HALF_X_BYTES >> 5), idesc, i > 0 || q > 0);
-                    umma_commit(ab_empty + 8 * s);
-                    if (i == p.G - 1) umma_commit(acc_full + 8 * d);
-                }
-                __syncwarp();
-            }
-        }
-        if (elected) {
-            umma_commit(drained);      // the MMAs end before tensor memory is given back, also where a wait ran out
-            mbar_drain(drained, 0);
-        }
-        __syncwarp();
-    } else if (warp == 3) {
-        bool ok = true;
-        int bt = 0, j = 0;
-        constexpr int PER_LANE = FEATURES / 32;
-        pdl_wait();      // no bounded wait should have to last as long as the kernels before
-        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++j) {
-            const int f0 = tile / p.tiles_m * FEATURES;
-            const __nv_bfloat16* sw[PER_LANE];
-#pragma unroll
-            for (int q = 0; q < PER_LANE; ++q) sw[q] = p.scales + min(f0 + q * 32 + lane, p.N - 1);
-            uint32_t most[PER_LANE] = {};      // as bits: what is no number above all numbers
-#pragma unroll 4
-            for (int i = 0; i < p.G; ++i)
-#pragma unroll
-                for (int q = 0; q < PER_LANE; ++q) most[q] = max(most[q], (uint32_t)__bfloat16_as_ushort(sw[q][(size_t)i * p.N]) & 0x7fffu);
-            // the epilogue of the tile before the last one has read its powers
-            ok = mbar_wait(acc_empty + 8 * (j & 1), ((j >> 1) & 1) ^ 1, abort_flag, p.err_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            float down[PER_LANE];
-#pragma unroll
-            for (int q = 0; q < PER_LANE; ++q) {
-                const int e = power_of(most[q] << 16, 11);
-                down[q] = exp2f((float)-e);
-                reinterpret_cast<float*>(gen + L::POW_OFF)[(j & 1) * FEATURES + q * 32 + lane] = exp2f((float)e);
-            }
-            for (int i0 = 0; i0 < p.G && ok; i0 += BATCH, ++bt) {
-                const int s = bt % S_STAGES;
-                float v[BATCH][PER_LANE];
-#pragma unroll
-                for (int b = 0; b < BATCH; ++b)
-#pragma unroll
-                    for (int q = 0; q < PER_LANE; ++q) v[b][q] = __bfloat162float(sw[q][(size_t)min(i0 + b, p.G - 1) * p.N]) * down[q];
-                ok = mbar_wait(sw_empty + 8 * s, ((bt / S_STAGES) & 1) ^ 1, abort_flag, p.err_flag);
-                ok = __all_sync(0xffffffffu, ok);
-#pragma unroll
-                for (int b = 0; b < BATCH; ++b)
-#pragma unroll
-                    for (int q = 0; q < PER_LANE; ++q)
-                        reinterpret_cast<__half*>(gen + L::SW_OFF)[(s * BATCH + b) * FEATURES + q * 32 + lane] = __float2half_rn(v[b][q]);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sw_full + 8 * s);
-            }
-        }
-    } else if (warp >= 4 && warp < HALF_EPI0) {
-        const int quarter = warp & 3, row = quarter * 32 + lane, set = (warp >> 2) - 1;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        bool ok = true;
-        int it = 0, bt = 0;
-        pdl_wait();      // no bounded wait should have to last as long as the kernels before
-        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
-            for (int i0 = 0; i0 < p.G && ok; i0 += BATCH, ++bt) {
-                const int ss = bt % S_STAGES, most = min(BATCH, p.G - i0);
-                ok = mbar_wait(sw_full + 8 * ss, (bt / S_STAGES) & 1, abort_flag, p.err_flag);
-                for (int b = (set - it) & (HALF_SETS - 1); b < most; b += HALF_SETS) {
-                    const int at = it + b, s = at % HALF_W_STAGES, sa = at % HALF_STAGES;
-                    ok = mbar_wait(w_full + 8 * s, (at / HALF_W_STAGES) & 1, abort_flag, p.err_flag) && ok;
-                    const uint8_t* const src = gen + L::W_OFF + s * W_BYTES + row * 64;      // 64-byte swizzle: a chunk of 16 bytes by bits 7 and 8
-                    const __half one = reinterpret_cast<const __half*>(gen + L::SW_OFF)[(ss * BATCH + b) * FEATURES + row];
-                    const __half2 m = __half2half2(one), m16 = __half2half2(__hmul(one, __float2half_rn(0.0625f)));
-                    uint4 v[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const uint4*>(src + ((q ^ ((row >> 1) & 3)) << 4));
-                    ok = mbar_wait(ab_empty + 8 * sa, ((at / HALF_STAGES) & 1) ^ 1, abort_flag, p.err_flag) && ok;
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t a[16];
-                        halves_of(v[q].x, m, m16, a);
-                        halves_of(v[q].y, m, m16, a + 4);
-                        halves_of(v[q].z, m, m16, a + 8);
-                        halves_of(v[q].w, m, m16, a + 12);
-                        tmem_st16(tmem + lanes + L::A_COL0 + sa * HALF_A_COLS + 16 * q, a);
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(w_empty + 8 * s);
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(ab_full + 8 * sa);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sw_empty + 8 * ss);
-                it += most;
-            }
-        }
-    } else if (warp >= HALF_EPI0) {
-        constexpr int COLS = HALF_TN / 2;
-        const int quarter = warp & 3, row = quarter * 32 + lane, col0 = ((warp - HALF_EPI0) >> 2) * COLS;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        pdl_wait();
-        bool ok = true;
-        int j = 0;
-        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++j) {
-            const int f0 = tile / p.tiles_m * FEATURES, t0 = tile % p.tiles_m * HALF_TN + col0, d = j & 1;
-            ok = mbar_wait(acc_full + 8 * d, (j >> 1) & 1, abort_flag, p.err_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float power = reinterpret_cast<const float*>(gen + L::POW_OFF)[d * FEATURES + row];
-#pragma unroll 1
-            for (int c = 0; c < COLS; c += 16) {
-                int v[16];
-                tmem_ld16(tmem + lanes + d * HALF_TN + col0 + c, v);
-                uint64_t sum[8];
-                tmem_wait16(v);
-                if (c + 16 == COLS) {
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty + 8 * d);
-                }
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    sum[q] = mul2(pack2(__int_as_float(v[2 * q]), __int_as_float(v[2 * q + 1])),
-                                  pack2(power * token_powers[min(t0 + c + 2 * q, p.M - 1)], power * token_powers[min(t0 + c + 2 * q + 1, p.M - 1)]));
-                leave<__nv_bfloat16, 16>(p, reinterpret_cast<float*>(gen + L::OUT_OFF) + (warp - HALF_EPI0) * 512, sum, f0, quarter, t0 + c, 0);
-            }
-        }
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if (warp == 1) {
-        __syncwarp();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-    }
-}
-
-// Rows of signed bytes, times their scales over a power of two of the row, as half floats; the powers.  A block per row, 16 elements a thread and turn.
-__global__ void __launch_bounds__(256)
-w4_half_rows_kernel(const uint8_t* rows, const float* scales, long long ld_scales, __half* out, float* powers, int G) {
-    __shared__ uint32_t most_of[8];
-    pdl_trigger();
-    pdl_wait();
-    const int t = blockIdx.x, lane = threadIdx.x & 31;
-    uint32_t most = 0;
-    for (int g = threadIdx.x; g < G; g += 256) most = max(most, __float_as_uint(scales[(size_t)g * ld_scales + t]) & 0x7fffffffu);
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) most_of[threadIdx.x >> 5] = most;
-    __syncthreads();
-    most = __reduce_max_sync(0xffffffffu, most_of[lane & 7]);
-    const int e = power_of(most, 3);
-    if (threadIdx.x == 0) powers[t] = exp2f((float)e);
-    const float down = exp2f((float)-e);
-    const uint4* const from = reinterpret_cast<const uint4*>(rows + (size_t)t * G * GROUP);
-    uint4* const to = reinterpret_cast<uint4*>(out + (size_t)t * G * GROUP);
-    for (int i = threadIdx.x; i < G * (GROUP / 16); i += 256) {
-        const uint4 v = from[i];
-        const float s = scales[(size_t)(i / (GROUP / 16)) * ld_scales + t] * down;
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        uint32_t h[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const int k = 16 * (q & 1);
-            h[q] = half2_bits(__floats2half2_rn((float)(int8_t)(w[q >> 1] >> k) * s, (float)(int8_t)(w[q >> 1] >> (k + 8)) * s));
-        }
-        to[2 * i] = make_uint4(h[0], h[1], h[2], h[3]);
-        to[2 * i + 1] = make_uint4(h[4], h[5], h[6], h[7]);
-    }
-}
-
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -942,16 +612,6 @@ EncodeTiledFn encode_tiled() {
             fn = reinterpret_cast<EncodeTiledFn>(ptr);
     }
     return fn;
-}
-// A map of half floats [rows][pitch] in boxes of `high` rows of 64.
-bool half_map(CUtensorMap* map, const void* p, int rows, long long pitch, int high) {
-    EncodeTiledFn fn = encode_tiled();
-    if (!fn) return false;
-    cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)pitch * 2};
-    cuuint32_t box[2] = {64, (cuuint32_t)high}, elem[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // A map of bytes [rows][pitch] in boxes of `high` rows of `wide` bytes.
 bool byte_map(CUtensorMap* map, const void* p, int rows, long long pitch, int wide, int high) {
@@ -982,30 +642,6 @@ int launch_many(const W4Params& w, int splits, cudaStream_t stream) {
     p.tiles = (int)tiles;
     const int items = p.tiles * splits, sms = pyre_sm_count();
     const cudaError_t e = pyre_launch(w4_many_kernel<TN, T>, dim3(items < sms ? items : sms), dim3(MANY_THREADS), (size_t)L::TOTAL, stream, mw, mx, p);
-    if (e != cudaSuccess) return (int)e;
-    PYRE_LAUNCH_CHECK();
-    return 0;
-}
-
-int launch_half(const W4Params& w, void* workspace, cudaStream_t stream) {
-    static bool configured_on[PYRE_MAX_DEVICES] = {};      // the attribute is per device
-    bool& configured = configured_on[pyre_current_device()];
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(w4_half_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Half::TOTAL);
-        if (e != cudaSuccess) return (int)e;
-        configured = true;
-    }
-    __half* const rows = (__half*)workspace;
-    float* const powers = (float*)(rows + (size_t)w.M * w.G * GROUP);
-    CUtensorMap mw, mx;
-    if (!byte_map(&mw, w.packed, w.N, 64ll * w.G, 64, FEATURES) || !half_map(&mx, rows, w.M, 128ll * w.G, HALF_TN)) return PYRE_ERR_BAD_ARG;
-    const long long tiles = (long long)ceil_div(w.M, HALF_TN) * ceil_div(w.N, FEATURES);
-    if (tiles > 0x7fffffffll) return PYRE_ERR_UNSUPPORTED;
-    cudaError_t e = pyre_launch(w4_half_rows_kernel, dim3(w.M), dim3(256), (size_t)0, stream, w.rows, w.row_scales, w.ld_scales, rows, powers, w.G);
-    if (e != cudaSuccess) return (int)e;
-    const ManyParams p = {w.row_scales, w.ld_scales, w.scales, w.out, w.M, w.N, w.G, ceil_div(w.M, HALF_TN), (int)tiles, 1, w.G,
-                          w.N % 8 == 0 && !((uintptr_t)w.out & 15), w.err_flag};
-    e = pyre_launch(w4_half_kernel, dim3((unsigned)min((long long)pyre_sm_count(), tiles)), dim3(HALF_THREADS), (size_t)Half::TOTAL, stream, mw, mx, p, (const float*)powers);
     if (e != cudaSuccess) return (int)e;
     PYRE_LAUNCH_CHECK();
     return 0;
@@ -1126,15 +762,9 @@ PYRE_API int pyre_w4_values(const void* packed, const void* scales, void* out, i
     return 0;
 }
 
-// Bytes of memory that a product of these sizes takes while it runs, for the rows as half floats (0: none).
-PYRE_API long long pyre_w4_workspace(int M, int N, int G, int dtype) {
-    const long long tiles = (long long)ceil_div(M, HALF_TN) * ceil_div(N, FEATURES);
-    return dtype == PYRE_BF16 && M >= HALF_ROWS && G >= HALF_GROUPS && tiles >= pyre_sm_count() ? 256ll * M * G + 4ll * M : 0;
-}
-
 // Shares of K that a product of these sizes leaves (1: none), by what fills the SMs.
-PYRE_API int pyre_w4_splits(int M, int N, int G, int dtype) {
-    if (M <= FEW || pyre_w4_workspace(M, N, G, dtype)) return 1;
+PYRE_API int pyre_w4_splits(int M, int N, int G) {
+    if (M <= FEW) return 1;
     const int tiles = ceil_div(M, M <= 64 ? 64 : 128) * ceil_div(N, FEATURES), sms = pyre_sm_count();
     int splits = min(min(8, sms / max(1, tiles)), G / 4);
     if (splits <= 1) return 1;
@@ -1142,16 +772,15 @@ PYRE_API int pyre_w4_splits(int M, int N, int G, int dtype) {
 }
 
 // rows [M][128 G] and packed [N][64 G] on 16-byte boundaries; out [M, N] of `dtype`, or where `splits` is not 1 float [splits][M][N] (to be added up in
-// order); workspace: as many bytes as `pyre_w4_workspace` says, on a 16-byte boundary
+// order)
 PYRE_API int pyre_w4_linear(const void* rows, const float* row_scales, long long ld_scales, const void* packed, const void* scales, void* out,
-                            int M, int N, int G, int splits, int dtype, void* workspace, int* err_flag, cudaStream_t stream) {
+                            int M, int N, int G, int splits, int dtype, int* err_flag, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (G <= 0 || ((uintptr_t)rows & 15) || ((uintptr_t)packed & 15)) return PYRE_ERR_BAD_ARG;
     if (dtype != PYRE_F32 && dtype != PYRE_BF16) return PYRE_ERR_BAD_ARG;
     if (splits < 1 || (splits > 1 && (M <= FEW || dtype != PYRE_F32 || (splits - 1) * ceil_div(G, splits) >= G))) return PYRE_ERR_BAD_ARG;
     const W4Params p = {(const uint8_t*)rows, row_scales, ld_scales, (const uint8_t*)packed, (const __nv_bfloat16*)scales, out, M, N, G, err_flag};
     if (M <= FEW) return dtype == PYRE_F32 ? launch_few<float>(p, stream) : launch_few<__nv_bfloat16>(p, stream);
-    if (splits == 1 && pyre_w4_workspace(M, N, G, dtype)) return workspace && !((uintptr_t)workspace & 15) ? launch_half(p, workspace, stream) : PYRE_ERR_BAD_ARG;
     if (M <= 64) return dtype == PYRE_F32 ? launch_many<64, float>(p, splits, stream) : launch_many<64, __nv_bfloat16>(p, splits, stream);
     return dtype == PYRE_F32 ? launch_many<128, float>(p, splits, stream) : launch_many<128, __nv_bfloat16>(p, splits, stream);
 }

@@ -93,13 +93,12 @@ SIGNATURES: dict[str, tuple[str, list]] = {
     "pyre_rows8_values": ("rows8", [P, P, LL, P, I, I, I, P]),
     "pyre_w4_quantize": ("gemm_w4", [P, LL, P, P, I, I, I, P]),
     "pyre_w4_values": ("gemm_w4", [P, P, P, I, I, I, P]),
-    "pyre_w4_splits": ("gemm_w4", [I, I, I, I]),
-    "pyre_w4_workspace": ("gemm_w4", [I, I, I, I]),
-    "pyre_w4_linear": ("gemm_w4", [P, P, LL, P, P, P, I, I, I, I, I, P, P, P]),
+    "pyre_w4_splits": ("gemm_w4", [I, I, I]),
+    "pyre_w4_linear": ("gemm_w4", [P, P, LL, P, P, P, I, I, I, I, I, P, P]),
 }
 
 #: functions that return a number of another type than int (sizes; see ``call_value``)
-RESULTS = {"pyre_fixed_workspace": c_longlong, "pyre_w4_workspace": c_longlong}
+RESULTS = {"pyre_fixed_workspace": c_longlong}
 
 _ERRORS = {100001: "bad argument", 100002: "unsupported size"}
 

@@ -481,15 +481,14 @@ def linear4(x: "torch.Tensor | Rows8", w: Weight4, out_dtype: "torch.dtype | Non
     if packed.device != rows.device:
         require_current_device(packed.device, "w")
     dtype, groups = out_dtype or x.dtype, scales.shape[0]
-    splits, size = _w4_plan(T, N, groups, _dt(torch.float32 if partials_ok else dtype), rows.get_device()) if T > W4_STREAM_ROWS else (1, 0)
-    work = torch.empty(size, dtype=torch.uint8, device=rows.device) if size else None
+    splits = _w4_splits(T, N, groups, rows.get_device()) if T > W4_STREAM_ROWS else 1
     shares = partials_ok or splits > 1
     if shares:
         out = torch.empty(splits, T, N, dtype=torch.float32, device=rows.device)
     else:
         out = torch.empty(T, N, dtype=dtype, device=rows.device)
     lib.call("pyre_w4_linear", rows.data_ptr(), scales.data_ptr(), scales.stride(0), packed.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
-             T, N, groups, splits, _dt(out.dtype), _ptr(work), device_error_flag(rows.device).data_ptr(), _stream())
+             T, N, groups, splits, _dt(out.dtype), device_error_flag(rows.device).data_ptr(), _stream())
     if not shares:
         return out
     out = PartialSums(out, dtype)
@@ -500,9 +499,8 @@ W4_STREAM_ROWS = 32      # up to here ``pyre_w4_linear`` shares K within cluster
 
 
 @functools.lru_cache(maxsize=4096)
-def _w4_plan(T: int, N: int, groups: int, dtype: int, device: int) -> "tuple[int, int]":
-    """Shares of K, and bytes of memory that the product takes while it runs."""
-    return lib.call_value("pyre_w4_splits", T, N, groups, dtype), lib.call_value("pyre_w4_workspace", T, N, groups, dtype)
+def _w4_splits(T: int, N: int, groups: int, device: int) -> int:
+    return lib.call_value("pyre_w4_splits", T, N, groups)
 
 
 def add_residual(x: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:
