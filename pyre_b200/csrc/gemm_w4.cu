@@ -44,32 +44,69 @@ __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
     while (!mbar_try_wait(bar, parity) && clock64() - t0 < PYRE_WAIT_CYCLES) {}
 }
 
+// What the CTAs of a cluster hold of the tile of F features from f0 and `tokens` tokens from t0 on, SETS times [token][F + 4] floats each (`stride` apart, at
+// the start of shared memory), added up in order.  (A row of F + 4: what a warp stores at once falls on different banks.)
+template <int SETS, int F, typename T>
+__device__ __forceinline__ void add_shares(const W4Params& p, uint8_t* gen, int stride, bool failed, int f0, int t0, int tokens) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    if (C > 1) cluster.sync();
+    if (!failed) {      // (a CTA that gave up raised the error word: what the others write is not looked at)
+        const bool vec = p.N % 4 == 0 && !((uintptr_t)p.out & (4 * sizeof(T) - 1));
+        for (int i = rank * blockDim.x + threadIdx.x; i < tokens * (F / 4); i += C * blockDim.x) {
+            const int t = i / (F / 4), f = i % (F / 4) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int q = 0; q < C; ++q) {
+                const float* const sums = reinterpret_cast<const float*>(C > 1 ? cluster.map_shared_rank(gen, q) : gen) + t * (F + 4) + f;
+#pragma unroll
+                for (int e = 0; e < SETS; ++e) {
+                    const float4 a = *reinterpret_cast<const float4*>(sums + e * stride);
+                    v.x += a.x;
+                    v.y += a.y;
+                    v.z += a.z;
+                    v.w += a.w;
+                }
+            }
+            T* const out = (T*)p.out + (size_t)(t0 + t) * p.N + f0 + f;
+            const Vec<T, 4> rounded = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+            if (vec) {
+                if (f0 + f < p.N) store_vec<T, 4>(out, rounded);
+            } else
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (f0 + f + k < p.N) out[k] = rounded.v[k];
+        }
+    }
+    if (C > 1) cluster.sync();      // the others' sums are read
+}
+
 // ---------------------------------------------------------------------------
-// Few rows: a stream of weights from memory.  A CTA owns 128 features and up to 8 NT tokens; the CTAs of a cluster share a tile's K.
-//   warp 8, one thread : TMA.  Two groups of 128 k at a time into a ring of STAGES: the weights as they are packed, the tokens' bytes.  (A copy of one group
-//                        has rows of 64 bytes, which hold up its engine: 24 x 5,120 x 27,648 took 22.6 us with them, ROWS128 with two.)
-//   warp 9             : the groups' scales, of the features (a sixteenth of them: the integers are sixteen times as large) and of the tokens.
-//   warps 0..7         : two sets of four that take the stages in turn; a warp owns 32 features.  Lane l holds 32 neighbouring elements (the l % 4th quarter
+// Few rows: a stream of weights from memory.  A CTA owns F features (128 or 96) and up to 8 NT tokens; the CTAs of a cluster share a tile's K.
+//   two last warps     : one thread, TMA.  Two groups of 128 k at a time into a ring of STAGES: the weights as they are packed, the tokens' bytes.  (A copy of one group
+//                        has rows of 64 bytes, which hold up its engine.)  And the
+//                        groups' scales, of the features (a sixteenth of them: the integers are sixteen times as large) and of the tokens.
+//   the others         : two sets of F / 32 that take the stages in turn; a warp owns 32 features.  Lane l holds 32 neighbouring elements (the l % 4th quarter
 //                        of the group) of four features and of token l / 4: which k an MMA step sums over is free as long as both
 //                        operands agree.
 // The sets' and the cluster's shares meet in shared memory and are added in order.
 // ---------------------------------------------------------------------------
-constexpr int STREAM_THREADS = 320, STREAM_STAGES = 4, PAIR = 2;
-constexpr int ROW = FEATURES + 4;      // of a token's sums: what a warp stores at once falls on different banks
+constexpr int STREAM_STAGES = 4, PAIR = 2;
 
-template <int NT> struct Stream {
+template <int NT, int F> struct Stream {
+    static constexpr int WARPS = F / 32, THREADS = (2 * WARPS + 2) * 32, ROW = F + 4, W_BYTES = F * GROUP / 2;      // of a set; ...; a token's sums (see below); a group's
     static constexpr int X_BYTES = NT * 8 * GROUP;                                                    // a group's
     static constexpr int STAGE = PAIR * (W_BYTES + X_BYTES);                                          // multiples of 1,024: the swizzles' patterns
-    static constexpr int SCALES = STREAM_STAGES * STAGE, SCALE = (FEATURES + NT * 8) * 4;             // [stage][group][features, tokens] floats
+    static constexpr int SCALES = STREAM_STAGES * STAGE, SCALE = (F + NT * 8) * 4;             // [stage][group][features, tokens] floats
     static constexpr int BARS = SCALES + STREAM_STAGES * PAIR * SCALE;
     static constexpr int TOTAL = BARS + STREAM_STAGES * 16 + 16 + 1024;
     static_assert(2 * NT * 8 * ROW * 4 <= SCALES && 2 * (TOTAL + 1024) <= 233472 && STREAM_STAGES % 2 == 0, "the sets' sums take the ring's place; two CTAs");
 };
 
-template <int NT, typename T>
-__global__ void __launch_bounds__(STREAM_THREADS, 2)
+template <int NT, int F, typename T>
+__global__ void __launch_bounds__(2 * F + 64, 2)
 w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const W4Params p) {
-    using L = Stream<NT>;
+    using L = Stream<NT, F>;
+    constexpr int W_BYTES = L::W_BYTES, WARPS = L::WARPS, ROW = L::ROW;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
@@ -78,18 +115,18 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int f0 = blockIdx.x / C * FEATURES, t0 = blockIdx.y * NT * 8;
+    const int f0 = blockIdx.x / C * F, t0 = blockIdx.y * NT * 8;
     const int first = (int)((long long)rank * p.G / C), n = (int)((rank + 1ll) * p.G / C) - first, steps = (n + PAIR - 1) / PAIR;      // four groups at least
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
-        for (int s = 0; s < STREAM_STAGES; ++s) { mbar_init(full + 8 * s, 2); mbar_init(empty + 8 * s, 4); }
+        for (int s = 0; s < STREAM_STAGES; ++s) { mbar_init(full + 8 * s, 2); mbar_init(empty + 8 * s, WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
     pdl_trigger();
     bool ok = true;
-    if (warp == 8) {
+    if (warp == 2 * WARPS) {
         if (lane == 0) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
@@ -115,16 +152,16 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             if (!ok)      // a wait ran out: the copies in flight end first
                 for (int i = max(0, asked - STREAM_STAGES); i < asked; ++i) mbar_drain(full + 8 * (i % STREAM_STAGES), (i / STREAM_STAGES) & 1);
         }
-    } else if (warp == 9) {
-        constexpr int BATCH = 4, F = FEATURES / 32;
+    } else if (warp == 2 * WARPS + 1) {
+        constexpr int BATCH = 4;
         static_assert(BATCH % PAIR == 0 && NT <= 4, "whole stages, a lane per token");
         bool waited = false;
         for (int i0 = 0; i0 < n && ok; i0 += BATCH) {
-            float v[BATCH][F], x[BATCH];
+            float v[BATCH][WARPS], x[BATCH];
 #pragma unroll
             for (int j = 0; j < BATCH; ++j)
 #pragma unroll
-                for (int q = 0; q < F; ++q)
+                for (int q = 0; q < WARPS; ++q)
                     v[j][q] = __bfloat162float(p.scales[(size_t)(first + min(i0 + j, n - 1)) * p.N + min(f0 + q * 32 + lane, p.N - 1)]) * 0.0625f;
             if (!waited) pdl_wait();
             waited = true;
@@ -141,8 +178,8 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 }
                 float* const to = reinterpret_cast<float*>(gen + L::SCALES + (s * PAIR + j % PAIR) * L::SCALE);
 #pragma unroll
-                for (int q = 0; q < F; ++q) to[q * 32 + lane] = v[j][q];
-                if (lane < NT * 8) to[FEATURES + lane] = x[j];
+                for (int q = 0; q < WARPS; ++q) to[q * 32 + lane] = v[j][q];
+                if (lane < NT * 8) to[F + lane] = x[j];
                 if (j % PAIR == PAIR - 1) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(full + 8 * s);
@@ -151,7 +188,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
         if (!waited) pdl_wait();
     } else {
-        const int set = warp >> 2, row0 = (warp & 3) * 32, quad = lane >> 2, c = lane & 3;
+        const int set = warp / WARPS, row0 = warp % WARPS * 32, quad = lane >> 2, c = lane & 3;
         // The feature of a lane among eight: neighbouring lanes of four read rows four apart, whose swizzles are different.
         const int row8 = (quad >> 1) | (quad & 1) << 2;
         float total[NT][2][4] = {};
@@ -182,7 +219,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                     const uint4 x0 = *reinterpret_cast<const uint4*>(src + (((2 * c) ^ quad) << 4));
                     const uint4 x1 = *reinterpret_cast<const uint4*>(src + (((2 * c + 1) ^ quad) << 4));
                     const uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-                    const float2 sx = *reinterpret_cast<const float2*>(scales + FEATURES + t * 8 + 2 * c);
+                    const float2 sx = *reinterpret_cast<const float2*>(scales + F + t * 8 + 2 * c);
                     int d[2][4] = {};
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -201,7 +238,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             if (lane == 0) mbar_arrive(empty + 8 * s);
         }
         // [set][token][feature]; the ring is free once both sets are through it
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(2 * F) : "memory");
         float* const sums = reinterpret_cast<float*>(gen) + set * NT * 8 * ROW;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -211,33 +248,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 for (int e = 0; e < 4; ++e) sums[(t * 8 + 2 * c + (e & 1)) * ROW + row0 + h * 16 + (e >> 1) * 8 + row8] = total[t][h][e];
     }
     const bool failed = __syncthreads_or(!ok);
-    if (C > 1) cluster.sync();
-    if (!failed) {
-        // (a CTA that gave up raised the error word: what the others write is not looked at)
-        const int tokens = min(NT * 8, p.M - t0);
-        const bool vec = p.N % 4 == 0 && !((uintptr_t)p.out & (4 * sizeof(T) - 1));
-        for (int i = rank * STREAM_THREADS + threadIdx.x; i < tokens * (FEATURES / 4); i += C * STREAM_THREADS) {
-            const int t = i / (FEATURES / 4), f = i % (FEATURES / 4) * 4;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int q = 0; q < C; ++q) {
-                const float* const sums = reinterpret_cast<const float*>(C > 1 ? cluster.map_shared_rank(gen, q) : gen) + t * ROW + f;
-                const float4 a = *reinterpret_cast<const float4*>(sums), b = *reinterpret_cast<const float4*>(sums + NT * 8 * ROW);
-                v.x += a.x + b.x;
-                v.y += a.y + b.y;
-                v.z += a.z + b.z;
-                v.w += a.w + b.w;
-            }
-            T* const out = (T*)p.out + (size_t)(t0 + t) * p.N + f0 + f;
-            const Vec<T, 4> rounded = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
-            if (vec) {
-                if (f0 + f < p.N) store_vec<T, 4>(out, rounded);
-            } else
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (f0 + f + k < p.N) out[k] = rounded.v[k];
-        }
-    }
-    if (C > 1) cluster.sync();      // the others' sums are read
+    add_shares<2, F, T>(p, gen, NT * 8 * ROW, failed, f0, t0, min(NT * 8, p.M - t0));
 }
 
 // ---------------------------------------------------------------------------
@@ -249,23 +260,11 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 //   warp 2             : the scales of four groups at a time, of features and of tokens, to shared memory.
 //   warps 8..15        : a thread owns a feature and half of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
 //                        feature and added to float sums in registers, by ascending group.
-// An output tile whose K is shared among CTAs (few tiles) leaves float shares, added up in order by whoever reads them.
+// Where there are few tiles the CTAs of a cluster share a tile's K, and their sums meet in shared memory.
 // ---------------------------------------------------------------------------
 constexpr int MANY_THREADS = 512, EPI_WARP0 = 8, EPI_WARPS = 8, A_COLS = 32;
 constexpr int W_STAGES = 6, STAGES = 6;               // packed weights; both operands of the MMAs
 constexpr int BATCH = 4, S_STAGES = 2;                // groups whose scales come at a time
-
-struct ManyParams {
-    const float* row_scales;
-    long long ld_scales;
-    const __nv_bfloat16* scales;
-    void* out;                    // [M][N], or float [splits][M][N]
-    int M, N, G;
-    int tiles_m, tiles;           // tiles of tokens (fastest); of everything
-    int splits, per_split;        // of K, in groups
-    int vec;                      // output rows lie on 16-byte boundaries
-    int* err_flag;
-};
 
 __device__ __forceinline__ bool elect_one() {
     uint32_t one;
@@ -313,14 +312,14 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // A warp's part of a tile (32 features from f0 + 32 quarter on, COLS tokens from t0 on) leaves by whole 16-byte pieces, 16 tokens at a time through shared
 // memory (`stage`): single elements (32 stores a thread) took 220 of 1,180 cycles a group where K is 3,584.  Rows off 16-byte boundaries leave by elements.
 template <typename T, int COLS>
-__device__ __forceinline__ void leave(const ManyParams& p, float* stage, const uint64_t (&sum)[COLS / 2], int f0, int quarter, int t0, int split) {
+__device__ __forceinline__ void leave(const W4Params& p, float* stage, const uint64_t (&sum)[COLS / 2], int f0, int quarter, int t0, bool vec) {
     const int lane = threadIdx.x & 31, row = quarter * 32 + lane;
-    T* const out = (T*)p.out + (size_t)split * p.M * p.N;
+    T* const out = (T*)p.out;
     constexpr int PIECE = 16 / sizeof(T), PIECES = 32 / PIECE, ROWS = 32 / PIECES;      // elements; a warp's features in pieces; rows at a time
     const int left = p.M - t0;
 #pragma unroll
     for (int c = 0; c < COLS; c += 16) {
-        if (p.vec) {
+        if (vec) {
             __syncwarp();
 #pragma unroll
             for (int q = 0; q < 16; q += 2) {
@@ -361,12 +360,13 @@ template <int TN> struct Many {
     static constexpr int N_BARS = 2 * (W_STAGES + STAGES + S_STAGES + 2) + 1;
     static constexpr int TOTAL = BARS + N_BARS * 8 + 24 + 1024;
     static constexpr int A_COL0 = 2 * TN;
-    static_assert(A_COL0 + STAGES * A_COLS <= 512 && TOTAL <= 232448 && TN % 64 == 0, "fits");
+    static_assert(A_COL0 + STAGES * A_COLS <= 512 && TOTAL <= 232448 && TN % 64 == 0 && TN * (FEATURES + 4) * 4 <= SX_OFF, "fits");
 };
 
-template <int TN, typename T>
+// SHARED: the CTAs of a cluster share a tile's K, a tile each; else a CTA takes tile after tile.
+template <int TN, bool SHARED, typename T>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
-w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ ManyParams p) {
+w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ W4Params p, int tiles_m, int tiles) {
     using L = Many<TN>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -378,7 +378,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + L::BARS + L::N_BARS * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::BARS + L::N_BARS * 8 + 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int items = p.tiles * p.splits;
+    const int C = SHARED ? (int)cg::this_cluster().num_blocks() : 1, rank = SHARED ? (int)cg::this_cluster().block_rank() : 0;
+    const int first = SHARED ? (int)((long long)rank * p.G / C) : 0, n = SHARED ? (int)((rank + 1ll) * p.G / C) - first : p.G;
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -400,16 +401,11 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const uint32_t tmem = *tmem_slot;
     pdl_trigger();
 
-    auto range = [&](int item, int& f0, int& t0, int& split, int& first, int& n) {
-        const int tile = item % p.tiles;
-        split = item / p.tiles;
-        f0 = tile / p.tiles_m * FEATURES;
-        t0 = tile % p.tiles_m * TN;
-        first = split * p.per_split;
-        n = min(p.per_split, p.G - first);      // at least one: no share is empty
+    int f0, t0;
+    auto place = [&](int tile) {
+        f0 = tile / tiles_m * FEATURES;
+        t0 = tile % tiles_m * TN;
     };
-
-    int f0, t0, split, first, n;
     if (warp == 0 || warp == 3) {
         if (lane == 0) {
             // the weights have a thread of their own: they are converted, so they are wanted well before the rows are
@@ -419,8 +415,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
             bool waited = false, ok = true;
             uint32_t it = 0;
-            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-                range(item, f0, t0, split, first, n);
+            for (int tile = blockIdx.x / C; tile < tiles && ok; tile += gridDim.x / C) {
+                place(tile);
                 for (int i = 0; i < n; ++i) {
                     if (!waited && (rows || it == W_STAGES)) { pdl_wait(); waited = true; }      // (the weights depend on no earlier kernel)
                     const uint32_t s = it % stages;
@@ -443,8 +439,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         int it = 0, s = 0;
         bool ok = true;
         pdl_wait();      // no bounded wait should have to last as long as the kernels before
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-            range(item, f0, t0, split, first, n);
+        for (int tile = blockIdx.x / C; tile < tiles && ok; tile += gridDim.x / C) {
+            place(tile);
             for (int i = 0; i < n; ++i, ++it) {
                 const int d = it & 1;
                 ok = mbar_wait(acc_empty + 8 * d, ((it >> 1) & 1) ^ 1, abort_flag, p.err_flag) &&
@@ -474,8 +470,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         bool ok = true;
         int bt = 0;
         pdl_wait();
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-            range(item, f0, t0, split, first, n);
+        for (int tile = blockIdx.x / C; tile < tiles && ok; tile += gridDim.x / C) {
+            place(tile);
             for (int i0 = 0; i0 < n && ok; i0 += BATCH, ++bt) {
                 const int s = bt % S_STAGES;
                 constexpr int F = FEATURES / 32, X = TN / 32;
@@ -508,8 +504,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         bool waited = false, ok = true;
         int it = 0;
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-            range(item, f0, t0, split, first, n);
+        for (int tile = blockIdx.x / C; tile < tiles && ok; tile += gridDim.x / C) {
+            place(tile);
             for (int i = 0; i < n && ok; ++i, ++it) {
                 const int s = it % W_STAGES, sa = it % STAGES;
                 ok = mbar_wait(w_full + 8 * s, (it / W_STAGES) & 1, abort_flag, p.err_flag);
@@ -544,8 +540,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         pdl_wait();
         bool ok = true;
         int it = 0, bt = 0;
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-            range(item, f0, t0, split, first, n);
+        for (int tile = blockIdx.x / C; tile < tiles && ok; tile += gridDim.x / C) {
+            place(tile);
             uint64_t sum[COLS / 2];
 #pragma unroll
             for (int q = 0; q < COLS / 2; ++q) sum[q] = 0;
@@ -589,7 +585,14 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 if (lane == 0) mbar_arrive(s_empty + 8 * s);
             }
             if (!ok) break;
-            leave<T, COLS>(p, reinterpret_cast<float*>(gen + L::OUT_OFF) + (warp - EPI_WARP0) * 512, sum, f0, quarter, t0 + col0, split);
+            if (!SHARED) {
+                leave<T, COLS>(p, reinterpret_cast<float*>(gen + L::OUT_OFF) + (warp - EPI_WARP0) * 512, sum, f0, quarter, t0 + col0,
+                               p.N % (16 / sizeof(T)) == 0 && !((uintptr_t)p.out & 15));
+            } else {      // [token][feature], in the rings' place: all that was in them has been used
+                float* const sums = reinterpret_cast<float*>(gen) + col0 * (FEATURES + 4) + row;
+#pragma unroll
+                for (int q = 0; q < COLS; ++q) sums[q * (FEATURES + 4)] = __uint_as_float((uint32_t)(sum[q / 2] >> (q & 1 ? 32 : 0)));
+            }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -597,6 +600,10 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (warp == 1) {
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+    if (SHARED) {
+        place(blockIdx.x / C);
+        add_shares<1, FEATURES, T>(p, gen, 0, *abort_flag != 0, f0, t0, min(TN, p.M - t0));
     }
 }
 
@@ -624,70 +631,103 @@ bool byte_map(CUtensorMap* map, const void* p, int rows, long long pitch, int wi
               wide == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int TN, typename T>
-int launch_many(const W4Params& w, int splits, cudaStream_t stream) {
-    using L = Many<TN>;
-    static bool configured_on[PYRE_MAX_DEVICES] = {};      // the attribute is per device
-    bool& configured = configured_on[pyre_current_device()];
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(w4_many_kernel<TN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
-        if (e != cudaSuccess) return (int)e;
-        configured = true;
-    }
-    CUtensorMap mw, mx;
-    if (!byte_map(&mw, w.packed, w.N, 64ll * w.G, 64, FEATURES) || !byte_map(&mx, w.rows, w.M, 128ll * w.G, 128, TN)) return PYRE_ERR_BAD_ARG;
-    ManyParams p = {w.row_scales, w.ld_scales, w.scales, w.out, w.M, w.N, w.G, ceil_div(w.M, TN), 0, splits, ceil_div(w.G, splits), w.N % (16 / (int)sizeof(T)) == 0 && !((uintptr_t)w.out & 15), w.err_flag};
-    const long long tiles = (long long)p.tiles_m * ceil_div(w.N, FEATURES);
-    if (tiles * splits > 0x7fffffffll) return PYRE_ERR_UNSUPPORTED;
-    p.tiles = (int)tiles;
-    const int items = p.tiles * splits, sms = pyre_sm_count();
-    const cudaError_t e = pyre_launch(w4_many_kernel<TN, T>, dim3(items < sms ? items : sms), dim3(MANY_THREADS), (size_t)L::TOTAL, stream, mw, mx, p);
-    if (e != cudaSuccess) return (int)e;
-    PYRE_LAUNCH_CHECK();
-    return 0;
-}
-
-// CTAs that share a tile's K: as many as find room on the SMs, each with four groups at least.
-template <int NT, typename T>
-int launch_stream(const W4Params& p, cudaStream_t stream) {
-    using L = Stream<NT>;
-    static bool configured_on[PYRE_MAX_DEVICES] = {};      // the attribute is per device
-    bool& configured = configured_on[pyre_current_device()];
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(w4_stream_kernel<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
-        if (e != cudaSuccess) return (int)e;
-        configured = true;
-    }
-    CUtensorMap mw, mx;
-    if (!byte_map(&mw, p.packed, p.N, 64ll * p.G, 128, FEATURES) || !byte_map(&mx, p.rows, p.M, 128ll * p.G, 128, NT * 8)) return PYRE_ERR_BAD_ARG;
-    const int tiles = ceil_div(p.N, FEATURES), rows = ceil_div(p.M, NT * 8), room = 2 * pyre_sm_count();
-    int C = 1;
-    while (C < 8 && 2ll * C * tiles * rows <= room && p.G >= 8 * C) C *= 2;
+// Clusters of `kernel` that find room at once, by their CTAs' number's logarithm (a cluster needs its CTAs on neighbouring SMs; the driver knows how many there
+// are room for).  Worked out once per kernel and device.
+struct Room {
+    int known, clusters[4];
+};
+template <typename... Args>
+cudaError_t find_room(void (*kernel)(Args...), int threads, int bytes, Room& room) {
+    if (room.known) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)rows);
-    cfg.blockDim = dim3(STREAM_THREADS);
-    cfg.dynamicSmemBytes = L::TOTAL;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = bytes;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    for (int i = 1; i < 4; ++i) {
+        attr.val.clusterDim.x = 1 << i;
+        cfg.gridDim = dim3(1 << i);
+        e = cudaOccupancyMaxActiveClusters(&room.clusters[i], kernel, &cfg);
+        if (e != cudaSuccess) return e;
+    }
+    room.known = 1;
+    return cudaSuccess;
+}
+// The logarithm of the number of CTAs that share a tile's K: as many as find room, each with four groups at least.
+int shares_of(const Room& room, long long tiles, int G) {
+    int i = 3;
+    while (i > 0 && (tiles > room.clusters[i] || G < 4 << i)) --i;
+    return i;
+}
+template <typename... Args>
+int launch_clusters(void (*kernel)(Args...), dim3 grid, int cluster, int threads, int bytes, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pyre_pdl_enabled() ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_stream_kernel<NT, T>, mw, mx, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess) return (int)e;
     PYRE_LAUNCH_CHECK();
     return 0;
 }
+template <int TN, typename T>
+int launch_many(const W4Params& p, cudaStream_t stream) {
+    using L = Many<TN>;
+    static Room shared_room[PYRE_MAX_DEVICES] = {}, room[PYRE_MAX_DEVICES] = {};
+    const int dev = pyre_current_device();
+    cudaError_t e = find_room(w4_many_kernel<TN, true, T>, MANY_THREADS, L::TOTAL, shared_room[dev]);
+    if (e == cudaSuccess) e = find_room(w4_many_kernel<TN, false, T>, MANY_THREADS, L::TOTAL, room[dev]);
+    if (e != cudaSuccess) return (int)e;
+    CUtensorMap mw, mx;
+    if (!byte_map(&mw, p.packed, p.N, 64ll * p.G, 64, FEATURES) || !byte_map(&mx, p.rows, p.M, 128ll * p.G, 128, TN)) return PYRE_ERR_BAD_ARG;
+    const int tiles_m = ceil_div(p.M, TN);
+    const long long tiles = (long long)tiles_m * ceil_div(p.N, FEATURES);
+    if (tiles > 0x7fffffffll) return PYRE_ERR_UNSUPPORTED;
+    const int i = shares_of(shared_room[dev], tiles, p.G);
+    if (i > 0) return launch_clusters(w4_many_kernel<TN, true, T>, dim3((unsigned)tiles << i), 1 << i, MANY_THREADS, L::TOTAL, stream, mw, mx, p, tiles_m, (int)tiles);
+    return launch_clusters(w4_many_kernel<TN, false, T>, dim3((unsigned)min(tiles, (long long)pyre_sm_count())), 1, MANY_THREADS, L::TOTAL, stream, mw, mx, p, tiles_m, (int)tiles);
+}
+template <int NT, int F, typename T>
+int launch_stream(const W4Params& p, cudaStream_t stream) {
+    using L = Stream<NT, F>;
+    static Room room[PYRE_MAX_DEVICES] = {};
+    const int dev = pyre_current_device(), tiles = ceil_div(p.N, F), rows = ceil_div(p.M, NT * 8);
+    const cudaError_t e = find_room(w4_stream_kernel<NT, F, T>, L::THREADS, L::TOTAL, room[dev]);
+    if (e != cudaSuccess) return (int)e;
+    CUtensorMap mw, mx;
+    if (!byte_map(&mw, p.packed, p.N, 64ll * p.G, 128, F) || !byte_map(&mx, p.rows, p.M, 128ll * p.G, 128, NT * 8)) return PYRE_ERR_BAD_ARG;
+    const int i = shares_of(room[dev], (long long)tiles * rows, p.G);
+    return launch_clusters(w4_stream_kernel<NT, F, T>, dim3((unsigned)tiles << i, (unsigned)rows), 1 << i, L::THREADS, L::TOTAL, stream, mw, mx, p);
+}
+// Tiles of 96 features where those of 128 would leave an SM more of them: 24 x 5,120 x 27,648 (216 tiles, two on some SMs, or 288) 18.1 us against 22.3.
+template <int NT, typename T>
+int launch_tiles(const W4Params& p, cudaStream_t stream) {
+    const int sms = pyre_sm_count();
+    auto features = [&](int F) { return ceil_div(ceil_div(p.N, F), sms) * F; };
+    return ceil_div(p.N, FEATURES) > sms && ceil_div(p.N, 96) <= 2 * sms && features(96) < features(FEATURES) ? launch_stream<NT, 96, T>(p, stream)
+                                                                                                            : launch_stream<NT, FEATURES, T>(p, stream);
+}
 template <typename T>
 int launch_few(const W4Params& p, cudaStream_t stream) {
     switch (ceil_div(p.M, 8)) {
-        case 1: return launch_stream<1, T>(p, stream);
-        case 2: return launch_stream<2, T>(p, stream);
-        case 3: return launch_stream<3, T>(p, stream);
-        default: return launch_stream<4, T>(p, stream);
+        case 1: return launch_tiles<1, T>(p, stream);
+        case 2: return launch_tiles<2, T>(p, stream);
+        case 3: return launch_tiles<3, T>(p, stream);
+        default: return launch_tiles<4, T>(p, stream);
     }
 }
 constexpr int FEW = 32;      // rows up to here take the stream
@@ -762,25 +802,14 @@ PYRE_API int pyre_w4_values(const void* packed, const void* scales, void* out, i
     return 0;
 }
 
-// Shares of K that a product of these sizes leaves (1: none), by what fills the SMs.
-PYRE_API int pyre_w4_splits(int M, int N, int G) {
-    if (M <= FEW) return 1;
-    const int tiles = ceil_div(M, M <= 64 ? 64 : 128) * ceil_div(N, FEATURES), sms = pyre_sm_count();
-    int splits = min(min(8, sms / max(1, tiles)), G / 4);
-    if (splits <= 1) return 1;
-    return ceil_div(G, ceil_div(G, splits));      // no empty share
-}
-
-// rows [M][128 G] and packed [N][64 G] on 16-byte boundaries; out [M, N] of `dtype`, or where `splits` is not 1 float [splits][M][N] (to be added up in
-// order)
+// rows [M][128 G] and packed [N][64 G] on 16-byte boundaries; out [M, N] of `dtype`
 PYRE_API int pyre_w4_linear(const void* rows, const float* row_scales, long long ld_scales, const void* packed, const void* scales, void* out,
-                            int M, int N, int G, int splits, int dtype, int* err_flag, cudaStream_t stream) {
+                            int M, int N, int G, int dtype, int* err_flag, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (G <= 0 || ((uintptr_t)rows & 15) || ((uintptr_t)packed & 15)) return PYRE_ERR_BAD_ARG;
     if (dtype != PYRE_F32 && dtype != PYRE_BF16) return PYRE_ERR_BAD_ARG;
-    if (splits < 1 || (splits > 1 && (M <= FEW || dtype != PYRE_F32 || (splits - 1) * ceil_div(G, splits) >= G))) return PYRE_ERR_BAD_ARG;
     const W4Params p = {(const uint8_t*)rows, row_scales, ld_scales, (const uint8_t*)packed, (const __nv_bfloat16*)scales, out, M, N, G, err_flag};
     if (M <= FEW) return dtype == PYRE_F32 ? launch_few<float>(p, stream) : launch_few<__nv_bfloat16>(p, stream);
-    if (M <= 64) return dtype == PYRE_F32 ? launch_many<64, float>(p, splits, stream) : launch_many<64, __nv_bfloat16>(p, splits, stream);
-    return dtype == PYRE_F32 ? launch_many<128, float>(p, splits, stream) : launch_many<128, __nv_bfloat16>(p, splits, stream);
+    if (M <= 64) return dtype == PYRE_F32 ? launch_many<64, float>(p, stream) : launch_many<64, __nv_bfloat16>(p, stream);
+    return dtype == PYRE_F32 ? launch_many<128, float>(p, stream) : launch_many<128, __nv_bfloat16>(p, stream);
 }

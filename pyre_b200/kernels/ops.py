@@ -134,10 +134,10 @@ class Rows8:
     product with a ``Weight4`` reads them as they are; anything else calls ``materialize``, which rounds to ``dtype``."""
 
     def __init__(self, rows: torch.Tensor, scales: torch.Tensor, width: int, dtype: torch.dtype = torch.bfloat16):
-        groups = -(-width // GROUP8)
-        if rows.dtype != torch.int8 or rows.dim() != 2 or rows.shape[1] != groups * GROUP8 or width <= 0:
+        groups, shape = -(-width // GROUP8), rows.shape
+        if rows.dtype is not torch.int8 or len(shape) != 2 or shape[1] != groups * GROUP8 or width <= 0:
             raise ValueError(f"rows of {width} elements in 8 bits are int8 [T, {groups * GROUP8}], got {rows.dtype} {tuple(rows.shape)}")
-        if scales.dtype != torch.float32 or tuple(scales.shape) != (groups, rows.shape[0]):
+        if scales.dtype is not torch.float32 or scales.shape != (groups, shape[0]):
             raise ValueError(f"scales must be float32 {(groups, rows.shape[0])}, got {scales.dtype} {tuple(scales.shape)}")
         self.rows, self.scales, self.width, self.dtype = rows, scales, width, dtype
 
@@ -168,14 +168,13 @@ class Weight4:
     times its group's scale."""
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, width: int):
-        groups = -(-width // GROUP8)
-        if packed.dtype != torch.uint8 or packed.dim() != 2 or packed.shape[1] != groups * (GROUP8 // 2) or width <= 0:
+        groups, shape = -(-width // GROUP8), packed.shape
+        if packed.dtype is not torch.uint8 or len(shape) != 2 or shape[1] != groups * (GROUP8 // 2) or width <= 0:
             raise ValueError(f"a weight of {width} columns in 4 bits is uint8 [N, {groups * GROUP8 // 2}], got {packed.dtype} {tuple(packed.shape)}")
-        if scales.dtype != torch.bfloat16 or tuple(scales.shape) != (groups, packed.shape[0]):
+        if scales.dtype is not torch.bfloat16 or scales.shape != (groups, shape[0]):
             raise ValueError(f"scales must be bfloat16 {(groups, packed.shape[0])}, got {scales.dtype} {tuple(scales.shape)}")
-        for t, name in ((packed, "packed"), (scales, "scales")):
-            if not t.is_cuda or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous CUDA tensor")
+        if not (packed.is_cuda and scales.is_cuda and packed.is_contiguous() and scales.is_contiguous() and packed.device == scales.device):
+            raise ValueError("packed and scales must be contiguous CUDA tensors on one device")
         if packed.data_ptr() % 16:
             raise ValueError("packed must start on a 16-byte boundary")
         self.packed, self.scales, self.width = packed, scales, width
@@ -469,8 +468,7 @@ def quantize_weight4(w: torch.Tensor) -> Weight4:
 
 def linear4(x: "torch.Tensor | Rows8", w: Weight4, out_dtype: "torch.dtype | None" = None, partials_ok: bool = False) -> "torch.Tensor | PartialSums":
     """y = x W^T for a weight in 4 bits: whole numbers summed exactly within a group, the groups in float32.  Activations that are
-    not in 8 bits yet go through ``quantize_rows8`` first.  ``partials_ok``: ``PartialSums`` in float32 come back, one part or, where K is
-    shared among CTAs, several."""
+    not in 8 bits yet go through ``quantize_rows8`` first.  ``partials_ok``: the result comes back unrounded, as the one part of ``PartialSums``."""
     if not isinstance(x, Rows8):
         x = quantize_rows8(materialize(x))
     _check_rows8(x)
@@ -480,27 +478,11 @@ def linear4(x: "torch.Tensor | Rows8", w: Weight4, out_dtype: "torch.dtype | Non
         raise ValueError(f"inner sizes differ: x is [{T}, {K}], w is [{N}, {w.width}]")
     if packed.device != rows.device:
         require_current_device(packed.device, "w")
-    dtype, groups = out_dtype or x.dtype, scales.shape[0]
-    splits = _w4_splits(T, N, groups, rows.get_device()) if T > W4_STREAM_ROWS else 1
-    shares = partials_ok or splits > 1
-    if shares:
-        out = torch.empty(splits, T, N, dtype=torch.float32, device=rows.device)
-    else:
-        out = torch.empty(T, N, dtype=dtype, device=rows.device)
+    dtype = torch.float32 if partials_ok else out_dtype or x.dtype
+    out = torch.empty(T, N, dtype=dtype, device=rows.device)
     lib.call("pyre_w4_linear", rows.data_ptr(), scales.data_ptr(), scales.stride(0), packed.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
-             T, N, groups, splits, _dt(out.dtype), device_error_flag(rows.device).data_ptr(), _stream())
-    if not shares:
-        return out
-    out = PartialSums(out, dtype)
-    return out if partials_ok else materialize(out)
-
-
-W4_STREAM_ROWS = 32      # up to here ``pyre_w4_linear`` shares K within clusters (csrc/gemm_w4.cu: FEW)
-
-
-@functools.lru_cache(maxsize=4096)
-def _w4_splits(T: int, N: int, groups: int, device: int) -> int:
-    return lib.call_value("pyre_w4_splits", T, N, groups)
+             T, N, scales.shape[0], _dt(dtype), device_error_flag(rows.device).data_ptr(), _stream())
+    return PartialSums(out.unsqueeze(0), x.dtype) if partials_ok else out
 
 
 def add_residual(x: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:

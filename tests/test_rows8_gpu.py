@@ -363,7 +363,7 @@ def test_refusals():
         ops.linear(ops.Rows8(x.rows[::2], x.scales[:, ::2].contiguous(), 256), w)
     with pytest.raises(ValueError, match="contiguous"):
         ops.linear(ops.Rows8(x.rows, x.scales.t().contiguous().t(), 256), w)
-    with pytest.raises(ValueError, match="contiguous CUDA"):
+    with pytest.raises(ValueError, match="contiguous CUDA tensors"):
         ops.Weight4(w.packed[::2], w.scales[:, ::2], 256)
     with pytest.raises(ValueError, match="16-byte"):
         ops.Weight4(torch.zeros(128 * 4 + 8, dtype=torch.uint8, device="cuda")[8:].view(4, 128), w.scales[:, :4].contiguous(), 256)
