@@ -312,7 +312,7 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // A warp's part of a tile (32 features from f0 + 32 quarter on, COLS tokens from t0 on) leaves by whole 16-byte pieces, 16 tokens at a time through shared
 // memory (`stage`): single elements (32 stores a thread) took 220 of 1,180 cycles a group where K is 3,584.  Rows off 16-byte boundaries leave by elements.
 template <typename T, int COLS>
-__device__ __forceinline__ void leave(const W4Params& p, float* stage, const uint64_t (&sum)[COLS / 2], int f0, int quarter, int t0, bool vec) {
+__device__ __forceinline__ void leave(const W4Params& p, float* stage, const uint64_t (&sum)[COLS / 2], int f0, int quarter, int t0, int vec) {
     const int lane = threadIdx.x & 31, row = quarter * 32 + lane;
     T* const out = (T*)p.out;
     constexpr int PIECE = 16 / sizeof(T), PIECES = 32 / PIECE, ROWS = 32 / PIECES;      // elements; a warp's features in pieces; rows at a time
@@ -363,10 +363,10 @@ template <int TN> struct Many {
     static_assert(A_COL0 + STAGES * A_COLS <= 512 && TOTAL <= 232448 && TN % 64 == 0 && TN * (FEATURES + 4) * 4 <= SX_OFF, "fits");
 };
 
-// SHARED: the CTAs of a cluster share a tile's K, a tile each; else a CTA takes tile after tile.
+// SHARED: the CTAs of a cluster share a tile's K (`share` groups each), a tile each; else a CTA takes tile after tile.  vec: whole pieces of 16 bytes leave.
 template <int TN, bool SHARED, typename T>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
-w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ W4Params p, int tiles_m, int tiles) {
+w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ W4Params p, int tiles_m, int tiles, int share, int vec) {
     using L = Many<TN>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -379,7 +379,6 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L::BARS + L::N_BARS * 8 + 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int C = SHARED ? (int)cg::this_cluster().num_blocks() : 1, rank = SHARED ? (int)cg::this_cluster().block_rank() : 0;
-    const int first = SHARED ? (int)((long long)rank * p.G / C) : 0, n = SHARED ? (int)((rank + 1ll) * p.G / C) - first : p.G;
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -401,10 +400,12 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const uint32_t tmem = *tmem_slot;
     pdl_trigger();
 
-    int f0, t0;
+    int f0, t0, first, n;
     auto place = [&](int tile) {
         f0 = tile / tiles_m * FEATURES;
         t0 = tile % tiles_m * TN;
+        first = rank * share;      // (the last of many CTAs may have none left)
+        n = min(share, p.G - first);
     };
     if (warp == 0 || warp == 3) {
         if (lane == 0) {
@@ -586,8 +587,7 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             }
             if (!ok) break;
             if (!SHARED) {
-                leave<T, COLS>(p, reinterpret_cast<float*>(gen + L::OUT_OFF) + (warp - EPI_WARP0) * 512, sum, f0, quarter, t0 + col0,
-                               p.N % (16 / sizeof(T)) == 0 && !((uintptr_t)p.out & 15));
+                leave<T, COLS>(p, reinterpret_cast<float*>(gen + L::OUT_OFF) + (warp - EPI_WARP0) * 512, sum, f0, quarter, t0 + col0, vec);
             } else {      // [token][feature], in the rings' place: all that was in them has been used
                 float* const sums = reinterpret_cast<float*>(gen) + col0 * (FEATURES + 4) + row;
 #pragma unroll
@@ -677,8 +677,8 @@ int launch_clusters(void (*kernel)(Args...), dim3 grid, int cluster, int threads
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pyre_pdl_enabled() ? 2 : 1;
+    cfg.attrs = cluster > 1 ? attr : attr + 1;
+    cfg.numAttrs = (cluster > 1) + pyre_pdl_enabled();
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess) return (int)e;
     PYRE_LAUNCH_CHECK();
@@ -697,9 +697,9 @@ int launch_many(const W4Params& p, cudaStream_t stream) {
     const int tiles_m = ceil_div(p.M, TN);
     const long long tiles = (long long)tiles_m * ceil_div(p.N, FEATURES);
     if (tiles > 0x7fffffffll) return PYRE_ERR_UNSUPPORTED;
-    const int i = shares_of(shared_room[dev], tiles, p.G);
-    if (i > 0) return launch_clusters(w4_many_kernel<TN, true, T>, dim3((unsigned)tiles << i), 1 << i, MANY_THREADS, L::TOTAL, stream, mw, mx, p, tiles_m, (int)tiles);
-    return launch_clusters(w4_many_kernel<TN, false, T>, dim3((unsigned)min(tiles, (long long)pyre_sm_count())), 1, MANY_THREADS, L::TOTAL, stream, mw, mx, p, tiles_m, (int)tiles);
+    const int i = shares_of(shared_room[dev], tiles, p.G), share = ceil_div(p.G, 1 << i), vec = p.N % (16 / (int)sizeof(T)) == 0 && !((uintptr_t)p.out & 15);
+    if (i > 0) return launch_clusters(w4_many_kernel<TN, true, T>, dim3((unsigned)tiles << i), 1 << i, MANY_THREADS, L::TOTAL, stream, mw, mx, p, tiles_m, (int)tiles, share, vec);
+    return launch_clusters(w4_many_kernel<TN, false, T>, dim3((unsigned)min(tiles, (long long)pyre_sm_count())), 1, MANY_THREADS, L::TOTAL, stream, mw, mx, p, tiles_m, (int)tiles, share, vec);
 }
 template <int NT, int F, typename T>
 int launch_stream(const W4Params& p, cudaStream_t stream) {
