@@ -4,8 +4,12 @@
 // a feature.  A word of four bytes holds eight elements: byte i element i in its lower half and element i + 4 in its upper one, so that
 // two masks give two words of four bytes in the order in which the rows lie.  Both are padded with zeros to a multiple of 128 elements.
 // The inner sums are exact (32-bit integers: |sum| <= 16 * 8 * 127 * 128 < 2^21, a weight's half byte stays in the upper half of its byte, which
-// makes it sixteen times as large and spares the sign's extension), the outer ones in float, by ascending group in each of a CTA's warps,
-// then over the warps in order.
+// makes it sixteen times as large and spares the sign's extension), the outer ones in float: by ascending group in each of a CTA's sets of warps
+// (one, or two that take the stages in turn), then over the sets and over the CTAs that share a tile's K, in order.
+//
+// Bound: up to some 24 rows the weights' bytes (1 x 3,584 x 37,888 in 13.9 us, 4.9 TB/s of packed weights; 8 x 5,120 x 27,648 15.6), above them each group's
+// conversion and scaling, two operations or three for every sum of 128 products, beside the matrix instructions, which take a tenth to a fifth of the
+// time (2,048 x 3,584 x 37,888 in 546 to 550 us).  Below 10 us what a launch takes to start and to meet shows (1 x 3,584 x 4,608: 4.8 us, its bytes 1.3).
 #include <cooperative_groups.h>
 
 #include "tensor_core.cuh"
@@ -192,6 +196,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         // The feature of a lane among eight: neighbouring lanes of four read rows four apart, whose swizzles are different.
         const int row8 = (quad >> 1) | (quad & 1) << 2;
         float total[NT][2][4] = {};
+        pdl_wait();      // no bounded wait should have to last as long as the kernels before
         for (int i = set; i < steps; i += 2) {
             const int s = i % STREAM_STAGES;
             ok = mbar_wait(full + 8 * s, (i / STREAM_STAGES) & 1, abort_flag, p.err_flag);
@@ -509,6 +514,7 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             place(tile);
             for (int i = 0; i < n && ok; ++i, ++it) {
                 const int s = it % W_STAGES, sa = it % STAGES;
+                if (!waited && it >= min(W_STAGES, STAGES)) { pdl_wait(); waited = true; }      // from here on the copies and the MMAs have to run
                 ok = mbar_wait(w_full + 8 * s, (it / W_STAGES) & 1, abort_flag, p.err_flag);
                 const uint32_t src = base + L::W_OFF + s * W_BYTES + row * 64;      // 64-byte swizzle: a chunk of 16 bytes by bits 7 and 8
                 uint32_t v[16], a[32];
@@ -520,7 +526,6 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 for (int q = 0; q < 16; ++q) { a[2 * q] = lower(v[q]); a[2 * q + 1] = upper(v[q]); }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(w_empty + 8 * s);
-                if (!waited && it >= STAGES) { pdl_wait(); waited = true; }      // from here on the MMAs have to run
                 ok = mbar_wait(ab_empty + 8 * sa, ((it / STAGES) & 1) ^ 1, abort_flag, p.err_flag) && ok;
                 ok = __all_sync(0xffffffffu, ok);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -730,13 +735,15 @@ int launch_few(const W4Params& p, cudaStream_t stream) {
         default: return launch_tiles<4, T>(p, stream);
     }
 }
-constexpr int FEW = 32;      // rows up to here take the stream
+// Rows up to here take the stream.  5,120 x 27,648, us on it / on the tensor cores: 8 rows 15.6 / 32.3, 24 17.6 / 32.3, 32 23.2 / 32.4 (40: 33);
+// 18,944 x 3,584: 16 13.3 / 18.4, 32 19.1 / 18.4.
+constexpr int FEW = 32;
 
 // A warp per group of a feature: s = bf16(max |w| / 7), q = rint(w / s) within -8 .. 7.  A group of zeros (or below 2^-100) has s = 0, one with an
 // infinity or a NaN s = NaN.
 template <typename T>
 __global__ void w4_quantize_kernel(const T* w, long long ld, uint8_t* packed, __nv_bfloat16* scales, int N, int K) {
-    pdl_wait();      // no trigger: a product reads the weight ahead of its own wait
+    pdl_wait();      // no trigger: a product reads the weight ahead of its own wait, which is once all blocks here have ended
     const int G = (K + GROUP - 1) / GROUP, lane = threadIdx.x & 31;
     const long long items = (long long)N * G, step = (long long)gridDim.x * (blockDim.x >> 5);
     for (long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); item < items; item += step) {
@@ -760,6 +767,7 @@ __global__ void w4_quantize_kernel(const T* w, long long ld, uint8_t* packed, __
         if ((lane & 1) == 0) reinterpret_cast<uint32_t*>(packed)[item * (GROUP / 8) + (lane >> 1)] = q | next << 4;
         if (lane == 0) scales[(size_t)g * N + n] = s;
     }
+    __threadfence();
 }
 
 template <typename T>

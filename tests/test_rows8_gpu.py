@@ -202,7 +202,8 @@ def check_product(y, x, w, out_dtype):
 SIZES = [(1, 1, 128), (1, 17, 1), (2, 16, 77), (1, 4608, 3584), (3, 130, 384), (8, 300, 1001), (9, 257, 640), (15, 100, 2176), (17, 48, 512), (31, 999, 256), (33, 640, 1152),
          (64, 129, 384), (65, 200, 896), (127, 384, 128), (128, 128, 1280), (129, 385, 640), (200, 1000, 1001), (300, 515, 2048), (8, 3584, 18944), (16, 64, 18944), (511, 260, 2176),
          (512, 300, 2176), (513, 129, 2048), (700, 515, 2047), (1000, 1, 2560), (640, 2000, 1920), (530, 3999, 4480), (2048, 1000, 3584),
-         (256, 9500, 2048), (257, 9472, 2304), (300, 9001, 2050), (1290, 5000, 2048)]
+         (256, 9500, 2048), (257, 9472, 2304), (300, 9001, 2050), (1290, 5000, 2048),
+         (8, 130, 4224), (40, 130, 4224), (100, 200, 4200), (64, 500, 2700)]      # shares of K of several lengths, of none
 
 
 @pytest.mark.parametrize("T,N,K", SIZES)
@@ -288,6 +289,80 @@ def test_another_stream_and_a_captured_replay(T, K):
             g.replay()
         check_product(graphs[0][1], fv, wv, torch.float32)
         check_product(graphs[1][1], fv, ov, torch.float32)
+
+
+def test_weights_made_just_before_their_product():
+    """A product asks for weights ahead of the kernels before it: one that follows its weight's own kernel finds them whole."""
+    from pyre_b200.kernels import ops
+    N, K = 4000, 2048
+    plain = [normal(71 + i, N, K, dtype=torch.bfloat16) for i in range(4)]
+    for T in (4, 90):
+        x, _ = rows8(70, T, K)
+        want = []
+        for p in plain:
+            w = ops.quantize_weight4(p)
+            torch.cuda.synchronize()
+            want.append(ops.linear(x, w))
+        got = [ops.linear(x, ops.quantize_weight4(p)) for p in plain for _ in range(5)]
+        assert all(torch.equal(y, want[i // 5]) for i, y in enumerate(got))
+        # ... and weights that a plain copy has just put in their place
+        both = [ops.quantize_weight4(p) for p in plain[:2]]
+        w = ops.Weight4(both[0].packed.clone(), both[0].scales.clone(), K)
+        got = []
+        for i in range(10):
+            w.packed.copy_(both[i % 2].packed)
+            w.scales.copy_(both[i % 2].scales)
+            got.append(ops.linear(x, w))
+        assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
+
+
+def test_two_streams_at_once():
+    from pyre_b200.kernels import ops
+    K = 2048
+    cases = [(rows8(81, 6, K)[0], weight(82, 3000, K)[0]), (rows8(83, 200, K)[0], weight(84, 1500, K)[0])]
+    want = [ops.linear(x, w) for x, w in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.linear(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_offsets_beyond_32_bits():
+    """Rows, weights and streams of more than 2^31 elements: the last ones against the same ones alone."""
+    from pyre_b200.kernels import ops
+    T, K, N = 70000, 31000, 24
+    x = torch.empty((T, K), device="cuda")
+    x.normal_(generator=gen(91))
+    gain = 1 + 0.1 * normal(92, K)
+    tail = x[-5:].clone()
+    r, alone = ops.add_rmsnorm_rows8(x, None, gain, 1e-6), ops.add_rmsnorm_rows8(tail, None, gain, 1e-6)
+    assert torch.equal(r.rows[-5:], alone.rows) and torch.equal(r.scales[:, -5:], alone.scales)
+    r, alone = ops.quantize_rows8(x), ops.quantize_rows8(tail)
+    assert torch.equal(r.rows[-5:], alone.rows) and torch.equal(r.scales[:, -5:], alone.scales)
+    del x
+    assert torch.equal(ops.materialize(r)[-5:], ops.materialize(alone))
+    w, wv = weight(93, N, K)
+    check_product(ops.linear(r, w, out_dtype=torch.float32)[-5:], grouped(values(alone)).view(5, -1), wv, torch.float32)
+    del r
+    G, N = -(-K // GROUP), 140000
+    plain = torch.empty((N, K), dtype=torch.bfloat16, device="cuda").normal_(generator=gen(94))
+    w, last = ops.quantize_weight4(plain), ops.quantize_weight4(plain[-40:].clone())
+    del plain
+    assert torch.equal(w.packed[-40:], last.packed) and torch.equal(w.scales[:, -40:], last.scales)
+    assert torch.equal(w.values(torch.bfloat16)[-40:], last.values(torch.bfloat16))
+    wv = grouped(last.values()).view(40, -1)
+    for n in (2, 5):
+        part = ops.Rows8(alone.rows[:n], alone.scales[:, :n], K)
+        check_product(ops.linear(part, w, out_dtype=torch.float32)[:, -40:], grouped(values(alone)).view(5, -1)[:n], wv, torch.float32)
+    many = ops.quantize_rows8(normal(95, 66, K))
+    check_product(ops.linear(many, w, out_dtype=torch.float32)[:, -40:], grouped(values(many)).view(66, -1), wv, torch.float32)
 
 
 def test_a_run_of_them_as_a_layer_uses_them():

@@ -239,6 +239,31 @@ def test_only_some_of_the_arguments_a_replay_and_another_stream():
     assert call(logits[:0], T[:0], seeds[:0], index[:0], k[:0], p[:0], m[:0]).shape == (0,)
 
 
+def test_rows_far_apart_and_two_streams_at_once():
+    """Rows whose offsets pass 32 bits; two streams with rows of their own."""
+    V, step, R = 40000, 1100000000, 3
+    near = torch.randn((R, V), generator=gen(31), device="cuda") * 2
+    far = torch.empty(2 * step + V, device="cuda").as_strided((R, V), (step, 1))
+    far.copy_(near)
+    rule = tuple(t[5:8].contiguous() for t in rules(33, 9))
+    assert torch.equal(call(far, *rule), call(near, *rule))
+    del far
+    many, each = torch.randn((150, V), generator=gen(35), device="cuda") * 2, rules(37, 150)
+    cases = ((near, *rule), (many, *each))
+    want = [call(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(ids, want[i]) for ids in got[i])
+
+
 def test_refusals():
     from pyre_b200.kernels import ops
     logits = torch.zeros((3, 50), device="cuda")
