@@ -125,6 +125,29 @@ def test_gate(T, K, dtype, kind, limit):
     check_rows8(ops.gate_rows8(gu, kind, limit), y)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,K", [(2500, 520), (1301, 1001), (9999, 77), (130, 9472)])
+def test_many_groups_are_as_few(T, K, dtype):
+    """Above some 10,000 groups a warp takes four at a time: the bytes and scales are those of the same rows a few at a time, NaN and zeros included."""
+    from pyre_b200.kernels import ops
+    gu = normal(9, T, 2 * K, dtype=dtype) * 3
+    gu[3, 5], gu[4, 70], gu[5] = float("inf"), float("nan"), 0
+    x = gu[:, :K]
+    live = torch.ones(T, dtype=torch.bool, device="cuda")
+    live[3:5] = False
+    check = ops.quantize_rows8(x[8:].contiguous())
+    check_rows8(check, x[8:].double())
+    for form in (lambda v: ops.quantize_rows8(v[:, :K]), ops.gate_rows8, lambda v: ops.gate_rows8(v, "relu"), lambda v: ops.gate_rows8(v, "clamped", 1.5)):
+        r = form(gu)
+        for a in (0, T // 2, T - 9):
+            few = form(gu[a:a + 9].contiguous())
+            assert torch.equal(r.rows[a:a + 9], few.rows) and torch.equal(r.scales[:, a:a + 9].nan_to_num(-1), few.scales.nan_to_num(-1))
+        assert (r.rows.view(T, -1)[:, K:] == 0).all()
+        v, want = ops.materialize(r), values(r)
+        off = (v.double() - want).abs()
+        assert (off[live] <= want[live].abs() * EPS[dtype] * 1.01).all()      # one product in 32 bits and a rounding
+
+
 def test_groups_of_zeros_and_of_what_is_no_number():
     from pyre_b200.kernels import ops
     x = normal(6, 4, 384)
