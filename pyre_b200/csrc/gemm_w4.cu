@@ -263,11 +263,11 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 //                        is where the MMAs take their A operand from.
 //   warp 1, one thread : four MMAs (kind::i8, 32 k each) a group, into one of two accumulators of 32-bit integers.
 //   warp 2             : the scales of four groups at a time, of features and of tokens, to shared memory.
-//   warps 8..15        : a thread owns a feature and half of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
+//   warps 8 to the last: a thread owns a feature and 32 of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
 //                        feature and added to float sums in registers, by ascending group.
 // Where there are few tiles the CTAs of a cluster share a tile's K, and their sums meet in shared memory.
 // ---------------------------------------------------------------------------
-constexpr int MANY_THREADS = 512, EPI_WARP0 = 8, EPI_WARPS = 8, A_COLS = 32;
+constexpr int EPI_WARP0 = 8, COLS = 32, A_COLS = 32;      // the first warp for the sums, the tokens of such a warp; columns of a group's weights
 constexpr int W_STAGES = 6, STAGES = 6;               // packed weights; both operands of the MMAs
 constexpr int BATCH = 4, S_STAGES = 2;                // groups whose scales come at a time
 
@@ -314,65 +314,51 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     return v;
 }
 
-// A warp's part of a tile (32 features from f0 + 32 quarter on, COLS tokens from t0 on) leaves by whole 16-byte pieces, 16 tokens at a time through shared
-// memory (`stage`): single elements (32 stores a thread) took 220 of 1,180 cycles a group where K is 3,584.  Rows off 16-byte boundaries leave by elements.
-template <typename T, int COLS>
-__device__ __forceinline__ void leave(const W4Params& p, float* stage, const uint64_t (&sum)[COLS / 2], int f0, int quarter, int t0, int vec) {
-    const int lane = threadIdx.x & 31, row = quarter * 32 + lane;
-    T* const out = (T*)p.out;
-    constexpr int PIECE = 16 / sizeof(T), PIECES = 32 / PIECE, ROWS = 32 / PIECES;      // elements; a warp's features in pieces; rows at a time
-    const int left = p.M - t0;
+// A warp's part of a tile (32 features from f on, COLS tokens from t0 on) leaves from shared memory (`stage`, [token][feature]) by a copy of its own, so that
+// the warp goes on with its next tile.  (By pieces of 16 bytes, stored by the warp itself, a tile took 3,100 cycles in which no sums were taken: 2,048 x
+// 3,584 x 37,888 506 us.)  Rows off 16-byte boundaries leave by elements.
+template <typename T>
+__device__ __forceinline__ void leave(const W4Params& p, const CUtensorMap* map, T* stage, const uint64_t (&sum)[COLS / 2], int f, int t0, int vec) {
+    const int lane = threadIdx.x & 31;
+    if (vec) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the tile before has left
+        __syncwarp();
 #pragma unroll
-    for (int c = 0; c < COLS; c += 16) {
-        if (vec) {
-            __syncwarp();
-#pragma unroll
-            for (int q = 0; q < 16; q += 2) {
-                stage[q * 32 + lane] = __uint_as_float((uint32_t)sum[(c + q) / 2]);
-                stage[(q + 1) * 32 + lane] = __uint_as_float((uint32_t)(sum[(c + q) / 2] >> 32));
-            }
-            __syncwarp();
-            const int f = f0 + quarter * 32 + lane % PIECES * PIECE;
-#pragma unroll
-            for (int t = lane / PIECES; t < 16; t += ROWS) {
-                Vec<T, PIECE> v;
-#pragma unroll
-                for (int k = 0; k < PIECE; k += 4) {
-                    const float4 a = *reinterpret_cast<const float4*>(stage + t * 32 + lane % PIECES * PIECE + k);
-                    v.v[k] = from_f32<T>(a.x);
-                    v.v[k + 1] = from_f32<T>(a.y);
-                    v.v[k + 2] = from_f32<T>(a.z);
-                    v.v[k + 3] = from_f32<T>(a.w);
-                }
-                if (c + t < left && f < p.N) store_vec<T, PIECE>(out + (size_t)(t0 + c + t) * p.N + f, v);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                const uint32_t bits = q & 1 ? (uint32_t)(sum[(c + q) / 2] >> 32) : (uint32_t)sum[(c + q) / 2];
-                if (c + q < left && f0 + row < p.N) ElemOps<T>::store(out + (size_t)(t0 + c + q) * p.N + f0 + row, __uint_as_float(bits));
-            }
+        for (int q = 0; q < COLS; ++q) stage[q * 32 + lane] = from_f32<T>(__uint_as_float((uint32_t)(sum[q / 2] >> (q & 1 ? 32 : 0))));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0 && f < p.N && t0 < p.M) {      // (what lies beyond the matrix is left out by the copy)
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                         ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(stage)), "r"(f), "r"(t0) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
+    } else {
+        T* const out = (T*)p.out + (size_t)t0 * p.N + f + lane;
+#pragma unroll
+        for (int q = 0; q < COLS; ++q)
+            if (q < p.M - t0 && f + lane < p.N) ElemOps<T>::store(out + (size_t)q * p.N, __uint_as_float((uint32_t)(sum[q / 2] >> (q & 1 ? 32 : 0))));
     }
 }
 
-template <int TN> struct Many {
+template <int TN, typename T> struct Many {
+    static constexpr int EPI_WARPS = 4 * TN / COLS, THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
     static constexpr int X_BYTES = TN * GROUP;
     static constexpr int W_OFF = 0, X_OFF = W_STAGES * W_BYTES;
     static constexpr int SX_OFF = X_OFF + STAGES * X_BYTES, SW_OFF = SX_OFF + S_STAGES * BATCH * TN * 4;      // [stage][group][token], [..][feature]
-    static constexpr int OUT_OFF = SW_OFF + S_STAGES * BATCH * FEATURES * 4;      // [warp][16 tokens][32 features] floats
-    static constexpr int BARS = OUT_OFF + EPI_WARPS * 512 * 4;
+    static constexpr int OUT_OFF = SW_OFF + S_STAGES * BATCH * FEATURES * 4;      // [warp][token][32 features]
+    static constexpr int BARS = OUT_OFF + EPI_WARPS * COLS * 32 * (int)sizeof(T);
     static constexpr int N_BARS = 2 * (W_STAGES + STAGES + S_STAGES + 2) + 1;
     static constexpr int TOTAL = BARS + N_BARS * 8 + 24 + 1024;
     static constexpr int A_COL0 = 2 * TN;
-    static_assert(A_COL0 + STAGES * A_COLS <= 512 && TOTAL <= 232448 && TN % 64 == 0 && TN * (FEATURES + 4) * 4 <= SX_OFF, "fits");
+    static_assert(A_COL0 + STAGES * A_COLS <= 512 && TOTAL <= 232448 && TN % 64 == 0 && TN * (FEATURES + 4) * 4 <= SX_OFF && OUT_OFF % 128 == 0, "fits");
 };
 
 // SHARED: the CTAs of a cluster share a tile's K (`share` groups each), a tile each; else a CTA takes tile after tile.  vec: whole pieces of 16 bytes leave.
 template <int TN, bool SHARED, typename T>
-__global__ void __launch_bounds__(MANY_THREADS, 1)
-w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ W4Params p, int tiles_m, int tiles, int share, int vec) {
-    using L = Many<TN>;
+__global__ void __launch_bounds__(Many<TN, T>::THREADS, 1)
+w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out, const __grid_constant__ W4Params p, int tiles_m, int tiles, int share, int vec) {
+    using L = Many<TN, T>;
+    constexpr int EPI_WARPS = L::EPI_WARPS;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
@@ -539,8 +525,6 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         }
         if (!waited) pdl_wait();
     } else {
-        constexpr int COLS = TN / 2;
-        static_assert(EPI_WARPS == 8 && COLS % 16 == 0, "two warps side by side, whole loads from tensor memory");
         const int quarter = warp & 3, row = quarter * 32 + lane, col0 = ((warp - EPI_WARP0) >> 2) * COLS;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         pdl_wait();
@@ -592,13 +576,14 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             }
             if (!ok) break;
             if (!SHARED) {
-                leave<T, COLS>(p, reinterpret_cast<float*>(gen + L::OUT_OFF) + (warp - EPI_WARP0) * 512, sum, f0, quarter, t0 + col0, vec);
+                leave<T>(p, &map_out, reinterpret_cast<T*>(gen + L::OUT_OFF) + (warp - EPI_WARP0) * COLS * 32, sum, f0 + quarter * 32, t0 + col0, vec);
             } else {      // [token][feature], in the rings' place: all that was in them has been used
                 float* const sums = reinterpret_cast<float*>(gen) + col0 * (FEATURES + 4) + row;
 #pragma unroll
                 for (int q = 0; q < COLS; ++q) sums[q * (FEATURES + 4)] = __uint_as_float((uint32_t)(sum[q / 2] >> (q & 1 ? 32 : 0)));
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -634,6 +619,18 @@ bool byte_map(CUtensorMap* map, const void* p, int rows, long long pitch, int wi
     cuuint32_t box[2] = {(cuuint32_t)wide, (cuuint32_t)high}, elem[2] = {1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
               wide == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A map of results [rows][n] in boxes of `high` rows of 32.
+template <typename T>
+bool result_map(CUtensorMap* map, void* p, int rows, int n, int high) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)n, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)n * sizeof(T)};
+    cuuint32_t box[2] = {32, (cuuint32_t)high}, elem[2] = {1, 1};
+    return fn(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p, dims, strides, box, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Clusters of `kernel` that find room at once, by their CTAs' number's logarithm (a cluster needs its CTAs on neighbouring SMs; the driver knows how many there
@@ -691,11 +688,11 @@ int launch_clusters(void (*kernel)(Args...), dim3 grid, int cluster, int threads
 }
 template <int TN, typename T>
 int launch_many(const W4Params& p, cudaStream_t stream) {
-    using L = Many<TN>;
+    using L = Many<TN, T>;
     static Room shared_room[PYRE_MAX_DEVICES] = {}, room[PYRE_MAX_DEVICES] = {};
     const int dev = pyre_current_device();
-    cudaError_t e = find_room(w4_many_kernel<TN, true, T>, MANY_THREADS, L::TOTAL, shared_room[dev]);
-    if (e == cudaSuccess) e = find_room(w4_many_kernel<TN, false, T>, MANY_THREADS, L::TOTAL, room[dev]);
+    cudaError_t e = find_room(w4_many_kernel<TN, true, T>, L::THREADS, L::TOTAL, shared_room[dev]);
+    if (e == cudaSuccess) e = find_room(w4_many_kernel<TN, false, T>, L::THREADS, L::TOTAL, room[dev]);
     if (e != cudaSuccess) return (int)e;
     CUtensorMap mw, mx;
     if (!byte_map(&mw, p.packed, p.N, 64ll * p.G, 64, FEATURES) || !byte_map(&mx, p.rows, p.M, 128ll * p.G, 128, TN)) return PYRE_ERR_BAD_ARG;
@@ -703,8 +700,10 @@ int launch_many(const W4Params& p, cudaStream_t stream) {
     const long long tiles = (long long)tiles_m * ceil_div(p.N, FEATURES);
     if (tiles > 0x7fffffffll) return PYRE_ERR_UNSUPPORTED;
     const int i = shares_of(shared_room[dev], tiles, p.G), share = ceil_div(p.G, 1 << i), vec = p.N % (16 / (int)sizeof(T)) == 0 && !((uintptr_t)p.out & 15);
-    if (i > 0) return launch_clusters(w4_many_kernel<TN, true, T>, dim3((unsigned)tiles << i), 1 << i, MANY_THREADS, L::TOTAL, stream, mw, mx, p, tiles_m, (int)tiles, share, vec);
-    return launch_clusters(w4_many_kernel<TN, false, T>, dim3((unsigned)min(tiles, (long long)pyre_sm_count())), 1, MANY_THREADS, L::TOTAL, stream, mw, mx, p, tiles_m, (int)tiles, share, vec);
+    CUtensorMap mo = {};      // (only the copies of whole tiles use it)
+    if (i == 0 && vec && !result_map<T>(&mo, p.out, p.M, p.N, COLS)) return PYRE_ERR_BAD_ARG;
+    if (i > 0) return launch_clusters(w4_many_kernel<TN, true, T>, dim3((unsigned)tiles << i), 1 << i, L::THREADS, L::TOTAL, stream, mw, mx, mo, p, tiles_m, (int)tiles, share, vec);
+    return launch_clusters(w4_many_kernel<TN, false, T>, dim3((unsigned)min(tiles, (long long)pyre_sm_count())), 1, L::THREADS, L::TOTAL, stream, mw, mx, mo, p, tiles_m, (int)tiles, share, vec);
 }
 template <int NT, int F, typename T>
 int launch_stream(const W4Params& p, cudaStream_t stream) {
