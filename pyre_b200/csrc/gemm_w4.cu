@@ -9,7 +9,7 @@
 //
 // Bound: up to some 24 rows the weights' bytes (1 x 3,584 x 37,888 in 13.9 us, 4.9 TB/s of packed weights; 8 x 5,120 x 27,648 15.6), above them each group's
 // conversion and scaling, two operations or three for every sum of 128 products, beside the matrix instructions, which take a tenth to a fifth of the
-// time (2,048 x 3,584 x 37,888 in 546 to 550 us).  Below 10 us what a launch takes to start and to meet shows (1 x 3,584 x 4,608: 4.8 us, its bytes 1.3).
+// time (2,048 x 3,584 x 37,888 in 483 us).  Below 10 us what a launch takes to start and to meet shows (1 x 3,584 x 4,608: 4.8 us, its bytes 1.3).
 #include <cooperative_groups.h>
 
 #include "tensor_core.cuh"
@@ -266,6 +266,9 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 //   warps 8 to the last: a thread owns a feature and 32 of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
 //                        feature and added to float sums in registers, by ascending group.
 // Where there are few tiles the CTAs of a cluster share a tile's K, and their sums meet in shared memory.
+// Bound by the last warps: of 483 us for 2,048 x 3,584 x 37,888 some 200 go with the conversions, products and additions (with a quarter of them it takes 349), 48 with
+// the reads of the tokens' scales; a quarter of the MMAs or no unpacking changes nothing.  Four warps for 128 tokens took 574 us, eight 550, sixteen 506 (then the
+// tiles' copies); a third accumulator 514; sums by the MMAs' own fragments (half as many reads of scales) 508.
 // ---------------------------------------------------------------------------
 constexpr int EPI_WARP0 = 8, COLS = 32, A_COLS = 32;      // the first warp for the sums, the tokens of such a warp; columns of a group's weights
 constexpr int W_STAGES = 6, STAGES = 6;               // packed weights; both operands of the MMAs
@@ -734,8 +737,8 @@ int launch_few(const W4Params& p, cudaStream_t stream) {
         default: return launch_tiles<4, T>(p, stream);
     }
 }
-// Rows up to here take the stream.  5,120 x 27,648, us on it / on the tensor cores: 8 rows 15.6 / 32.3, 24 17.6 / 32.3, 32 23.2 / 32.4 (40: 33);
-// 18,944 x 3,584: 16 13.3 / 18.4, 32 19.1 / 18.4.
+// Rows up to here take the stream.  5,120 x 27,648, us on it / on the tensor cores: 8 rows 15.8 / 31.7, 24 18.1 / 31.6, 32 23.7 / 31.7;
+// 18,944 x 3,584: 16 13.5 / 18.9, 32 19.3 / 19.1; 3,584 x 3,584: 8 5.8 / 7.4.
 constexpr int FEW = 32;
 
 // A warp per group of a feature: s = bf16(max |w| / 7), q = rint(w / s) within -8 .. 7.  A group of zeros (or below 2^-100) has s = 0, one with an
@@ -817,6 +820,7 @@ PYRE_API int pyre_w4_linear(const void* rows, const float* row_scales, long long
     if (dtype != PYRE_F32 && dtype != PYRE_BF16) return PYRE_ERR_BAD_ARG;
     const W4Params p = {(const uint8_t*)rows, row_scales, ld_scales, (const uint8_t*)packed, (const __nv_bfloat16*)scales, out, M, N, G, err_flag};
     if (M <= FEW) return dtype == PYRE_F32 ? launch_few<float>(p, stream) : launch_few<__nv_bfloat16>(p, stream);
+    // tiles of 64 tokens / 128, us: 64 x 3,584 x 37,888 24.8 / 34.3, 64 x 3,584 x 3,584 8.0 / 9.9; 128 x 3,584 x 37,888 44.9 / 34.9, 128 x 18,944 x 3,584 32.2 / 27.4
     if (M <= 64) return dtype == PYRE_F32 ? launch_many<64, float>(p, stream) : launch_many<64, __nv_bfloat16>(p, stream);
     return dtype == PYRE_F32 ? launch_many<128, float>(p, stream) : launch_many<128, __nv_bfloat16>(p, stream);
 }
