@@ -110,6 +110,35 @@ def test_rows_off_every_boundary():
     check_rows8(ops.quantize_rows8(wide[:, 3:H]), wide[:, 3:H].double())
 
 
+def test_the_same_row_several_times_and_a_captured_norm():
+    from pyre_b200.kernels import ops
+    T, H = 6, 1100
+    x, d, w = normal(11, T, H), normal(12, T, H, dtype=torch.bfloat16), 1 + 0.1 * normal(13, H)
+    before = x.clone()
+    rows = torch.tensor([5, 0, 5, 5, 2, 2, 1, 5, 3], dtype=torch.int32, device="cuda")
+    v = (x.double() + d.double())[rows.long()]
+    check_rows8(ops.add_rmsnorm_rows8(x, d, w, 1e-6, rows=rows), v / torch.sqrt((v * v).mean(dim=1, keepdim=True) + 1e-6) * w.double())
+    assert torch.equal(x, before)      # rows may name one twice: nothing is added to the stream
+    graphs = []
+    for size in (T, 3):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            r = ops.add_rmsnorm_rows8(x[:size], d[:size], w, 1e-6)
+            values_ = ops.materialize(r)
+            gate = ops.gate_rows8(values_)
+        graphs.append((g, size, r, values_, gate))
+    v = before.double()
+    for i in (0, 1, 0, 1):
+        g, size, r, values_, gate = graphs[i]
+        g.replay()
+        v[:size] = (v[:size].float() + d[:size].float()).double()
+        assert torch.equal(x.double(), v)
+        y = v[:size]
+        check_rows8(r, y / torch.sqrt((y * y).mean(dim=1, keepdim=True) + 1e-6) * w.double())
+        a, u = values_.double().split(H // 2, dim=1)
+        check_rows8(gate, a / (1 + torch.exp(-a)) * u)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("T,K", [(1, 128), (4, 200), (3, 77), (65, 1024)])
 @pytest.mark.parametrize("kind,limit", [("silu", 0.0), ("relu", 0.0), ("clamped", 1.5)])

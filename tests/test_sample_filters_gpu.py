@@ -197,6 +197,26 @@ def test_any_number_of_ctas_per_row_gives_the_same(form, monkeypatch):
         assert torch.equal(ids, want), cluster
 
 
+@pytest.mark.parametrize("form", ["normal", "flat", "equal", "ends"])
+def test_long_rows_on_few_ctas(form, monkeypatch):
+    """More blocks of 128 entries than a CTA, or a row's first CTA, keeps the largest entries of."""
+    from pyre_b200.kernels import ops
+    R, V = 9, 700003
+    logits = torch.randn((R, V), generator=gen(78), device="cuda") * {"normal": 2, "flat": 0.01, "equal": 0, "ends": 0.5}[form]
+    if form == "ends":
+        logits[:, -30:] += 9
+        logits[:, :5] += 9
+    rule = rules(124, R)
+    want = None
+    for cluster in (1, 2, 4, 0):
+        monkeypatch.setattr(ops, "_SAMPLE_CLUSTER", cluster)
+        ids = call(logits, *rule)
+        if want is None:
+            check(ids, logits, *rule)
+            want = ids
+        assert torch.equal(ids, want), cluster
+
+
 def test_draws_follow_the_distribution():
     """Many draws of one row: frequencies against the renormalised probabilities of the kept tokens.  4,096 draws; a count's deviation is at most
     sqrt(n / 4) = 32, so five of them bound each of the few counts with a chance of error below 1e-5."""
