@@ -636,10 +636,11 @@ bool result_map(CUtensorMap* map, void* p, int rows, int n, int high) {
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Clusters of `kernel` that find room at once, by their CTAs' number's logarithm (a cluster needs its CTAs on neighbouring SMs; the driver knows how many there
+// Clusters of `kernel` that find room at once, by the number of their CTAs (a cluster needs its CTAs on neighbouring SMs; the driver knows how many there
 // are room for).  Worked out once per kernel and device.
+constexpr int MOST_SHARES = 8;
 struct Room {
-    int known, clusters[4];
+    int known, clusters[MOST_SHARES + 1];
 };
 template <typename... Args>
 cudaError_t find_room(void (*kernel)(Args...), int threads, int bytes, Room& room) {
@@ -654,20 +655,22 @@ cudaError_t find_room(void (*kernel)(Args...), int threads, int bytes, Room& roo
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    for (int i = 1; i < 4; ++i) {
-        attr.val.clusterDim.x = 1 << i;
-        cfg.gridDim = dim3(1 << i);
-        e = cudaOccupancyMaxActiveClusters(&room.clusters[i], kernel, &cfg);
+    for (int c = 2; c <= MOST_SHARES; ++c) {
+        attr.val.clusterDim.x = c;
+        cfg.gridDim = dim3(c);
+        e = cudaOccupancyMaxActiveClusters(&room.clusters[c], kernel, &cfg);
         if (e != cudaSuccess) return e;
     }
     room.known = 1;
     return cudaSuccess;
 }
-// The logarithm of the number of CTAs that share a tile's K: as many as find room, each with four groups at least.
+// CTAs that share a tile's K: as many as find room, each with four groups at least.  Two, four or eight where two CTAs are on an SM (16 x 5,120 x 7,168: 4 of
+// them 8.9 us, 5 12.2; 8 x 3,584 x 4,608: 4 5.9, 7 6.7), any number where one is (64 x 5,120 x 5,120: 3 11.3, 2 12.5; 128 x 5,120 x 2,560: as many as there is room for 11.6, 4 12.2).
+template <bool TWOS>
 int shares_of(const Room& room, long long tiles, int G) {
-    int i = 3;
-    while (i > 0 && (tiles > room.clusters[i] || G < 4 << i)) --i;
-    return i;
+    int c = MOST_SHARES;
+    while (c > 1 && (tiles > room.clusters[c] || G < 4 * c)) c = TWOS ? c / 2 : c - 1;
+    return c;
 }
 template <typename... Args>
 int launch_clusters(void (*kernel)(Args...), dim3 grid, int cluster, int threads, int bytes, cudaStream_t stream, Args... args) {
@@ -702,10 +705,10 @@ int launch_many(const W4Params& p, cudaStream_t stream) {
     const int tiles_m = ceil_div(p.M, TN);
     const long long tiles = (long long)tiles_m * ceil_div(p.N, FEATURES);
     if (tiles > 0x7fffffffll) return PYRE_ERR_UNSUPPORTED;
-    const int i = shares_of(shared_room[dev], tiles, p.G), share = ceil_div(p.G, 1 << i), vec = p.N % (16 / (int)sizeof(T)) == 0 && !((uintptr_t)p.out & 15);
+    const int C = shares_of<false>(shared_room[dev], tiles, p.G), share = ceil_div(p.G, C), vec = p.N % (16 / (int)sizeof(T)) == 0 && !((uintptr_t)p.out & 15);
     CUtensorMap mo = {};      // (only the copies of whole tiles use it)
-    if (i == 0 && vec && !result_map<T>(&mo, p.out, p.M, p.N, COLS)) return PYRE_ERR_BAD_ARG;
-    if (i > 0) return launch_clusters(w4_many_kernel<TN, true, T>, dim3((unsigned)tiles << i), 1 << i, L::THREADS, L::TOTAL, stream, mw, mx, mo, p, tiles_m, (int)tiles, share, vec);
+    if (C == 1 && vec && !result_map<T>(&mo, p.out, p.M, p.N, COLS)) return PYRE_ERR_BAD_ARG;
+    if (C > 1) return launch_clusters(w4_many_kernel<TN, true, T>, dim3((unsigned)(tiles * C)), C, L::THREADS, L::TOTAL, stream, mw, mx, mo, p, tiles_m, (int)tiles, share, vec);
     return launch_clusters(w4_many_kernel<TN, false, T>, dim3((unsigned)min(tiles, (long long)pyre_sm_count())), 1, L::THREADS, L::TOTAL, stream, mw, mx, mo, p, tiles_m, (int)tiles, share, vec);
 }
 template <int NT, int F, typename T>
@@ -717,8 +720,8 @@ int launch_stream(const W4Params& p, cudaStream_t stream) {
     if (e != cudaSuccess) return (int)e;
     CUtensorMap mw, mx;
     if (!byte_map(&mw, p.packed, p.N, 64ll * p.G, 128, F) || !byte_map(&mx, p.rows, p.M, 128ll * p.G, 128, NT * 8)) return PYRE_ERR_BAD_ARG;
-    const int i = shares_of(room[dev], (long long)tiles * rows, p.G);
-    return launch_clusters(w4_stream_kernel<NT, F, T>, dim3((unsigned)tiles << i, (unsigned)rows), 1 << i, L::THREADS, L::TOTAL, stream, mw, mx, p);
+    const int C = shares_of<true>(room[dev], (long long)tiles * rows, p.G);
+    return launch_clusters(w4_stream_kernel<NT, F, T>, dim3((unsigned)(tiles * C), (unsigned)rows), C, L::THREADS, L::TOTAL, stream, mw, mx, p);
 }
 // Tiles of 96 features where those of 128 would leave an SM more of them: 24 x 5,120 x 27,648 (216 tiles, two on some SMs, or 288) 18.1 us against 22.3.
 template <int NT, typename T>
