@@ -1027,10 +1027,12 @@ PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float
     if (n_rows <= 0) return 0;
     if (V <= 0 || (temperature && (!seeds || !token_index))) return PYRE_ERR_BAD_ARG;
     if (cluster < 0 || cluster > MAX_CLUSTER || (cluster & (cluster - 1))) return PYRE_ERR_BAD_ARG;
-    // CTAs per row: as many as find room, two to an SM.  152,064 entries, us on 1 / 2 / 4 / 8 CTAs a row: 1 row, k 22 / 16 / 13 / 12 (16 CTAs: 11); 64 rows,
-    // k 40 / 29 / 23 / 58, p 234 / 133 / 82 / 140; 256 rows, k 49 / 59 / 73 / 192, p 316 / 251 / 244 / 503.
-    int C = cluster > 0 ? cluster : 1;
-    while (!cluster && C < MAX_CLUSTER && n_rows * 2ll * C <= 2 * pyre_sm_count() && V > 2048 * C) C *= 2;
+    // CTAs per row.  152,064 entries, us on 1 / 2 / 4 / 8 / 16 CTAs a row: 1 row, k 22 / 16 / 13 / 12 / 11; 12 rows, k 17 / 15 / 14 for 4 / 8 / 16, p alone
+    // 65 / 40 / 32; 16 rows, k 18 / 21 / 22, p 67 / 50 / 44; 32 rows, k 27 / 21 / 35 / 35 for 2 / 4 / 8 / 16, p 123 / 75 / 79 / 69, rows of all kinds
+    // 102 / 61 / 49 / 40; 64 rows, k 40 / 29 / 23 / 58 for 1 / 2 / 4 / 8, p 234 / 133 / 82 / 140; 256 rows, k 49 / 59 / 73 / 192, p 316 / 251 / 244 / 503.
+    const int sms = pyre_sm_count();
+    int C = cluster > 0 ? cluster : n_rows <= (top_p ? sms / 4 : sms / 12) ? MAX_CLUSTER : n_rows <= sms / 2 ? 4 : n_rows <= sms ? 2 : 1;
+    while (!cluster && C > 1 && V <= 1024 * C) C /= 2;
     FilterParams p = {logits, ld, temperature, seeds, token_index, top_k, top_p, min_p, out, V, (ceil_div(V, C) + 3) / 4 * 4, 0};
     constexpr int RESIDENT = 77 * 1024;      // two CTAs on an SM
     size_t bytes = (size_t)p.slice * 4 + 16;

@@ -45,24 +45,22 @@ class Sampler:
             ids = ops.sample(logits)
         else:
             seeds = np.asarray([p.seed & 0x7FFFFFFFFFFFFFFF for p in params], dtype=np.int64)
-            filters = any(p.filters for p in params)
-            small = np.empty((5 if filters else 2, R), dtype=np.int32)
+            # only the filters that some row has: the kernel has less to look for
+            drawn = [p for p in params if p.temperature > 0.0]
+            filters = [name for name, off in (("top_k", 0), ("top_p", 1.0), ("min_p", 0.0)) if any(getattr(p, name) != off for p in drawn)]
+            small = np.empty((2 + len(filters), R), dtype=np.int32)
             small[0] = np.asarray([p.temperature for p in params], dtype=np.float32).view(np.int32)
             small[1] = np.asarray(token_index, dtype=np.int32)
-            if filters:
-                small[2] = np.asarray([p.top_k for p in params], dtype=np.int32)
-                small[3] = np.asarray([p.top_p for p in params], dtype=np.float32).view(np.int32)
-                small[4] = np.asarray([p.min_p for p in params], dtype=np.float32).view(np.int32)
+            for i, name in enumerate(filters):
+                values = [getattr(p, name) for p in params]
+                small[2 + i] = np.asarray(values, dtype=np.int32) if name == "top_k" else np.asarray(values, dtype=np.float32).view(np.int32)
             seeds_dev = torch.from_numpy(seeds).to(self.device)
             small_dev = torch.from_numpy(small).to(self.device)
             temperature = small_dev[0].view(torch.float32)
             self.bytes_uploaded += seeds.nbytes + small.nbytes
             tix = small_dev[1]
-            if filters:
-                ids = ops.sample(logits, temperature, seeds_dev, tix, top_k=small_dev[2], top_p=small_dev[3].view(torch.float32),
-                                 min_p=small_dev[4].view(torch.float32))
-            else:
-                ids = ops.sample(logits, temperature, seeds_dev, tix)
+            ids = ops.sample(logits, temperature, seeds_dev, tix, **{name: small_dev[2 + i] if name == "top_k" else small_dev[2 + i].view(torch.float32)
+                                                                     for i, name in enumerate(filters)})
         self.bytes_downloaded += R * 4
         i = self._turn
         self._turn ^= 1
