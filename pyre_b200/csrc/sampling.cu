@@ -999,20 +999,30 @@ sample_filtered_kernel(const FilterParams p) {
     auto put = [&](unsigned at, float, int i) {
         if (at < GATHERED) sh.gathered[at] = i;
     };
+    // A round takes as many blocks as the list is sure to hold (all, if they are but twice as many), the next ones as many as the last round's share of entries
+    // lets expect; what does not fit after all is taken again.  256 rows of 152,064, min_p 89 us with rounds of one size, 59 with these.  (Dense rows as
+    // they lie, not gathered: 358 us against 341 where 90,000 of each row stay.)
     constexpr int ROUND = GATHERED / 128 - 1;      // blocks, and the ends
-    for (int from = 0; from == 0 || from < s.all_blocks(); from += ROUND) {
+    const int all = s.all_blocks();
+    for (int from = 0, span = all <= 2 * ROUND ? max(all, 1) : ROUND; from == 0 || from < all;) {
         __syncthreads();
         if (tid == 0) sh.n_gathered = 0;
         __syncthreads();
-        s.pick(from, min(s.all_blocks(), from + ROUND), least, INFINITY, &sh.n_gathered, put);
+        s.pick(from, min(all, from + span), least, INFINITY, &sh.n_gathered, put);
         if (from == 0) s.pick_ends(least, INFINITY, &sh.n_gathered, put);
         __syncthreads();
-        const int count = min((int)sh.n_gathered, GATHERED);
+        const int count = (int)sh.n_gathered;
+        if (count > GATHERED) {
+            span = ROUND;
+            continue;
+        }
         for (int q = tid; q < count; q += F_THREADS) {
             const int i = sh.gathered[q];
             const float l = s.held[i];
             if (s.composite(l, i) >= border) score(l, begin + i);
         }
+        from += span;
+        span = max(ROUND, (int)min((long long)all, (long long)span * (GATHERED * 3 / 4) / max(count, 1)));
     }
     finish(best);
 }

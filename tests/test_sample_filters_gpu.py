@@ -217,6 +217,21 @@ def test_long_rows_on_few_ctas(form, monkeypatch):
         assert torch.equal(ids, want), cluster
 
 
+@pytest.mark.parametrize("V", [11000, 150001])
+def test_entries_that_stay_lie_in_one_end_of_a_row(V, monkeypatch):
+    """The share of a row's first entries that stay says nothing about the others."""
+    from pyre_b200.kernels import ops
+    R = 18
+    logits = torch.randn((R, V), generator=gen(79), device="cuda") * 0.01
+    logits[::2, :V * 2 // 3] -= 40
+    logits[1::2, V // 3:] -= 40
+    logits[::2, 100] = 0.5
+    rule = rules(125, R)
+    for cluster in (1, 2, 0):
+        monkeypatch.setattr(ops, "_SAMPLE_CLUSTER", cluster)
+        check(call(logits, *rule), logits, *rule)
+
+
 def test_draws_follow_the_distribution():
     """Many draws of one row: frequencies against the renormalised probabilities of the kept tokens.  4,096 draws; a count's deviation is at most
     sqrt(n / 4) = 32, so five of them bound each of the few counts with a chance of error below 1e-5."""
