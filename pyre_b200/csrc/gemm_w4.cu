@@ -8,7 +8,7 @@
 // (one, or two that take the stages in turn), then over the sets and over the CTAs that share a tile's K, in order.
 //
 // Bound: up to some 24 rows the weights' bytes (1 x 3,584 x 37,888 in 13.9 us, 4.9 TB/s of packed weights; 8 x 5,120 x 27,648 15.6), above them each group's
-// conversion and scaling, two operations or three for every sum of 128 products, beside the matrix instructions, which take a tenth to a fifth of the
+// conversion and scaling, two operations or three for every sum of 128 products, beside the matrix instructions, which take an eighth to a third of the
 // time (2,048 x 3,584 x 37,888 in 483 us).  Below 10 us what a launch takes to start and to meet shows (1 x 3,584 x 4,608: 4.8 us, its bytes 1.3).
 #include <cooperative_groups.h>
 
