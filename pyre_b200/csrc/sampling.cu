@@ -922,6 +922,7 @@ sample_filtered_kernel(const FilterParams p) {
                                 from = min(from, sh.warp_u64[0][w]);
                                 to = max(to, sh.warp_u64[1][w]);
                             }
+                            __syncthreads();      // the warps' counts take the same places
                         } else {
                             from = 0;
                             to = ~0ull;
