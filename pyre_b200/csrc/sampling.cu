@@ -51,11 +51,12 @@ __global__ void sample_kernel(const float* logits, long long ld, const float* te
     const unsigned long long seed = seeds ? seeds[r] : 0ull;
     const unsigned int tix = token_index ? (unsigned int)token_index[r] : 0u;
 
-    Best best{-INFINITY, 0x7fffffff};
+    // (a NaN is above nothing: it counts as -inf)
+    Best best{-INFINITY, (int)threadIdx.x < V ? (int)threadIdx.x : 0x7fffffff};
     for (int v = threadIdx.x; v < V; v += blockDim.x) {
         float s = row[v];
         if (!greedy) s = __fadd_rn(__fmul_rn(s, inv_t), gumbel(seed, tix, (unsigned int)v));
-        if (s > best.score || best.index == 0x7fffffff) best = Best{s, v};
+        if (s > best.score) best = Best{s, v};
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -94,11 +95,11 @@ __global__ void sample_slices_kernel(const float* logits, long long ld, const fl
     const unsigned long long seed = seeds ? seeds[r] : 0ull;
     const unsigned int tix = token_index ? (unsigned int)token_index[r] : 0u;
     const int begin = sl * slice, end = min(begin + slice, V);
-    Best best{-INFINITY, 0x7fffffff};
+    Best best{-INFINITY, begin + (int)threadIdx.x < end ? begin + (int)threadIdx.x : 0x7fffffff};
     for (int v = begin + threadIdx.x; v < end; v += blockDim.x) {
         float s = row[v];
         if (!greedy) s = __fadd_rn(__fmul_rn(s, inv_t), gumbel(seed, tix, (unsigned int)v));
-        if (s > best.score || best.index == 0x7fffffff) best = Best{s, v};
+        if (s > best.score) best = Best{s, v};
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
