@@ -177,7 +177,7 @@ PYRE_API int pyre_sample(const float* logits, long long ld, const float* tempera
 // All three keep a prefix of the order.  The token is argmax over it of (l_i - max l) / T + g(seed, index, i), the noise of the kernels
 // above.  A row without a filter is chosen from as above, bit for bit; a NaN counts as -inf.
 //
-// A cluster of CTAs shares a row; each keeps its slice in shared memory where two such CTAs fit on an SM, else it reads it again (out of L2).  Masses
+// A cluster of CTAs shares a row; each keeps its slice in shared memory where two such CTAs fit on an SM or each has one to itself, else it reads it again (out of L2).  Masses
 // are whole numbers (w 2^31, summed in 64 bits), so neither the order of the additions nor the cluster's size can move a border: results do
 // not depend on them.
 //   1. max l, and the largest entry of each block of 128: what follows reads the blocks again that hold entries it looks for.
@@ -1045,15 +1045,23 @@ PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float
     const int sms = pyre_sm_count();
     int C = cluster > 0 ? cluster : n_rows <= (top_p ? sms / 4 : sms / 12) ? MAX_CLUSTER : n_rows <= sms / 2 ? 4 : n_rows <= sms ? 2 : 1;
     while (!cluster && C > 1 && V <= 1024 * C) C /= 2;
-    FilterParams p = {logits, ld, temperature, seeds, token_index, top_k, top_p, min_p, out, V, (ceil_div(V, C) + 3) / 4 * 4, 0};
-    constexpr int RESIDENT = 77 * 1024;      // two CTAs on an SM
-    size_t bytes = (size_t)p.slice * 4 + 16;
-    p.resident = bytes <= RESIDENT;
-    if (!p.resident) bytes = 0;
+    // A slice stays in shared memory where two such CTAs fit on an SM (228 KB, 1 KB of it for each CTA: 17,700 entries a slice), or where each CTA
+    // has an SM to itself (19,700).  Slices between the two sizes are halved instead: 150 rows of 18,500 entries, k / p / rows of all kinds, 37 / 34 / 56 us on two
+    // CTAs, 47 / 43 / 66 on one that reads its row again, 39 / 42 / 55 on one that has the SM; 74 rows of 75,000 36 / 66 / 43 on eight, 29 / 60 / 44 on four that read it
+    // again, 38 / 80 / 52 on four that have an SM each.
+    constexpr int SM_BYTES = 233472, OWN_BYTES = (int)sizeof(FilterShared) + 1024;
+    constexpr int RESIDENT = (SM_BYTES / 2 - OWN_BYTES) / 16 * 16, RESIDENT_ALONE = 77 * 1024;
+    static_assert(RESIDENT > 0 && 2 * (RESIDENT + OWN_BYTES) <= SM_BYTES && RESIDENT_ALONE + OWN_BYTES <= SM_BYTES, "two CTAs, one CTA");
+    auto slice_of = [&](int ctas) { return (ceil_div(V, ctas) + 3) / 4 * 4; };
+    auto bytes_of = [&](int ctas) { return (long long)slice_of(ctas) * 4 + 16; };
+    if (!cluster && C < MAX_CLUSTER && (long long)n_rows * C > sms && bytes_of(C) > RESIDENT && bytes_of(C) <= RESIDENT_ALONE) C *= 2;
+    FilterParams p = {logits, ld, temperature, seeds, token_index, top_k, top_p, min_p, out, V, slice_of(C), 0};
+    p.resident = bytes_of(C) <= ((long long)n_rows * C <= sms ? RESIDENT_ALONE : RESIDENT);
+    const size_t bytes = p.resident ? (size_t)bytes_of(C) : 0;
     static bool configured[PYRE_MAX_DEVICES] = {};      // the attribute is per device
     bool& done = configured[pyre_current_device()];
     if (!done) {
-        cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RESIDENT);
+        cudaError_t e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RESIDENT_ALONE);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_filtered_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return (int)e;
         done = true;
