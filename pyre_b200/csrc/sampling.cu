@@ -1039,22 +1039,32 @@ PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float
     if (n_rows <= 0) return 0;
     if (V <= 0 || (temperature && (!seeds || !token_index))) return PYRE_ERR_BAD_ARG;
     if (cluster < 0 || cluster > MAX_CLUSTER || (cluster & (cluster - 1))) return PYRE_ERR_BAD_ARG;
-    // CTAs per row.  152,064 entries, us on 1 / 2 / 4 / 8 / 16 CTAs a row: 1 row, k 22 / 16 / 13 / 12 / 11; 12 rows, k 17 / 15 / 14 for 4 / 8 / 16, p alone
-    // 65 / 40 / 32; 16 rows, k 18 / 21 / 22, p 67 / 50 / 44; 32 rows, k 27 / 21 / 35 / 35 for 2 / 4 / 8 / 16, p 123 / 75 / 79 / 69, rows of all kinds
-    // 102 / 61 / 49 / 40; 64 rows, k 40 / 29 / 23 / 58 for 1 / 2 / 4 / 8, p 234 / 133 / 82 / 140; 256 rows, k 49 / 59 / 73 / 192, p 316 / 251 / 244 / 503.
-    const int sms = pyre_sm_count();
-    int C = cluster > 0 ? cluster : n_rows <= (top_p ? sms / 4 : sms / 12) ? MAX_CLUSTER : n_rows <= sms / 2 ? 4 : n_rows <= sms ? 2 : 1;
-    while (!cluster && C > 1 && V <= 1024 * C) C /= 2;
     // A slice stays in shared memory where two such CTAs fit on an SM (228 KB, 1 KB of it for each CTA: 17,700 entries a slice), or where each CTA
-    // has an SM to itself (19,700).  Slices between the two sizes are halved instead: 150 rows of 18,500 entries, k / p / rows of all kinds, 37 / 34 / 56 us on two
-    // CTAs, 47 / 43 / 66 on one that reads its row again, 39 / 42 / 55 on one that has the SM; 74 rows of 75,000 36 / 66 / 43 on eight, 29 / 60 / 44 on four that read it
-    // again, 38 / 80 / 52 on four that have an SM each.
+    // has an SM to itself (19,700).
     constexpr int SM_BYTES = 233472, OWN_BYTES = (int)sizeof(FilterShared) + 1024;
     constexpr int RESIDENT = (SM_BYTES / 2 - OWN_BYTES) / 16 * 16, RESIDENT_ALONE = 77 * 1024;
     static_assert(RESIDENT > 0 && 2 * (RESIDENT + OWN_BYTES) <= SM_BYTES && RESIDENT_ALONE + OWN_BYTES <= SM_BYTES, "two CTAs, one CTA");
     auto slice_of = [&](int ctas) { return (ceil_div(V, ctas) + 3) / 4 * 4; };
     auto bytes_of = [&](int ctas) { return (long long)slice_of(ctas) * 4 + 16; };
-    if (!cluster && C < MAX_CLUSTER && (long long)n_rows * C > sms && bytes_of(C) > RESIDENT && bytes_of(C) <= RESIDENT_ALONE) C *= 2;
+    // CTAs per row.  152,064 entries, us on 1 / 2 / 4 / 8 / 16 CTAs a row:
+    //   k            1 row 21 / 16 / 13 / 11 / 11, 12 rows 28 / 21 / 16 / 14 / 14, 16 30 / 22 / 18 / 21 / 21, 64 39 / 29 / 23 / 38 / 57, 100 40 / 30 / 37 / 52 / 84,
+    //                148 39 / 33 / 50 / 69 / 120, 200 45 / 54 / 57, 256 48 / 58 / 72; k and p 128 42 / 32 / 41, 256 48 / 58 / 73
+    //   p alone      1 134 / 75 / 45 / 29 / 22, 16 195 / 107 / 66 / 48 / 43, 28 - / - / 74 / 51 / 59, 37 220 / 120 / 78 / 64 / 74, 64 236 / 135 / 84 / 90 / 118,
+    //                100 254 / 149 / 116 / 131, 200 295 / 200 / 192 / 236, 256 313 / 242 / 232 / 294; of 65,536 entries 28 38 / 26 / 38 on 4 / 8 / 16, 256 139 / 117 / 126
+    //                on 1 / 2 / 4; of 24,000 256 56 / 54 / 69; of 16,000 (one CTA holds the row) 39 / 39, of 8,000 21 / 30
+    //   of all kinds 8 115 / 64 / 37 / 25 / 20, 32 179 / 100 / 59 / 42 / 40, 48 187 / 105 / 65 / 50 / 55, 100 210 / 122 / 82 / 81 / 102, 256 230 / 151 / 137 / 163
+    // (Rows of all kinds come with all three arrays, as rows with k and p do: they go by p where there are few and by k where there are more than SMs.)
+    // Slices between the two limits are halved: 150 rows of 18,500 entries, k / p / rows of all kinds, 37 / 34 / 56 us on two CTAs, 47 / 43 / 66 on one that reads its
+    // row again, 39 / 42 / 55 on one that has the SM; 74 rows of 75,000 36 / 66 / 43 on eight, 29 / 60 / 44 on four that read it again, 38 / 80 / 52 on four
+    // that have an SM each.  (Not those of eight: see 28 and 37 rows of p alone.)
+    const int sms = pyre_sm_count();
+    const bool mass_alone = top_p && !top_k;
+    int C = cluster > 0 ? cluster
+            : n_rows <= (mass_alone ? sms / 8 : top_p ? sms / 4 : sms / 12) ? MAX_CLUSTER
+            : mass_alone && n_rows <= sms / 4 ? 8
+            : n_rows <= sms / 2 ? 4 : n_rows <= sms || (mass_alone && bytes_of(1) > RESIDENT) ? 2 : 1;
+    while (!cluster && C > 1 && V <= 1024 * C) C /= 2;
+    if (!cluster && C <= 4 && (long long)n_rows * C > sms && bytes_of(C) > RESIDENT && bytes_of(C) <= RESIDENT_ALONE) C *= 2;
     FilterParams p = {logits, ld, temperature, seeds, token_index, top_k, top_p, min_p, out, V, slice_of(C), 0};
     p.resident = bytes_of(C) <= ((long long)n_rows * C <= sms ? RESIDENT_ALONE : RESIDENT);
     const size_t bytes = p.resident ? (size_t)bytes_of(C) : 0;
