@@ -33,6 +33,7 @@ struct W4Params {
     const __nv_bfloat16* scales;  // [G][N]
     void* out;                    // [M][N]
     int M, N, G;
+    int ahead;                    // the weight may be read before the kernels in front have ended: all that wrote it had ended before this launch
     int* err_flag;
 };
 
@@ -134,8 +135,9 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         if (lane == 0) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
-            const int early = min(steps, STREAM_STAGES);      // the weights depend on no earlier kernel
+            const int early = min(steps, STREAM_STAGES);
             int asked = 0;
+            if (!p.ahead) pdl_wait();
             auto weights = [&](int i) {
                 const int s = i % STREAM_STAGES;
                 mbar_expect_tx(full + 8 * s, L::STAGE);
@@ -160,6 +162,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         constexpr int BATCH = 4;
         static_assert(BATCH % PAIR == 0 && NT <= 4, "whole stages, a lane per token");
         bool waited = false;
+        if (!p.ahead) { pdl_wait(); waited = true; }
         for (int i0 = 0; i0 < n && ok; i0 += BATCH) {
             float v[BATCH][WARPS], x[BATCH];
 #pragma unroll
@@ -413,7 +416,7 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             for (int tile = blockIdx.x / C; tile < tiles && ok; tile += gridDim.x / C) {
                 place(tile);
                 for (int i = 0; i < n; ++i) {
-                    if (!waited && (rows || it == W_STAGES)) { pdl_wait(); waited = true; }      // (the weights depend on no earlier kernel)
+                    if (!waited && (rows || !p.ahead || it == W_STAGES)) { pdl_wait(); waited = true; }
                     const uint32_t s = it % stages;
                     if (!(ok = mbar_wait(empty + 8 * s, ((it / stages) & 1) ^ 1, abort_flag, p.err_flag))) break;
                     mbar_expect_tx(full + 8 * s, rows ? L::X_BYTES : W_BYTES);
@@ -503,7 +506,7 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             place(tile);
             for (int i = 0; i < n && ok; ++i, ++it) {
                 const int s = it % W_STAGES, sa = it % STAGES;
-                if (!waited && it >= min(W_STAGES, STAGES)) { pdl_wait(); waited = true; }      // from here on the copies and the MMAs have to run
+                if (!waited && (!p.ahead || it >= min(W_STAGES, STAGES))) { pdl_wait(); waited = true; }      // from here on the copies and the MMAs have to run
                 ok = mbar_wait(w_full + 8 * s, (it / W_STAGES) & 1, abort_flag, p.err_flag);
                 const uint32_t src = base + L::W_OFF + s * W_BYTES + row * 64;      // 64-byte swizzle: a chunk of 16 bytes by bits 7 and 8
                 uint32_t v[16], a[32];
@@ -748,7 +751,8 @@ constexpr int FEW = 32;
 // infinity or a NaN s = NaN.
 template <typename T>
 __global__ void w4_quantize_kernel(const T* w, long long ld, uint8_t* packed, __nv_bfloat16* scales, int N, int K) {
-    pdl_wait();      // no trigger: a product reads the weight ahead of its own wait, which is once all blocks here have ended
+    pdl_trigger();
+    pdl_wait();
     const int G = (K + GROUP - 1) / GROUP, lane = threadIdx.x & 31;
     const long long items = (long long)N * G, step = (long long)gridDim.x * (blockDim.x >> 5);
     for (long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); item < items; item += step) {
@@ -772,7 +776,6 @@ __global__ void w4_quantize_kernel(const T* w, long long ld, uint8_t* packed, __
         if ((lane & 1) == 0) reinterpret_cast<uint32_t*>(packed)[item * (GROUP / 8) + (lane >> 1)] = q | next << 4;
         if (lane == 0) scales[(size_t)g * N + n] = s;
     }
-    __threadfence();
 }
 
 template <typename T>
@@ -815,13 +818,14 @@ PYRE_API int pyre_w4_values(const void* packed, const void* scales, void* out, i
     return 0;
 }
 
-// rows [M][128 G] and packed [N][64 G] on 16-byte boundaries; out [M, N] of `dtype`
+// rows [M][128 G] and packed [N][64 G] on 16-byte boundaries; out [M, N] of `dtype`.  ahead: whatever wrote packed and scales had ended, waited for by the host, before
+// this call; the kernel then asks for them while the kernels in front of it still run.
 PYRE_API int pyre_w4_linear(const void* rows, const float* row_scales, long long ld_scales, const void* packed, const void* scales, void* out,
-                            int M, int N, int G, int dtype, int* err_flag, cudaStream_t stream) {
+                            int M, int N, int G, int dtype, int ahead, int* err_flag, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (G <= 0 || ((uintptr_t)rows & 15) || ((uintptr_t)packed & 15)) return PYRE_ERR_BAD_ARG;
     if (dtype != PYRE_F32 && dtype != PYRE_BF16) return PYRE_ERR_BAD_ARG;
-    const W4Params p = {(const uint8_t*)rows, row_scales, ld_scales, (const uint8_t*)packed, (const __nv_bfloat16*)scales, out, M, N, G, err_flag};
+    const W4Params p = {(const uint8_t*)rows, row_scales, ld_scales, (const uint8_t*)packed, (const __nv_bfloat16*)scales, out, M, N, G, ahead, err_flag};
     if (M <= FEW) return dtype == PYRE_F32 ? launch_few<float>(p, stream) : launch_few<__nv_bfloat16>(p, stream);
     // tiles of 64 tokens / 128, us: 64 x 3,584 x 37,888 24.8 / 34.3, 64 x 3,584 x 3,584 8.0 / 9.9; 128 x 3,584 x 37,888 44.9 / 34.9, 128 x 18,944 x 3,584 32.2 / 27.4
     if (M <= 64) return dtype == PYRE_F32 ? launch_many<64, float>(p, stream) : launch_many<64, __nv_bfloat16>(p, stream);

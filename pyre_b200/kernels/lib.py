@@ -93,7 +93,7 @@ SIGNATURES: dict[str, tuple[str, list]] = {
     "pyre_rows8_values": ("rows8", [P, P, LL, P, I, I, I, P]),
     "pyre_w4_quantize": ("gemm_w4", [P, LL, P, P, I, I, I, P]),
     "pyre_w4_values": ("gemm_w4", [P, P, P, I, I, I, P]),
-    "pyre_w4_linear": ("gemm_w4", [P, P, LL, P, P, P, I, I, I, I, P, P]),
+    "pyre_w4_linear": ("gemm_w4", [P, P, LL, P, P, P, I, I, I, I, I, P, P]),
 }
 
 #: functions that return a number of another type than int (sizes; see ``call_value``)

@@ -165,7 +165,10 @@ class Weight4:
     """A weight [N, K] in 4 bits with a bfloat16 scale per 128 neighbouring elements of a feature (csrc/gemm_w4.cu; ``quantize_weight4``):
     ``packed`` uint8 [N, 64 G], zeros beyond K, and ``scales`` [G, N] (G = ceil(K / 128)).  Of every four bytes, which hold eight elements,
     byte i holds element i in its lower half and element i + 4 in its upper one, two's complement -8 .. 7; an element stands for itself
-    times its group's scale."""
+    times its group's scale.
+
+    A product reads a weight when the kernels in front of it have ended, whatever wrote it.  One that is ``settle``d, as those that parts load are, it
+    reads ahead of them, as long as the tensors' version counters say that nothing has changed it since."""
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, width: int):
         groups, shape = -(-width // GROUP8), packed.shape
@@ -178,6 +181,19 @@ class Weight4:
         if packed.data_ptr() % 16:
             raise ValueError("packed must start on a 16-byte boundary")
         self.packed, self.scales, self.width = packed, scales, width
+        self._settled = None      # the tensors' versions when ``settle`` had waited
+
+    def settle(self) -> "Weight4":
+        """Wait for whatever writes the weight; from here on products read it ahead of the kernels in front of them (programmatic dependent
+        launch).  A change in place ends that until the next ``settle``; whoever writes to the memory past torch calls it again, or makes another ``Weight4``."""
+        torch.cuda.synchronize(self.device)
+        # (a tensor of inference mode has no version: its weight is not read ahead)
+        self._settled = None if self.packed.is_inference() or self.scales.is_inference() else (self.packed._version, self.scales._version)
+        return self
+
+    @property
+    def settled(self) -> bool:
+        return self._settled is not None and self._settled == (self.packed._version, self.scales._version)
 
     @property
     def shape(self):
@@ -481,7 +497,7 @@ def linear4(x: "torch.Tensor | Rows8", w: Weight4, out_dtype: "torch.dtype | Non
     dtype = torch.float32 if partials_ok else out_dtype or x.dtype
     out = torch.empty(T, N, dtype=dtype, device=rows.device)
     lib.call("pyre_w4_linear", rows.data_ptr(), scales.data_ptr(), scales.stride(0), packed.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
-             T, N, scales.shape[0], _dt(dtype), device_error_flag(rows.device).data_ptr(), _stream())
+             T, N, scales.shape[0], _dt(dtype), w.settled, device_error_flag(rows.device).data_ptr(), _stream())
     return PartialSums(out.unsqueeze(0), x.dtype) if partials_ok else out
 
 
@@ -1049,10 +1065,10 @@ def known_weight_bits(bits: "int | None") -> "int | None":
 
 
 def linear_weight(w: torch.Tensor, bits: "int | None" = None) -> "torch.Tensor | FixedWeight | Weight4":
-    """A weight as ``linear`` wants it: with ``bits`` 4 a ``Weight4``; else float32 matrices that the fixed-point product takes with their rows' exponents, others as
+    """A weight as ``linear`` wants it: with ``bits`` 4 a ``Weight4`` that is settled; else float32 matrices that the fixed-point product takes with their rows' exponents, others as
     they are; so are those of which more than one feature in 64 has no scale (an element far above the rest of its row)."""
     if bits == 4:
-        return quantize_weight4(w)
+        return quantize_weight4(w).settle()
     if not fixed_supported(w):
         return w
     with torch.cuda.device(w.device):
