@@ -155,8 +155,8 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                     tma_load_2d(base + s * L::STAGE + PAIR * W_BYTES + h * L::X_BYTES, &map_x, full + 8 * s, (first + PAIR * i + h) * GROUP, t0);
                 asked = i + 1;
             }
-            if (!ok)      // a wait ran out: the copies in flight end first
-                for (int i = max(0, asked - STREAM_STAGES); i < asked; ++i) mbar_drain(full + 8 * (i % STREAM_STAGES), (i / STREAM_STAGES) & 1);
+            // the copies end before the CTA does, also where a reader's wait ran out after this thread had asked for the last of them
+            for (int i = max(0, asked - STREAM_STAGES); i < asked; ++i) mbar_drain(full + 8 * (i % STREAM_STAGES), (i / STREAM_STAGES) & 1);
         }
     } else if (warp == 2 * WARPS + 1) {
         constexpr int BATCH = 4;
@@ -426,8 +426,8 @@ w4_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 }
             }
             if (!waited) pdl_wait();
-            if (!ok)      // a wait ran out: the copies in flight end first
-                for (uint32_t at = it > stages ? it - stages : 0; at < it; ++at) mbar_drain(full + 8 * (at % stages), (at / stages) & 1);
+            // the copies end before the CTA does, also where a reader's wait ran out after this thread had asked for the last of them
+            for (uint32_t at = it > stages ? it - stages : 0; at < it; ++at) mbar_drain(full + 8 * (at % stages), (at / stages) & 1);
         }
     } else if (warp == 1) {
         // D 32-bit integers (2 at bit 4), A and B signed bytes (1 at bits 7 and 10), N >> 3 at bit 17, M >> 4 at bit 24
