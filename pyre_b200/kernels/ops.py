@@ -426,12 +426,12 @@ def add_rmsnorm_rows8(x: torch.Tensor, delta: "torch.Tensor | PartialSums | Defe
     if delta is not None and delta.shape != (T, H):
         raise ValueError(f"delta shape {tuple(delta.shape)} != x shape {(T, H)}")
     parts, n_parts = None, 0
-    if isinstance(delta, torch.Tensor):
-        _check(delta, "delta", dtype, 2)
+    if isinstance(delta, DeferredProduct):
+        delta = delta.partials()
+    if isinstance(delta, PartialSums):
+        parts, n_parts, delta = delta.parts, delta.n, None
     elif delta is not None:
-        if isinstance(delta, DeferredProduct):
-            delta = delta.partials()
-        parts, n_parts, delta = (delta.parts, delta.n, None) if isinstance(delta, PartialSums) else (None, 0, delta)
+        _check(delta, "delta", dtype, 2)
     n_rows = T
     if rows is not None:
         _check(rows, "rows", torch.int32, 1)
