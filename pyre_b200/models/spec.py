@@ -81,16 +81,18 @@ class ModelSpec:
 
 def with_weight_bits(spec: ModelSpec, bits: "int | None") -> ModelSpec:
     """The same model with the products of its blocks' mixers and feed-forwards held in ``bits`` bits.  A model with a mixer or
-    feed-forward that has no such form is refused as a whole: some of its layers in 4 bits is not what was asked for."""
+    feed-forward that has no such form is refused as a whole: some of its layers in 4 bits is not what was asked for.  So is one with a
+    block that names neither (an arrangement of its own, whose products would stay as they are without a word)."""
     if bits is None:
         return spec
 
     def of(block: PartSpec) -> PartSpec:
         params = dict(block.params)
-        for role in ("mixer", "ffn"):
-            part = params.get(role)
-            if part is None:
-                continue
+        roles = [role for role in ("mixer", "ffn") if params.get(role) is not None]
+        if not roles:
+            raise ValueError(f"weights in {bits} bits: the block {block.kind!r} of this architecture has neither a mixer nor a feed-forward")
+        for role in roles:
+            part = params[role]
             if not takes_weight_bits(role, part.kind):
                 raise ValueError(f"weights in {bits} bits: the {role} part {part.kind!r} of this architecture has none")
             params[role] = PartSpec(part.kind, {**part.params, "weight_bits": bits})
