@@ -46,8 +46,8 @@ class Sampler:
         else:
             seeds = np.asarray([p.seed & 0x7FFFFFFFFFFFFFFF for p in params], dtype=np.int64)
             # only the filters that some row has: the kernel has less to look for
-            drawn = [p for p in params if p.temperature > 0.0]
-            filters = [name for name, off in (("top_k", 0), ("top_p", 1.0), ("min_p", 0.0)) if any(getattr(p, name) != off for p in drawn)]
+            filtered = [p for p in params if p.filters]
+            filters = [name for name, off in (("top_k", 0), ("top_p", 1.0), ("min_p", 0.0)) if any(getattr(p, name) != off for p in filtered)]
             small = np.empty((2 + len(filters), R), dtype=np.int32)
             small[0] = np.asarray([p.temperature for p in params], dtype=np.float32).view(np.int32)
             small[1] = np.asarray(token_index, dtype=np.int32)
