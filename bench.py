@@ -1321,7 +1321,8 @@ def run_gugidra(args) -> dict:
 def run_sweep(args) -> dict:
     """Decode throughput over a grid of batch sizes and context lengths and prefill throughput over
     several portion lengths on the 7B shape, each with its fraction of the roofline (device-timed,
-    the same way as the headline numbers).  One JSON object; not part of the one-line contract."""
+    the same way as the headline numbers); ``--weight-bits 4``: with the layers' projections in 4 bits (the roofline of
+    the decode steps counts their bytes then).  One JSON object; not part of the one-line contract."""
     import numpy as np
     import torch
 
@@ -1340,9 +1341,16 @@ def run_sweep(args) -> dict:
     grid = [(1, 512), (1, 8192), (1, 32768), (8, 512), (8, 2048), (8, 8192), (8, 32768), (32, 2048), (64, 512), (64, 2048),
             (64, 8192), (128, 2048)]
     biggest = max(b * (c + SETTLE_STEPS + 64) for b, c in grid)
-    eng = Engine(config=cfg, seed=0, dtype="bfloat16", page_size=PAGE_SIZE, max_cache_tokens=biggest + 8192,
+    if args.weight_bits is not None:
+        # what the bf16 model reads of the projections, in 4 bits with a bf16 scale per 128 elements
+        h, inter, d = cfg_raw["hidden_size"], cfg_raw["intermediate_size"], cfg.head_dim
+        sizes = [((cfg_raw["num_attention_heads"] + 2 * cfg_raw["num_key_value_heads"]) * d, h), (h, cfg_raw["num_attention_heads"] * d), (2 * inter, h), (h, inter)]
+        weight_bytes -= layers * sum(n * (2 * k - (64 + 2) * -(-k // 128)) for n, k in sizes)
+    held = torch.cuda.memory_allocated()
+    eng = Engine(config=cfg, seed=0, dtype="bfloat16", weight_bits=args.weight_bits, page_size=PAGE_SIZE, max_cache_tokens=biggest + 8192,
                  max_num_seqs=128, max_num_batched_tokens=8192, prefill_chunk=8192, max_model_len=40960)
     st, cache = eng.stepper, eng.cache
+    held = torch.cuda.memory_allocated() - held
     rng = np.random.default_rng(0)
     vocab = cfg.vocab_size
 
@@ -1395,7 +1403,8 @@ def run_sweep(args) -> dict:
                         "flops_frac": round(flops(T, start, 1) / (ms * 1e-3) / (peaks["bf16_tflops"] * 1e12), 3)})
     cache.check()
     st.check_device_errors()
-    return {"workload": "sweep", "layers": layers, "peaks": peaks, "decode": decode, "prefill": prefill}
+    return {"workload": "sweep", "layers": layers, "weight_bits": args.weight_bits, "weight_gb_per_step": round(weight_bytes / 1e9, 2),
+            "held_gb": round(held / 1e9, 2), "cache_tokens": biggest + 8192, "peaks": peaks, "decode": decode, "prefill": prefill}
 
 
 def environment() -> dict:
@@ -1446,12 +1455,15 @@ def main() -> int:
                          "portion lengths on the 7B shape, the Modovik or the Pivinex design beside the Qwen2.5 decoder at "
                          "equal layer sizes, the Tekarax design beside the closest layers of those two, the Nipudra design beside the closest "
                          "layers of Tekarax and Modovik, the Gadopel design beside the closest layers of Pivinex and Tekarax, or the Gugidra design beside the closest layers of Tekarax and Modovik, instead (prints its own JSON line)")
+    ap.add_argument("--weight-bits", type=int, choices=[4], default=None, help="sweep: hold the layers' projections in 4 bits (EngineConfig.weight_bits)")
     ap.add_argument("--cache-fraction", type=float, default=1.0,
                     help="serve14b: cache capacity as a fraction of what all requests need at once (< 1 forces preemption)")
     args = ap.parse_args()
     if args.gpus != 1:
         print(f"bench.py measures a single-GPU engine: --gpus {args.gpus} is not supported, run with --gpus 1")
         return 2
+    if args.weight_bits is not None and args.workload != "sweep":
+        ap.error("--weight-bits goes with --workload sweep")
     if args.workload:
         result = run_sweep(args) if args.workload == "sweep" else run_modovik(args) if args.workload == "modovik" else \
             run_pivinex(args) if args.workload == "pivinex" else run_tekarax(args) if args.workload == "tekarax" else run_nipudra(args) if args.workload == "nipudra" else \
