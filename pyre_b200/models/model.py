@@ -133,6 +133,10 @@ class Model:
             # the block has packed what it needs; drop the originals of this layer
             for name in [n for n in tensors if n.startswith(prefix)]:
                 del tensors[name]
+            # ... and where they are larger than what was packed, their memory: the next layer's small weights would settle in it piece by
+            # piece, and the cache, whose size may go by what is free, could not have it
+            if self.device.type == "cuda" and any(getattr(p, "weight_bits", None) for p in b.children().values()):
+                torch.cuda.empty_cache()
         load_part(self.tail, tensors, self.spec.tail_prefix)
         self.vectors = {name: tensors[name] for name in self.spec.vectors}
         self.loaded = True
