@@ -7,9 +7,12 @@
 // makes it sixteen times as large and spares the sign's extension), the outer ones in float: by ascending group in each of a CTA's sets of warps
 // (one, or two that take the stages in turn), then over the sets and over the CTAs that share a tile's K, in order.
 //
-// Bound: up to some 24 rows the weights' bytes (1 x 3,584 x 37,888 in 13.9 us, 4.9 TB/s of packed weights; 8 x 5,120 x 27,648 15.6), above them each group's
-// conversion and scaling, two operations or three for every sum of 128 products, beside the matrix instructions, which take an eighth to a third of the
-// time (2,048 x 3,584 x 37,888 in 483 us).  Below 10 us what a launch takes to start and to meet shows (1 x 3,584 x 4,608: 4.8 us, its bytes 1.3).
+// Bound: up to eight rows the weights' bytes (1 x 3,584 x 37,888 in 13.3 us, 5.1 TB/s of packed weights; 8 x 5,120 x 27,648 14.8).  From there to 64 rows no unit of
+// an SM is near its limit (24 x 5,120 x 27,648 17.2 us: issue slots 43 %, DRAM 39, tensor pipe 32, ALU 29; 64 x 3,584 x 37,888 24.0): the warps wait, on each other's
+// stages by the look of it.  Above, each group's conversion and scaling, two operations or three for every sum of 128 products, beside the matrix instructions,
+// which take a quarter of the time (2,048 x 3,584 x 37,888 in 483 to 509 us, by the GPU and how long it has been at it).  Below 10 us what a launch takes to
+// start and to meet shows (1 x 3,584 x 4,608: 4.7 us, its bytes 1.3).  A weight that is not settled (read after the kernels in front) takes a microsecond
+// more: 1 x 3,584 x 4,608 5.8, 24 x 5,120 x 27,648 18.7, 8 x 18,944 x 3,584 12.5 against 11.8.
 #include <cooperative_groups.h>
 
 #include "tensor_core.cuh"
@@ -269,7 +272,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 //   warps 8 to the last: a thread owns a feature and 32 of the tokens.  The group's integers come out of tensor memory, are scaled by token and by
 //                        feature and added to float sums in registers, by ascending group.
 // Where there are few tiles the CTAs of a cluster share a tile's K, and their sums meet in shared memory.
-// Bound by the last warps: of 483 us for 2,048 x 3,584 x 37,888 some 200 go with the conversions, products and additions (with a quarter of them it takes 349), 48 with
+// Bound by the last warps: of 483 us (on the fastest GPU, as all figures here) for 2,048 x 3,584 x 37,888 some 200 go with the conversions, products and additions (with a quarter of them it takes 349), 48 with
 // the reads of the tokens' scales; a quarter of the MMAs or no unpacking changes nothing.  Four warps for 128 tokens took 574 us, eight 550, sixteen 506 (then the
 // tiles' copies); a third accumulator 514; sums by the MMAs' own fragments (half as many reads of scales) 508.
 // ---------------------------------------------------------------------------

@@ -179,7 +179,8 @@ PYRE_API int pyre_sample(const float* logits, long long ld, const float* tempera
 //
 // A cluster of CTAs shares a row; each keeps its slice in shared memory where two such CTAs fit on an SM or each has one to itself, else it reads it again (out of L2).  Masses
 // are whole numbers (w 2^31, summed in 64 bits), so neither the order of the additions nor the cluster's size can move a border: results do
-// not depend on them.
+// not depend on them.  A token's mass is off by half a unit, beside what its exponential is (see mass_of): the mass before a border by 2^-32 of the
+// best token's per token at most (152,064 tokens: 3.5e-5 of it, where all are cut off alike; some 5e-8 where they differ).
 //   1. max l, and the largest entry of each block of 128: what follows reads the blocks again that hold entries it looks for.
 //   2. k: as many blocks as k have an entry of at least t, where t is the k-th of their largest ones (or somewhat below): no token below t is among the first
 //      k.  The tokens from t on, hardly more than k, go to the first CTA's list, and the other CTAs are done.  It ranks them by (l, index), which
@@ -1046,12 +1047,13 @@ PYRE_API int pyre_sample_filtered(const float* logits, long long ld, const float
     static_assert(RESIDENT > 0 && 2 * (RESIDENT + OWN_BYTES) <= SM_BYTES && RESIDENT_ALONE + OWN_BYTES <= SM_BYTES, "two CTAs, one CTA");
     auto slice_of = [&](int ctas) { return (ceil_div(V, ctas) + 3) / 4 * 4; };
     auto bytes_of = [&](int ctas) { return (long long)slice_of(ctas) * 4 + 16; };
-    // CTAs per row.  152,064 entries, us on 1 / 2 / 4 / 8 / 16 CTAs a row:
+    // CTAs per row.  152,064 entries, p, m, k and the temperature drawn for each row, us on 1 / 2 / 4 / 8 / 16 CTAs a row:
     //   k            1 row 21 / 16 / 13 / 11 / 11, 12 rows 28 / 21 / 16 / 14 / 14, 16 30 / 22 / 18 / 21 / 21, 64 39 / 29 / 23 / 38 / 57, 100 40 / 30 / 37 / 52 / 84,
     //                148 39 / 33 / 50 / 69 / 120, 200 45 / 54 / 57, 256 48 / 58 / 72; k and p 128 42 / 32 / 41, 256 48 / 58 / 73
     //   p alone      1 134 / 75 / 45 / 29 / 22, 16 195 / 107 / 66 / 48 / 43, 28 - / - / 74 / 51 / 59, 37 220 / 120 / 78 / 64 / 74, 64 236 / 135 / 84 / 90 / 118,
     //                100 254 / 149 / 116 / 131, 200 295 / 200 / 192 / 236, 256 313 / 242 / 232 / 294; of 65,536 entries 28 38 / 26 / 38 on 4 / 8 / 16, 256 139 / 117 / 126
-    //                on 1 / 2 / 4; of 24,000 256 56 / 54 / 69; of 16,000 (one CTA holds the row) 39 / 39, of 8,000 21 / 30
+    //                on 1 / 2 / 4; of 24,000 256 56 / 54 / 69; of 16,000 (one CTA holds the row) 39 / 39, of 8,000 21 / 30.  (What two CTAs gain on 256 rows is the rows'
+    //                difference: where all keep 30,000 tokens they take 243 on one or two, 90,000 339.)
     //   of all kinds 8 115 / 64 / 37 / 25 / 20, 32 179 / 100 / 59 / 42 / 40, 48 187 / 105 / 65 / 50 / 55, 100 210 / 122 / 82 / 81 / 102, 256 230 / 151 / 137 / 163
     // (Rows of all kinds come with all three arrays, as rows with k and p do: they go by p where there are few and by k where there are more than SMs.)
     // Slices between the two limits are halved: 150 rows of 18,500 entries, k / p / rows of all kinds, 37 / 34 / 56 us on two CTAs, 47 / 43 / 66 on one that reads its

@@ -629,7 +629,8 @@ def sample(logits: torch.Tensor, temperature: "torch.Tensor | None" = None, seed
     Where temperature is not 0, ``top_k`` (int32 [R], 0 = off), ``top_p`` (float32 [R], 1 = off) and ``min_p`` (float32 [R], 0 = off) leave
     a row's likeliest tokens to choose from, in the order of the logits (the lower index first where they are equal): the first k; of
     those the shortest run from the best on with at least p of their mass; of those the ones with at least min_p of the best
-    one's probability.  The best one always stays.  A row without any of them gets the same token with and without the arguments; a NaN counts as -inf."""
+    one's probability.  The best one always stays.  Masses are whole multiples of 2^-31 of the best one's: those before a border are off by 2^-32 of it
+    per token at most.  A row without any of them gets the same token with and without the arguments; a NaN counts as -inf, with or without them."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda or logits.stride(1) != 1:
         raise ValueError("logits must be a CUDA float32 matrix with contiguous rows")
     R, V = logits.shape
