@@ -181,19 +181,22 @@ class Weight4:
         if packed.data_ptr() % 16:
             raise ValueError("packed must start on a 16-byte boundary")
         self.packed, self.scales, self.width = packed, scales, width
-        self._settled = None      # the tensors' versions when ``settle`` had waited
+        self._settled = None      # the tensors and their versions when ``settle`` had waited
 
     def settle(self) -> "Weight4":
         """Wait for whatever writes the weight; from here on products read it ahead of the kernels in front of them (programmatic dependent
-        launch).  A change in place ends that until the next ``settle``; whoever writes to the memory past torch calls it again, or makes another ``Weight4``."""
+        launch).  A change in place ends that until the next ``settle``; whoever writes to the memory past the version counters (by ``.data`` or raw
+        pointers) calls it again before the next product, or makes another ``Weight4``."""
         torch.cuda.synchronize(self.device)
+        packed, scales = self.packed, self.scales
         # (a tensor of inference mode has no version: its weight is not read ahead)
-        self._settled = None if self.packed.is_inference() or self.scales.is_inference() else (self.packed._version, self.scales._version)
+        self._settled = None if packed.is_inference() or scales.is_inference() else (packed, packed._version, scales, scales._version)
         return self
 
     @property
     def settled(self) -> bool:
-        return self._settled is not None and self._settled == (self.packed._version, self.scales._version)
+        s = self._settled
+        return s is not None and s[0] is self.packed and s[1] == s[0]._version and s[2] is self.scales and s[3] == s[2]._version
 
     @property
     def shape(self):

@@ -46,6 +46,13 @@ def test_which_weights_are_read_ahead(read_ahead):
         change()
         assert not given.settled and not ahead(given) and not ahead(given)
         assert ahead(given.settle())
+    with torch.inference_mode():      # of ordinary tensors: their versions count
+        given.scales.mul_(1)
+    assert not ahead(given)
+    for name in ("packed", "scales"):      # other tensors in the same handle
+        given.settle()
+        setattr(given, name, getattr(given, name).clone())
+        assert not ahead(given)
     other = ops.Weight4(given.packed, given.scales, 512)      # the same memory, with a handle of its own
     assert not ahead(other)
     with torch.inference_mode():
